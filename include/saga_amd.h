@@ -53,6 +53,7 @@ extern "C" {
 #define SAGA_DTYPE_BOOL 3 /* one byte, 0 or 1; masks only */
 #define SAGA_DTYPE_I32 4
 #define SAGA_DTYPE_I64 5
+#define SAGA_DTYPE_U8 6 /* bytes of two 4-bit codes, the first in the low half */
 
 #define SAGA_OK 0
 #define SAGA_ERR_INVALID (-1)     /* null pointer, bad shape/stride/dtype */
@@ -407,6 +408,85 @@ int saga_argmax(const saga_tensor* x, int64_t* out, void* workspace, size_t work
 int saga_prefill_attention(const saga_tensor* query, const saga_tensor* key, const saga_tensor* value,
                            const saga_tensor* mask, float scale, int32_t causal, int64_t causal_offset,
                            saga_tensor* out, saga_stream_t stream);
+
+/* ---- data held in 4 bits ---- */
+
+/* A group of consecutive values is held as codes c of 4 bits, one scale s and
+ * one offset z in f16: value = s * c + z.  What the library quantises takes
+ * z = the largest f16 <= the group's minimum, s = the smallest f16 >=
+ * (maximum - z) / 15 and c = (value - z) / s rounded to the nearest (ties to
+ * even), so that a value is off by at most s / 2.  A group that holds a NaN, an
+ * infinity or a magnitude above 65504 is stored as s = z = NaN: it reads back
+ * as NaN.
+ *
+ * A key / value cache of Lmax positions, groups along the head dim d (64 or
+ * 128), all groups of one size (32 or 64) in k and v:
+ *   codes  U8  [B, heads, Lmax, d / 2], innermost stride 1, rows 16-byte aligned
+ *   scales F16 [B, heads, Lmax, 2 * d / group]: (s, z) of each group, innermost
+ *          stride 1, rows aligned to 4 * d / group bytes
+ * Nibbles of a code row: keys have dim 32 j + 8 s + e (s < 4, e < 8) in nibble
+ * 8 (s * d / 32 + j) + e; values have dim 16 e + c (c < 16) in nibble
+ * c * d / 16 + e.  Rows of any strides (batch rows and heads may overlap for
+ * reading). */
+typedef struct saga_kv_q4 {
+  saga_tensor k_codes, k_scales, v_codes, v_scales;
+} saga_kv_q4;
+
+/* saga_rope_kv_append into a 4-bit cache: the rotated keys and the values are
+ * quantised from fp32 and written at [batch[n], :, pos[n]] (batch == NULL: token
+ * n is batch row n).  qkv [N, >= (n_q + n_k + n_v) * d] (bf16, f16 or f32), n_k
+ * and n_v the cache's heads.  rope_table: the tokens' rotations as
+ * saga_rope_table writes them (required; 16-byte aligned).  q_out [N, n_q, d] of
+ * qkv's type receives the rotated queries.  A pos or batch index out of range
+ * writes no cache row and NaN queries.  The (batch, pos) of a call's tokens must
+ * differ from each other. */
+int saga_rope_kv_append_q4(const saga_tensor* qkv, int64_t n_q, const float* rope_table, const int32_t* pos,
+                           const int32_t* batch, saga_tensor* q_out, const saga_kv_q4* cache,
+                           saga_stream_t stream);
+
+/* Rows of a 4-bit cache as values: k [N, n_k, d] and v [N, n_v, d] (one type,
+ * bf16, f16 or f32; unit innermost stride) of the positions [batch[n], :, pos[n]]
+ * (batch == NULL: row n), for a prompt's attention over what is held.  An index
+ * out of range gives NaN. */
+int saga_kv_q4_read(const saga_kv_q4* cache, const int32_t* pos, const int32_t* batch, saga_tensor* k,
+                    saga_tensor* v, saga_stream_t stream);
+
+/* saga_dense_decode over a 4-bit cache: query [b, q_h, 1, d] bf16 or f16, b and
+ * the heads of the cache's, L its positions; mask, kv_len, scale and out as
+ * there.  Any number of query heads per key head.  Scores, softmax and sums in
+ * fp32; a softmax weight enters the second product with 16 bits. */
+size_t saga_dense_q4_workspace_bytes(int64_t b, int64_t q_h, int64_t L, int64_t d);
+int saga_dense_decode_q4(const saga_tensor* query, const saga_kv_q4* cache, const saga_tensor* mask,
+                         const int32_t* kv_len, float scale, saga_tensor* out, void* workspace,
+                         size_t workspace_bytes, saga_stream_t stream);
+
+/* A projection weight [N, K] in 4 bits, groups of 32, 64 or 128 along K (K a
+ * multiple of the group and N of 16):
+ *   codes  U8  [N / 16, ceil(K / 128), 1024], contiguous, 16-byte aligned
+ *   scales F16 [N / 16, K / group, 16, 2], contiguous: (s, z) of row 16 t + r
+ * Unit [t][j] holds 16 rows x 128 columns as 64 lanes of 16 bytes: word i of lane
+ * 16 q + r is row 16 t + r at columns 128 j + 32 i + 8 q + (0, 2, 4, 6, 1, 3, 5, 7),
+ * nibble by nibble (codes past K are not read as values). */
+typedef struct saga_q4_weight {
+  saga_tensor codes, scales;
+} saga_q4_weight;
+
+/* saga_gemv for a weight in 4 bits: x [M <= 32, K] bf16, the same epilogues,
+ * bias and fused RMSNorm.  Products with the codes are exact, sums in fp32.
+ * workspace: as saga_gemv's, of saga_gemv_q4_workspace_bytes(M, N, K) bytes (the
+ * size may be 0; without it results are equal to rounding). */
+size_t saga_gemv_q4_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int saga_gemv_q4(const saga_tensor* x, const saga_q4_weight* w, const saga_tensor* bias, float rms_eps,
+                 int32_t epilogue, saga_tensor* y, void* workspace, size_t workspace_bytes, saga_stream_t stream);
+
+/* saga_unpack_gemv for weights in 4 bits: n (1 to SAGA_UNPACK_MAX) weights to
+ * row-major bf16 out [N, K] in one launch, rows reordered as there. */
+typedef struct saga_unpack_q4_item {
+  saga_q4_weight w;
+  saga_tensor out;
+  int64_t rot_heads, head_rows;
+} saga_unpack_q4_item;
+int saga_unpack_gemv_q4(const saga_unpack_q4_item* items, int32_t n, saga_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsaga_amd.so")
 
-DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_BOOL, DTYPE_I32, DTYPE_I64 = range(6)
+DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_BOOL, DTYPE_I32, DTYPE_I64, DTYPE_U8 = range(7)
 _TORCH_DTYPES = {
     torch.float32: DTYPE_F32,
     torch.bfloat16: DTYPE_BF16,
@@ -24,6 +24,7 @@ _TORCH_DTYPES = {
     torch.bool: DTYPE_BOOL,
     torch.int32: DTYPE_I32,
     torch.int64: DTYPE_I64,
+    torch.uint8: DTYPE_U8,
 }
 
 SAGA_OK = 0
@@ -49,6 +50,18 @@ assert struct.calcsize("=Qii4q4q") == ctypes.sizeof(SagaTensor)
 
 class UnpackItem(ctypes.Structure):
     _fields_ = [("w", SagaTensor), ("out", SagaTensor), ("rot_heads", ctypes.c_int64), ("head_rows", ctypes.c_int64)]
+
+
+class KvQ4(ctypes.Structure):
+    _fields_ = [("k_codes", SagaTensor), ("k_scales", SagaTensor), ("v_codes", SagaTensor), ("v_scales", SagaTensor)]
+
+
+class Q4Weight(ctypes.Structure):
+    _fields_ = [("codes", SagaTensor), ("scales", SagaTensor)]
+
+
+class UnpackQ4Item(ctypes.Structure):
+    _fields_ = [("w", Q4Weight), ("out", SagaTensor), ("rot_heads", ctypes.c_int64), ("head_rows", ctypes.c_int64)]
 
 
 class AtopnLayout(ctypes.Structure):
@@ -97,6 +110,15 @@ _SIGS = {
     "saga_argmax_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
     "saga_argmax": (ctypes.c_int, [_T, _P, _P, ctypes.c_size_t, _P]),
     "saga_prefill_attention": (ctypes.c_int, [_T, _T, _T, _T, ctypes.c_float, ctypes.c_int32, ctypes.c_int64, _T, _P]),
+    "saga_rope_kv_append_q4": (ctypes.c_int, [_T, _I64, _P, _P, _P, _T, ctypes.POINTER(KvQ4), _P]),
+    "saga_kv_q4_read": (ctypes.c_int, [ctypes.POINTER(KvQ4), _P, _P, _T, _T, _P]),
+    "saga_dense_q4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64]),
+    "saga_dense_decode_q4": (ctypes.c_int, [_T, ctypes.POINTER(KvQ4), _T, _P, ctypes.c_float, _T, _P, ctypes.c_size_t,
+                                            _P]),
+    "saga_gemv_q4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
+    "saga_gemv_q4": (ctypes.c_int, [_T, ctypes.POINTER(Q4Weight), _T, ctypes.c_float, ctypes.c_int32, _T, _P,
+                                    ctypes.c_size_t, _P]),
+    "saga_unpack_gemv_q4": (ctypes.c_int, [ctypes.POINTER(UnpackQ4Item), ctypes.c_int32, _P]),
 }
 GEMV_STORE, GEMV_ADD, GEMV_SILU_PAIRS = 0, 1, 2
 K2_AUTO, K2_ROW_BLOCK, K2_SLICE_ROW = 0, 1, 2
@@ -139,16 +161,25 @@ def dtype_code(dt: torch.dtype) -> int:
         raise TypeError(f"saga_amd: unsupported dtype {dt}") from None
 
 
-def descriptor(t: torch.Tensor) -> SagaTensor:
-    """saga_tensor descriptor of a torch tensor."""
+def _packed(t: torch.Tensor) -> bytes:
     if t.dim() > 4:
         raise ValueError("saga_amd: at most 4 dims")
     n = t.dim()
     if n == 4:
-        return SagaTensor.from_buffer_copy(_PACK(t.data_ptr(), dtype_code(t.dtype), 4, *t.shape, *t.stride()))
+        return _PACK(t.data_ptr(), dtype_code(t.dtype), 4, *t.shape, *t.stride())
     pad = (0,) * (4 - max(n, 1))
     shape, stride = (tuple(t.shape), t.stride()) if n else ((1,), (1,))
-    return SagaTensor.from_buffer_copy(_PACK(t.data_ptr(), dtype_code(t.dtype), max(n, 1), *shape, *pad, *stride, *pad))
+    return _PACK(t.data_ptr(), dtype_code(t.dtype), max(n, 1), *shape, *pad, *stride, *pad)
+
+
+def descriptor(t: torch.Tensor) -> SagaTensor:
+    """saga_tensor descriptor of a torch tensor."""
+    return SagaTensor.from_buffer_copy(_packed(t))
+
+
+def descriptors(kind, *ts: torch.Tensor):
+    """A structure of saga_tensor descriptors (KvQ4, Q4Weight)."""
+    return kind.from_buffer_copy(b"".join(map(_packed, ts)))
 
 
 def tensor(t: torch.Tensor | None):

@@ -49,6 +49,7 @@ int64_t elt_size(int dt) {
     case SAGA_DTYPE_BOOL: return 1;
     case SAGA_DTYPE_I32: return 4;
     case SAGA_DTYPE_I64: return 8;
+    case SAGA_DTYPE_U8: return 1;
     default: return 0;
   }
 }
@@ -1137,6 +1138,311 @@ int saga_prefill_attention(const saga_tensor* query, const saga_tensor* key, con
   if ((rc = hip_status(launch_prefill_attention(dt, static_cast<int>(d), p, static_cast<hipStream_t>(stream)),
                        "prefill launch")))
     return rc;
+  return ok();
+}
+
+}  // extern "C"
+
+namespace {
+
+// One kind (codes + scales) of a 4-bit cache: shapes, types and the alignment of its rows.
+int check_kv_q4_kind(const saga_tensor* codes, const saga_tensor* scales, const char* name, int64_t* heads) {
+  int rc;
+  if ((rc = check_tensor(codes, name, 4)) || (rc = check_tensor(scales, name, 4))) return rc;
+  if (codes->dtype != SAGA_DTYPE_U8 || scales->dtype != SAGA_DTYPE_F16)
+    return fail(SAGA_ERR_INVALID, "%s: codes must be u8 and scales f16", name);
+  for (int i = 0; i < 3; ++i)
+    if (codes->shape[i] != scales->shape[i])
+      return fail(SAGA_ERR_INVALID, "%s: codes [B, heads, Lmax, d / 2] and scales [B, heads, Lmax, 2 d / group] differ", name);
+  if ((rc = check_vec_rows(codes, name))) return rc;
+  const int64_t row = scales->shape[3] * 2;  // bytes: 4, 8 or 16 once the group is known to be 32 or 64
+  if (scales->stride[3] != 1 || reinterpret_cast<uintptr_t>(scales->data) % row)
+    return fail(SAGA_ERR_INVALID, "%s: scales need a unit innermost stride and rows aligned to their size", name);
+  for (int i = 0; i < 3; ++i)
+    if (scales->shape[i] > 1 && scales->stride[i] * 2 % row)
+      return fail(SAGA_ERR_INVALID, "%s: scales need a unit innermost stride and rows aligned to their size", name);
+  *heads = codes->shape[1];
+  return SAGA_OK;
+}
+
+int check_kv_q4(const saga_kv_q4* c, KvQ4& kv) {
+  if (!c) return fail(SAGA_ERR_INVALID, "cache: null");
+  int rc;
+  int64_t n_k, n_v;
+  const saga_tensor &kc = c->k_codes, &ks = c->k_scales, &vc = c->v_codes, &vs = c->v_scales;
+  if ((rc = check_kv_q4_kind(&kc, &ks, "key cache", &n_k)) || (rc = check_kv_q4_kind(&vc, &vs, "value cache", &n_v)))
+    return rc;
+  if (kc.shape[0] != vc.shape[0] || kc.shape[2] != vc.shape[2] || kc.shape[3] != vc.shape[3] ||
+      ks.shape[3] != vs.shape[3])
+    return fail(SAGA_ERR_INVALID, "cache: keys and values differ in batch, positions, head dim or group");
+  const int64_t d = kc.shape[3] * 2;
+  if (d != 64 && d != 128) return fail(SAGA_ERR_UNSUPPORTED, "cache: head_dim %lld not built (64, 128)", (long long)d);
+  const int64_t ng2 = ks.shape[3];
+  if (ng2 != 2 * d / 32 && ng2 != 2 * d / 64)
+    return fail(SAGA_ERR_UNSUPPORTED, "cache: groups of 32 or 64 dims, scales [B, heads, Lmax, 2 d / group] required");
+  if (kc.shape[2] >= kMaxLen || n_k > 65535 || n_v > 65535) return fail(SAGA_ERR_UNSUPPORTED, "cache: sizes too large");
+  kv = KvQ4{};
+  kv.kc = static_cast<const char*>(kc.data);
+  kv.kc_sb = kc.stride[0], kv.kc_sh = kc.stride[1], kv.kc_sl = kc.stride[2];
+  kv.ks = static_cast<const char*>(ks.data);
+  kv.ks_sb = 2 * ks.stride[0], kv.ks_sh = 2 * ks.stride[1], kv.ks_sl = 2 * ks.stride[2];
+  kv.vc = static_cast<const char*>(vc.data);
+  kv.vc_sb = vc.stride[0], kv.vc_sh = vc.stride[1], kv.vc_sl = vc.stride[2];
+  kv.vs = static_cast<const char*>(vs.data);
+  kv.vs_sb = 2 * vs.stride[0], kv.vs_sh = 2 * vs.stride[1], kv.vs_sl = 2 * vs.stride[2];
+  kv.B = static_cast<int32_t>(kc.shape[0]);
+  kv.n_k = static_cast<int32_t>(n_k);
+  kv.n_v = static_cast<int32_t>(n_v);
+  kv.Lmax = static_cast<int32_t>(kc.shape[2]);
+  kv.d = static_cast<int32_t>(d);
+  kv.group = static_cast<int32_t>(2 * d / ng2);
+  return SAGA_OK;
+}
+
+// 16-byte vectors of 8 elements of a 16-bit type at multiples of 8 elements.
+bool vec8(const saga_tensor* t) {
+  return elt_size(t->dtype) == 2 && reinterpret_cast<uintptr_t>(t->data) % 16 == 0 && t->stride[0] % 8 == 0 &&
+         (t->ndim < 3 || t->stride[1] % 8 == 0);
+}
+
+// A 4-bit weight [N, K] of saga_gemv_q4 / saga_unpack_gemv_q4.
+int check_q4_weight(const saga_q4_weight* w, int64_t K, int64_t* N, int64_t* group) {
+  int rc;
+  if (!w) return fail(SAGA_ERR_INVALID, "w: null");
+  const saga_tensor &c = w->codes, &z = w->scales;
+  if ((rc = check_tensor(&c, "w codes", 3)) || (rc = check_tensor(&z, "w scales", 4))) return rc;
+  if (c.dtype != SAGA_DTYPE_U8 || z.dtype != SAGA_DTYPE_F16)
+    return fail(SAGA_ERR_INVALID, "w: codes must be u8 and scales f16");
+  if (c.shape[2] != 1024 || c.shape[1] != (K + 127) / 128 || c.stride[2] != 1 ||
+      (c.shape[1] > 1 && c.stride[1] != 1024) || (c.shape[0] > 1 && c.stride[0] != c.shape[1] * 1024))
+    return fail(SAGA_ERR_INVALID, "w: codes must be contiguous [N / 16, ceil(K / 128), 1024]");
+  if (z.shape[0] != c.shape[0] || z.shape[2] != 16 || z.shape[3] != 2 || z.stride[3] != 1 || z.stride[2] != 2 ||
+      (z.shape[1] > 1 && z.stride[1] != 32) || (z.shape[0] > 1 && z.stride[0] != z.shape[1] * 32))
+    return fail(SAGA_ERR_INVALID, "w: scales must be contiguous [N / 16, K / group, 16, 2]");
+  if (reinterpret_cast<uintptr_t>(c.data) % 16 || reinterpret_cast<uintptr_t>(z.data) % 16)
+    return fail(SAGA_ERR_INVALID, "w: codes and scales must be 16-byte aligned");
+  if (K % z.shape[1]) return fail(SAGA_ERR_INVALID, "w: K must be a multiple of the group");
+  *group = K / z.shape[1];
+  if (*group != 32 && *group != 64 && *group != 128)
+    return fail(SAGA_ERR_UNSUPPORTED, "w: groups of %lld columns not built (32, 64, 128)", (long long)*group);
+  *N = c.shape[0] * 16;
+  if (K >= (1LL << 30) || *N >= (1LL << 27)) return fail(SAGA_ERR_UNSUPPORTED, "w: sizes too large");
+  return SAGA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int saga_rope_kv_append_q4(const saga_tensor* qkv, int64_t n_q, const float* rope_table, const int32_t* pos,
+                           const int32_t* batch, saga_tensor* q_out, const saga_kv_q4* cache, saga_stream_t stream) {
+  int rc;
+  RopeQ4Params p{};
+  if ((rc = check_tensor(qkv, "qkv", 2)) || (rc = check_tensor(q_out, "q_out", 3)) || (rc = check_kv_q4(cache, p.kv)))
+    return rc;
+  if (!is_float(qkv->dtype) || q_out->dtype != qkv->dtype)
+    return fail(SAGA_ERR_INVALID, "qkv and q_out must share one float dtype");
+  if (!pos || !rope_table) return fail(SAGA_ERR_INVALID, "pos or rope_table: null");
+  if (reinterpret_cast<uintptr_t>(rope_table) % 16) return fail(SAGA_ERR_INVALID, "rope_table must be 16-byte aligned");
+  const int64_t N = qkv->shape[0], d = p.kv.d;
+  if (n_q < 1 || n_q > 65535) return fail(SAGA_ERR_INVALID, "n_q: 1 to 65535 required");
+  if (q_out->shape[0] != N || q_out->shape[1] != n_q || q_out->shape[2] != d)
+    return fail(SAGA_ERR_INVALID, "q_out: shape must be [N, n_q, d]");
+  const int64_t heads = n_q + p.kv.n_k + p.kv.n_v;
+  if (qkv->shape[1] < heads * d) return fail(SAGA_ERR_INVALID, "qkv: row shorter than (n_q + n_k + n_v) * d");
+  if (qkv->stride[1] != 1 || q_out->stride[2] != 1) return fail(SAGA_ERR_INVALID, "innermost strides must be 1");
+  if (!batch && N > p.kv.B) return fail(SAGA_ERR_INVALID, "without batch indices N must be <= B");
+  if (N * heads * (d / 8) >= (1LL << 32) - 256) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  p.qkv = qkv->data;
+  p.qkv_ld = qkv->stride[0];
+  p.q_out = q_out->data;
+  p.q_sn = q_out->stride[0];
+  p.q_sh = q_out->stride[1];
+  p.dt = qkv->dtype;
+  p.N = static_cast<int32_t>(N);
+  p.n_q = static_cast<int32_t>(n_q);
+  p.vec = vec8(qkv) && vec8(q_out);
+  p.table = rope_table;
+  p.pos = pos;
+  p.batch = batch;
+  if ((rc = hip_status(launch_rope_kv_append_q4(p, static_cast<hipStream_t>(stream)), "rope_kv_append_q4 launch")))
+    return rc;
+  return ok();
+}
+
+int saga_kv_q4_read(const saga_kv_q4* cache, const int32_t* pos, const int32_t* batch, saga_tensor* k, saga_tensor* v,
+                    saga_stream_t stream) {
+  int rc;
+  KvQ4ReadParams p{};
+  if ((rc = check_kv_q4(cache, p.kv)) || (rc = check_tensor(k, "k", 3)) || (rc = check_tensor(v, "v", 3))) return rc;
+  if (!pos) return fail(SAGA_ERR_INVALID, "pos: null");
+  if (!is_float(k->dtype) || v->dtype != k->dtype) return fail(SAGA_ERR_INVALID, "k and v must share one float dtype");
+  const int64_t N = k->shape[0], d = p.kv.d;
+  if (k->shape[1] != p.kv.n_k || k->shape[2] != d || v->shape[0] != N || v->shape[1] != p.kv.n_v || v->shape[2] != d)
+    return fail(SAGA_ERR_INVALID, "k and v: shapes must be [N, n_k, d] and [N, n_v, d]");
+  if (k->stride[2] != 1 || v->stride[2] != 1) return fail(SAGA_ERR_INVALID, "innermost strides must be 1");
+  if (!batch && N > p.kv.B) return fail(SAGA_ERR_INVALID, "without batch indices N must be <= B");
+  if (N * (p.kv.n_k + p.kv.n_v) * (d / 8) >= (1LL << 32) - 256) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  p.pos = pos;
+  p.batch = batch;
+  p.k = k->data;
+  p.k_sn = k->stride[0];
+  p.k_sh = k->stride[1];
+  p.v = v->data;
+  p.v_sn = v->stride[0];
+  p.v_sh = v->stride[1];
+  p.dt = k->dtype;
+  p.N = static_cast<int32_t>(N);
+  p.vec = vec8(k) && vec8(v);
+  if ((rc = hip_status(launch_kv_q4_read(p, static_cast<hipStream_t>(stream)), "kv_q4_read launch"))) return rc;
+  return ok();
+}
+
+size_t saga_dense_q4_workspace_bytes(int64_t b, int64_t q_h, int64_t L, int64_t d) {
+  if (b < 1 || q_h < 1 || L < 1 || L >= kMaxLen || d < 1 || d > 1024 || b > (1LL << 22) / q_h) return 0;
+  int64_t ns, sl;
+  dense_q4_plan(b, L, &ns, &sl);
+  return static_cast<size_t>(align256(b * q_h * ns * (2 + d) * 4));
+}
+
+int saga_dense_decode_q4(const saga_tensor* query, const saga_kv_q4* cache, const saga_tensor* mask,
+                         const int32_t* kv_len, float scale, saga_tensor* out, void* workspace, size_t workspace_bytes,
+                         saga_stream_t stream) {
+  int rc;
+  DenseQ4Params p{};
+  if ((rc = check_tensor(query, "query", 4)) || (rc = check_kv_q4(cache, p.kv))) return rc;
+  Shape s{};
+  s.b = query->shape[0];
+  s.q_h = query->shape[1];
+  s.d = query->shape[3];
+  s.L = p.kv.Lmax;
+  if (query->shape[2] != 1)
+    return fail(SAGA_ERR_UNSUPPORTED, "query: decode path needs l_q == 1, got %lld", (long long)query->shape[2]);
+  if (query->dtype != SAGA_DTYPE_BF16 && query->dtype != SAGA_DTYPE_F16)
+    return fail(SAGA_ERR_UNSUPPORTED, "query: dtype must be bf16 or f16");
+  if (p.kv.B != s.b || p.kv.d != s.d) return fail(SAGA_ERR_INVALID, "cache: batch or head dim differs from the query's");
+  if (s.q_h % p.kv.n_k) return fail(SAGA_ERR_INVALID, "q_h (%lld) not a multiple of k_h (%d)", (long long)s.q_h, p.kv.n_k);
+  if (s.q_h % p.kv.n_v) return fail(SAGA_ERR_INVALID, "q_h (%lld) not a multiple of v_h (%d)", (long long)s.q_h, p.kv.n_v);
+  if (s.q_h > (1LL << 22) || s.b * s.q_h >= (1LL << 22)) return fail(SAGA_ERR_UNSUPPORTED, "b * q_h too large");
+  if ((rc = check_vec_rows(query, "query")) || (rc = check_out(out, s))) return rc;
+  if (mask) {
+    if ((rc = check_tensor(mask, "mask", 4))) return rc;
+    if (!is_float(mask->dtype) && mask->dtype != SAGA_DTYPE_BOOL)
+      return fail(SAGA_ERR_INVALID, "mask: dtype must be f32, bf16, f16 or bool");
+    if ((mask->shape[0] != 1 && mask->shape[0] != s.b) || (mask->shape[1] != 1 && mask->shape[1] != s.q_h) ||
+        mask->shape[2] != 1 || mask->shape[3] < s.L)
+      return fail(SAGA_ERR_INVALID, "mask: shape does not broadcast to [b, q_h, 1, L=%lld]", (long long)s.L);
+    p.mask = mask->data;
+    p.mask_dt = mask->dtype;
+    p.m_sb = mask->shape[0] == 1 ? 0 : mask->stride[0];
+    p.m_sh = mask->shape[1] == 1 ? 0 : mask->stride[1];
+    p.m_sl = mask->stride[3];
+  }
+  int64_t ns, sl;
+  dense_q4_plan(s.b, s.L, &ns, &sl);
+  const size_t need = static_cast<size_t>(s.b * s.q_h * ns * (2 + s.d) * 4);
+  if (ns > 1 && (!workspace || workspace_bytes < need))
+    return fail(SAGA_ERR_WORKSPACE, "workspace of %zu bytes, need %zu", workspace_bytes, need);
+  if (ns > 1 && reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(SAGA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  p.q = static_cast<const char*>(query->data);
+  p.q_sb = query->stride[0];
+  p.q_sh = query->stride[1];
+  p.q_dt = query->dtype;
+  p.kv_len = kv_len;
+  p.b = static_cast<int32_t>(s.b);
+  p.q_h = static_cast<int32_t>(s.q_h);
+  p.L = static_cast<int32_t>(s.L);
+  p.g = static_cast<int32_t>(s.q_h / p.kv.n_k);
+  p.g_v = static_cast<int32_t>(s.q_h / p.kv.n_v);
+  p.scale = scale;
+  p.out = out->data;
+  p.out_dt = out->dtype;
+  p.o_sb = out->stride[0];
+  p.o_sh = out->stride[1];
+  p.part = static_cast<float*>(workspace);
+  p.nsplit = static_cast<int32_t>(ns);
+  p.split_len = static_cast<int32_t>(sl);
+  if ((rc = hip_status(launch_dense_decode_q4(p, static_cast<hipStream_t>(stream)), "dense_decode_q4 launch"))) return rc;
+  return ok();
+}
+
+size_t saga_gemv_q4_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || M > 32 || N < 16 || K < 32 || N >= (1LL << 27) || K >= (1LL << 30)) return 0;
+  return static_cast<size_t>(gemv_q4_workspace_bytes(M, N, K));
+}
+
+int saga_gemv_q4(const saga_tensor* x, const saga_q4_weight* w, const saga_tensor* bias, float rms_eps,
+                 int32_t epilogue, saga_tensor* y, void* workspace, size_t workspace_bytes, saga_stream_t stream) {
+  int rc;
+  int64_t N, group;
+  if ((rc = check_tensor(x, "x", 2))) return rc;
+  const int64_t M = x->shape[0], K = x->shape[1];
+  if ((rc = check_q4_weight(w, K, &N, &group)) || (rc = check_tensor(y, "y", 2))) return rc;
+  if (x->dtype != SAGA_DTYPE_BF16 || y->dtype != SAGA_DTYPE_BF16) return fail(SAGA_ERR_UNSUPPORTED, "gemv_q4: bf16 only");
+  if (M > 32) return fail(SAGA_ERR_UNSUPPORTED, "gemv_q4: at most 32 rows");
+  if ((rc = check_vec_rows(x, "x"))) return rc;
+  if (epilogue != SAGA_GEMV_STORE && epilogue != SAGA_GEMV_ADD && epilogue != SAGA_GEMV_SILU_PAIRS)
+    return fail(SAGA_ERR_INVALID, "gemv_q4: unknown epilogue %d", epilogue);
+  const int64_t ny = epilogue == SAGA_GEMV_SILU_PAIRS ? N / 2 : N;
+  if (y->shape[0] != M || y->shape[1] != ny) return fail(SAGA_ERR_INVALID, "gemv_q4: y must be [M, %lld]", (long long)ny);
+  if (y->stride[1] != 1) return fail(SAGA_ERR_INVALID, "y: innermost stride must be 1");
+  if (bias) {
+    if (epilogue == SAGA_GEMV_SILU_PAIRS) return fail(SAGA_ERR_UNSUPPORTED, "bias with SILU_PAIRS");
+    if ((rc = check_tensor(bias, "bias", 1))) return rc;
+    if (bias->dtype != SAGA_DTYPE_BF16 || bias->shape[0] != N || bias->stride[0] != 1)
+      return fail(SAGA_ERR_INVALID, "bias must be bf16 [N]");
+  }
+  GemvQ4Params p{};
+  p.x = x->data;
+  p.x_ld = x->stride[0];
+  p.codes = w->codes.data;
+  p.scales = w->scales.data;
+  p.bias = bias ? bias->data : nullptr;
+  p.y = y->data;
+  p.y_ld = y->stride[0];
+  p.M = static_cast<int32_t>(M);
+  p.N = static_cast<int32_t>(N);
+  p.K = static_cast<int32_t>(K);
+  p.group = static_cast<int32_t>(group);
+  p.rms = rms_eps >= 0.f;
+  p.eps = rms_eps;
+  p.epilogue = epilogue;
+  const int64_t need = gemv_q4_workspace_bytes(M, N, K);
+  void* ws = workspace && need > 0 && workspace_bytes >= static_cast<size_t>(need) ? workspace : nullptr;
+  if (ws && reinterpret_cast<uintptr_t>(ws) % 256) return fail(SAGA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  if ((rc = hip_status(launch_gemv_q4(p, ws, static_cast<hipStream_t>(stream)), "gemv_q4 launch"))) return rc;
+  return ok();
+}
+
+int saga_unpack_gemv_q4(const saga_unpack_q4_item* items, int32_t n, saga_stream_t stream) {
+  if (!items || n < 1 || n > SAGA_UNPACK_MAX)
+    return fail(SAGA_ERR_INVALID, "unpack_q4: 1 to %d items required", SAGA_UNPACK_MAX);
+  UnpackQ4Params p{};
+  p.n = n;
+  int rc;
+  for (int32_t i = 0; i < n; ++i) {
+    const saga_unpack_q4_item& it = items[i];
+    int64_t N, group;
+    if ((rc = check_tensor(&it.out, "out", 2)) || (rc = check_q4_weight(&it.w, it.out.shape[1], &N, &group))) return rc;
+    if (it.out.dtype != SAGA_DTYPE_BF16) return fail(SAGA_ERR_UNSUPPORTED, "unpack_q4: bf16 only");
+    if (it.out.shape[0] != N) return fail(SAGA_ERR_INVALID, "unpack_q4: out must be [N, K] of w");
+    if ((rc = check_vec_rows(&it.out, "out"))) return rc;
+    if (it.rot_heads < 0 || it.head_rows < 0 ||
+        (it.head_rows > 0 && (it.head_rows % 2 || N % it.head_rows || it.rot_heads > N / it.head_rows)))
+      return fail(SAGA_ERR_INVALID, "unpack_q4: head_rows must be even and divide N, rot_heads at most N / head_rows");
+    UnpackQ4Params::Item& d = p.item[i];
+    d.codes = it.w.codes.data;
+    d.scales = it.w.scales.data;
+    d.dst = it.out.data;
+    d.dst_ld = it.out.stride[0];
+    d.N = static_cast<int32_t>(N);
+    d.K = static_cast<int32_t>(it.out.shape[1]);
+    d.group = static_cast<int32_t>(group);
+    d.rot_heads = static_cast<int32_t>(it.rot_heads);
+    d.head_rows = static_cast<int32_t>(it.head_rows);
+  }
+  if ((rc = hip_status(launch_unpack_q4(p, static_cast<hipStream_t>(stream)), "unpack_q4 launch"))) return rc;
   return ok();
 }
 

@@ -324,4 +324,85 @@ PrefillShape prefill_shape(int64_t b, int64_t q_h, int64_t Lq, int64_t keys, int
 int64_t prefill_query_blocks(const PrefillShape& shape, int64_t Lq);
 hipError_t launch_prefill_attention(int dtype, int d, const PrefillParams& p, hipStream_t st);
 
+// ---- data held in 4 bits (layouts: include/saga_amd.h) ----
+
+// A 4-bit cache: pointers, and strides in bytes (batch row, head, position).
+struct KvQ4 {
+  const char *kc, *ks, *vc, *vs;
+  int64_t kc_sb, kc_sh, kc_sl, ks_sb, ks_sh, ks_sl, vc_sb, vc_sh, vc_sl, vs_sb, vs_sh, vs_sl;
+  int32_t B, n_k, n_v, Lmax, d, group;
+};
+
+struct RopeQ4Params {
+  KvQ4 kv;
+  const void* qkv;
+  int64_t qkv_ld;
+  void* q_out;
+  int64_t q_sn, q_sh;
+  int32_t dt, N, n_q, vec;  // vec: qkv and q_out rows allow 16-byte vectors
+  const float* table;
+  const int32_t *pos, *batch;
+};
+hipError_t launch_rope_kv_append_q4(const RopeQ4Params& p, hipStream_t st);
+
+struct KvQ4ReadParams {
+  KvQ4 kv;
+  const int32_t *pos, *batch;
+  void *k, *v;
+  int64_t k_sn, k_sh, v_sn, v_sh;
+  int32_t dt, N, vec;
+};
+hipError_t launch_kv_q4_read(const KvQ4ReadParams& p, hipStream_t st);
+
+struct DenseQ4Params {
+  KvQ4 kv;
+  const char* q;
+  int64_t q_sb, q_sh;  // elements
+  int32_t q_dt;
+  const void* mask;
+  int32_t mask_dt;
+  int64_t m_sb, m_sh, m_sl;
+  const int32_t* kv_len;
+  int32_t b, q_h, L;
+  int32_t g, g_v;  // query heads per key head and per value head
+  int32_t nseg;    // blocks of query heads per batch row (set at launch)
+  float scale;
+  void* out;
+  int32_t out_dt;
+  int64_t o_sb, o_sh;
+  float* part;  // [b * q_h][nsplit][2 + d]
+  int32_t nsplit, split_len;
+};
+void dense_q4_plan(int64_t b, int64_t L, int64_t* nsplit, int64_t* split_len);
+hipError_t launch_dense_decode_q4(DenseQ4Params& p, hipStream_t st);
+
+struct GemvQ4Params {
+  const void* x;  // bf16 [M, K]
+  int64_t x_ld;
+  const void* codes;
+  const void* scales;
+  const void* bias;
+  void* y;
+  int64_t y_ld;
+  int32_t M, N, K, group;
+  int32_t rms;
+  float eps;
+  int32_t epilogue;
+};
+int64_t gemv_q4_workspace_bytes(int64_t M, int64_t N, int64_t K);
+hipError_t launch_gemv_q4(const GemvQ4Params& p, void* ws, hipStream_t st);
+
+struct UnpackQ4Params {
+  struct Item {
+    const void* codes;
+    const void* scales;
+    void* dst;
+    int64_t dst_ld;
+    int32_t N, K, group, rot_heads, head_rows;
+    int32_t block0;  // first block (set by the launcher)
+  } item[kUnpackMax];
+  int32_t n;
+};
+hipError_t launch_unpack_q4(UnpackQ4Params& p, hipStream_t st);
+
 }  // namespace saga

@@ -19,7 +19,7 @@ because the graph still holds its address; any other is freed at once.
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -676,4 +676,161 @@ def argmax_rows(x, out=None, workspace=None):
     ws = _take_workspace(workspace, x.device, "argmax", need) if need else None
     _lib.check(lib.saga_argmax(_lib.tensor(x), _lib.ptr(out), _lib.ptr(ws), ws.numel() if ws is not None else 0,
                                _lib.stream_of(x)), "argmax")
+    return out
+
+
+# ------------------------------------------------------- data held in 4 bits
+
+class Q4Weight(NamedTuple):
+    """A projection weight [N, K] in 4 bits (quantize_gemv_weight): codes uint8 [N/16, ceil(K/128), 1024] and
+    scales f16 [N/16, K/group, 16, 2], the (s, z) of value = s * code + z (layouts: include/saga_amd.h)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    group: int
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.codes.shape[0] * 16, self.scales.shape[1] * self.group
+
+
+class KVQ4(NamedTuple):
+    """A layer's 4-bit key / value cache: codes uint8 [B, heads, Lmax, d/2] and scales f16 [B, heads, Lmax,
+    2*d/group], the (s, z) of value = s * code + z per group of 32 or 64 dims (layouts: include/saga_amd.h)."""
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def _f16_down(x: torch.Tensor) -> torch.Tensor:
+    """The largest f16 that is at most x."""
+    h = x.to(torch.float16)
+    bits = h.view(torch.int16)
+    under = torch.where(bits > 0, bits - 1, torch.where(bits == 0, torch.full_like(bits, -32767), bits + 1))
+    return torch.where(h.float() > x, under, bits).view(torch.float16)
+
+
+def quantize_gemv_weight(w: torch.Tensor, group: int = 64) -> Q4Weight:
+    """W [N, K] in 4 bits for gemv_q4: per row and group of columns, codes c, an offset z (the largest f16 not above
+    the group's minimum) and a scale s (the smallest f16 that lets z + 15 s reach its maximum), every weight within
+    s / 2 of s * c + z.  N % 16 == 0, K a multiple of the group (32, 64 or 128)."""
+    if w.dim() != 2 or group not in (32, 64, 128) or w.shape[0] % 16 or w.shape[1] % group or not w.numel():
+        raise ValueError(f"saga_amd: 4-bit weights need [N, K] with N % 16 == 0 and K a multiple of the group "
+                         f"(32, 64 or 128), got {tuple(w.shape)} and {group}")
+    n, k = w.shape
+    x = w.float().reshape(n, k // group, group)
+    lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
+    if not bool((torch.maximum(lo.abs(), hi.abs()) <= 65504).all()):
+        raise ValueError("saga_amd: weights must be finite and at most 65504 in magnitude")
+    z = _f16_down(lo)
+    s = -_f16_down((z.float() - hi) / torch.full_like(hi, 15.0))
+    c = torch.round((x - z.float()) / torch.where(s == 0, torch.ones_like(s), s).float()).clamp_(0, 15)
+    c = torch.nn.functional.pad(c.to(torch.uint8).reshape(n, k), (0, -k % 128))
+    c = c.reshape(n // 16, 16, -1, 4, 4, 4, 2)  # tile, row, unit, word, lane group, pair, half
+    c = c.permute(0, 2, 4, 1, 3, 6, 5).reshape(n // 16, -1, 1024, 2)
+    scales = torch.cat([s, z], -1).reshape(n // 16, 16, k // group, 2).transpose(1, 2).contiguous()
+    return Q4Weight(c[..., 0] | (c[..., 1] << 4), scales, group)
+
+
+def _q4_weight(w: Q4Weight):
+    return _lib.descriptors(_lib.Q4Weight, w.codes, w.scales)
+
+
+def _check_group(w: Q4Weight, K: int) -> None:
+    if w.scales.shape[1] * w.group != K:
+        raise ValueError(f"saga_amd: a 4-bit weight of {w.scales.shape[1]} groups of {w.group} columns does not meet "
+                         f"{K} columns")
+
+
+def gemv_q4(x, w: Q4Weight, bias=None, rms_eps=None, epilogue="store", out=None, split_k=True, workspace=None):
+    """gemv for a weight in 4 bits (x [M <= 32, K] bf16): the same epilogues, bias and fused RMSNorm."""
+    _need_gpu(x, w.codes, w.scales, bias, out)
+    code = {"store": _lib.GEMV_STORE, "add": _lib.GEMV_ADD, "silu_pairs": _lib.GEMV_SILU_PAIRS}[epilogue]
+    M, N = x.shape[0], w.codes.shape[0] * 16
+    _check_group(w, x.shape[1])
+    if out is None:
+        if code == _lib.GEMV_ADD:
+            raise ValueError("saga_amd: epilogue 'add' needs out")
+        out = torch.empty(M, N // 2 if code == _lib.GEMV_SILU_PAIRS else N, dtype=x.dtype, device=x.device)
+    lib = _lib.load()
+    need = lib.saga_gemv_q4_workspace_bytes(M, N, x.shape[1]) if split_k else 0
+    ws = _take_workspace(workspace, x.device, "gemv_q4", need) if need else None
+    _lib.check(lib.saga_gemv_q4(_lib.tensor(x), _q4_weight(w), _lib.tensor(bias),
+                                -1.0 if rms_eps is None else float(rms_eps), code, _lib.tensor(out), _lib.ptr(ws),
+                                ws.numel() if ws is not None else 0, _lib.stream_of(x)), "gemv_q4")
+    return out
+
+
+def unpack_gemv_q4(weights, heads=None):
+    """Row-major bf16 [N, K] of weights in 4 bits, all in one launch; heads: as unpack_gemv_weights takes them."""
+    dev = _need_gpu(*(t for w in weights for t in w[:2]))
+    outs, items = [], []
+    for w, h in zip(weights, heads or [None] * len(weights)):
+        out = torch.empty(w.shape, dtype=torch.bfloat16, device=dev)
+        rot, rows = h if h is not None else (0, 0)
+        items.append(_lib.UnpackQ4Item(_q4_weight(w), _lib.descriptor(out), rot, rows))
+        outs.append(out)
+    _lib.check(_lib.load().saga_unpack_gemv_q4((_lib.UnpackQ4Item * len(items))(*items), len(items),
+                                               _lib.stream_of(outs[0])), "unpack_gemv_q4")
+    return outs
+
+
+def _indices(pos, batch, n: int) -> None:
+    for t, name in ((pos, "pos"), (batch, "batch")):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.shape != (n,)):
+            raise ValueError(f"saga_amd: {name} must be a contiguous int32 [{n}] tensor")
+
+
+def _kv_q4(cache: KVQ4):
+    return _lib.descriptors(_lib.KvQ4, *cache)
+
+
+def rope_kv_append_q4(qkv, n_q, rope_table, pos, cache: KVQ4, batch=None, q_out=None):
+    """rope_kv_append into a 4-bit cache: the new tokens' rotated keys and their values are quantised and written at
+    [batch, :, pos] (batch None: token n is batch row n), each pair (batch, pos) at most once per call.
+    qkv [N, (n_q+n_k+n_v)*d]; rope_table: rope_table(pos, d, theta) of these tokens.  Returns q_out [N, n_q, d]."""
+    dev = _need_gpu(qkv, rope_table, pos, batch, q_out, *cache)
+    n, d = qkv.shape[0], cache.k_codes.shape[-1] * 2
+    _indices(pos, batch, n)
+    if rope_table.dtype != torch.float32 or not rope_table.is_contiguous() or tuple(rope_table.shape) != (n, d // 2, 2):
+        raise ValueError("saga_amd: rope_table must be a contiguous float32 [N, d/2, 2] tensor")
+    if q_out is None:
+        q_out = torch.empty(n, n_q, d, dtype=qkv.dtype, device=dev)
+    _lib.check(_lib.load().saga_rope_kv_append_q4(_lib.tensor(qkv), n_q, _lib.ptr(rope_table), _lib.ptr(pos),
+                                                  _lib.ptr(batch), _lib.tensor(q_out), _kv_q4(cache),
+                                                  _lib.stream_of(qkv)), "rope_kv_append_q4")
+    return q_out
+
+
+def read_kv_q4(cache: KVQ4, pos, batch=None, dtype=torch.bfloat16):
+    """What a 4-bit cache holds at [batch, :, pos] (batch None: row n): k [N, n_k, d] and v [N, n_v, d] of `dtype`,
+    NaN where an index is out of range.  Transposed to [1, heads, N, d] they are prefill_attention's operands."""
+    dev = _need_gpu(pos, batch, *cache)
+    _indices(pos, batch, pos.shape[0])
+    d = cache.k_codes.shape[-1] * 2
+    k, v = (torch.empty(pos.shape[0], t.shape[1], d, dtype=dtype, device=dev) for t in (cache.k_codes, cache.v_codes))
+    _lib.check(_lib.load().saga_kv_q4_read(_kv_q4(cache), _lib.ptr(pos), _lib.ptr(batch), _lib.tensor(k),
+                                           _lib.tensor(v), _lib.stream_of(pos)), "read_kv_q4")
+    return k, v
+
+
+def dense_decode_q4(query, cache: KVQ4, attention_mask=None, scaling=None, kv_len=None, out=None, out_dtype=None,
+                    workspace=None):
+    """dense_decode over a 4-bit cache (query bf16 or f16 [b, q_h, 1, d])."""
+    dev = _need_gpu(query, attention_mask, kv_len, out, *cache)
+    query = _vec_ready(query)
+    b, q_h, l_q, d = query.shape
+    if l_q != 1:
+        raise NotImplementedError("saga_amd: the HIP decode kernels take l_q == 1")
+    L = cache.k_codes.shape[2]
+    mask = _mask_view(attention_mask, L)
+    if kv_len is not None and kv_len.shape != (b,):
+        raise ValueError("saga_amd: kv_len must be a contiguous int32 tensor [b]")
+    if out is None:
+        out = torch.empty(b, q_h, 1, d, dtype=out_dtype or query.dtype, device=dev)
+    lib = _lib.load()
+    ws = _take_workspace(workspace, dev, "dense_q4", lib.saga_dense_q4_workspace_bytes(b, q_h, L, d))
+    _lib.check(lib.saga_dense_decode_q4(_lib.tensor(query), _kv_q4(cache), _lib.tensor(mask), _lib.ptr(_kv_len(kv_len)),
+                                        _scale(query, scaling), _lib.tensor(out), _lib.ptr(ws), ws.numel(),
+                                        _lib.stream_of(query)), "dense_decode_q4")
     return out
