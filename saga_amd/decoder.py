@@ -17,6 +17,10 @@ projection accumulated into the residual stream.  Projections use the
 saga_amd skinny GEMM (batch <= 32; hipBLASLt otherwise), the LM head is
 followed by a row argmax kernel.  Positions advance on the device, so one
 captured graph serves every step.
+
+kv_bits=4 holds the caches in 4 bits (dense attention over them; RoPE and the
+quantising append are a launch of their own) and weight_bits=4 the decode
+projections and the LM head (opened layer by layer for a prompt's GEMMs).
 """
 from __future__ import annotations
 
@@ -90,14 +94,26 @@ class SagaDecoder:
     weights are released after packing unless keep_source_weights: the
     prefill then unpacks one layer's weights at a time.  k2_variant picks the
     fast step's selection + softmax.V kernels (ops.atopn_decode).
+    kv_bits 4 (mode "dense"): caches in 4 bits, groups of kv_group dims; a
+    prompt attends over what its cache holds.  weight_bits 4 (bf16, batch at
+    most 32): the projections and the LM head in 4 bits, groups of
+    weight_group columns, in prompts too; the embedding stays as it is.
     """
 
     def __init__(self, shape: DecoderShape, batch: int, max_len: int, mode: str = "atopn", top_n: int = 512,
                  exempt_layers=(), device="cuda", dtype=torch.bfloat16, seed: int = 0, fuse_rope: bool = True,
                  pack_weights: bool = True, weights: Optional[dict] = None, keep_source_weights: bool = False,
-                 k2_variant: int = 0):
+                 k2_variant: int = 0, kv_bits: int = 16, kv_group: int = 64, weight_bits: int = 16,
+                 weight_group: int = 64):
         if mode not in ("atopn", "dense", "vanilla"):
             raise ValueError(f"mode must be 'atopn', 'dense' or 'vanilla', got {mode!r}")
+        if kv_bits not in (4, 16) or weight_bits not in (4, 16):
+            raise ValueError(f"kv_bits and weight_bits must be 16 or 4, got {kv_bits} and {weight_bits}")
+        if kv_bits == 4 and (mode != "dense" or dtype not in (torch.bfloat16, torch.float16)):
+            raise ValueError("kv_bits=4 needs mode 'dense' and bf16 or f16")
+        if weight_bits == 4 and weight_group not in (32, 64, 128):
+            raise ValueError(f"weight_group must be 32, 64 or 128, got {weight_group}")
+        self.kv_bits, self.weight_bits, self.weight_group = kv_bits, weight_bits, weight_group
         self.shape, self.batch, self.max_len, self.mode, self.top_n = shape, batch, max_len, mode, top_n
         self.exempt = set(exempt_layers)
         self.device, self.dtype = torch.device(device), dtype
@@ -122,7 +138,7 @@ class SagaDecoder:
             self.w_d = [w(s.hidden, s.intermediate) for _ in range(s.layers)]
             self.ln_f = torch.ones(s.hidden, device=self.device, dtype=dtype)
         # separate key-head and value-head caches [layer][batch, heads, max_len, d]
-        self.kv = KVCache(s, batch, max_len, self.device, dtype)
+        self.kv = KVCache(s, batch, max_len, self.device, dtype, bits=kv_bits, group=kv_group)
         self.k_cache, self.v_cache = self.kv.k, self.kv.v
         # Atop-N threshold table, rows = batch * n_q (attention/attention.py:92-99)
         self.table = torch.zeros(max(s.layers, 1), batch * s.n_q, device=self.device, dtype=torch.float32)
@@ -143,8 +159,10 @@ class SagaDecoder:
         # decode projections: the skinny-GEMM kernel for up to 32 token rows
         self.use_gemv = (batch <= 32 and dtype == torch.bfloat16 and s.hidden % 32 == 0 and s.intermediate % 32 == 0
                          and (s.n_q * d) % 32 == 0 and s.qkv_width % 16 == 0 and s.vocab % 16 == 0)
+        if weight_bits == 4 and (not self.use_gemv or any(k % weight_group for k in (s.hidden, s.n_q * d, s.intermediate))):
+            raise ValueError("weight_bits=4 needs bf16, a batch of at most 32 and widths that are multiples of weight_group")
         # q/k/v projection, RoPE and cache append in one launch (pair-ordered rows)
-        self.fuse_rope = fuse_rope and self.use_gemv and d % 16 == 0
+        self.fuse_rope = fuse_rope and self.use_gemv and d % 16 == 0 and kv_bits == 16 and weight_bits == 16
         self.pack_weights = pack_weights
         self.keep_source_weights = keep_source_weights
         self.k2_variant = k2_variant
@@ -232,7 +250,19 @@ class SagaDecoder:
             self.kw_lm = (self.lm_head.float() * self.ln_f.float()).to(self.dtype)
             self.kw_o = list(self.w_o)
             self.kw_d = list(self.w_d)
-            if self.pack_weights:
+            if self.weight_bits == 4:
+                def q4(w):
+                    return ops.quantize_gemv_weight(w, self.weight_group)
+
+                self.kw_qkv, self.kw_gu, self.kw_o, self.kw_d = (
+                    [q4(w) for w in ws] for ws in (self.kw_qkv, self.kw_gu, self.kw_o, self.kw_d))
+                self.kw_lm = q4(self.kw_lm)
+                self._ones = torch.ones(s.hidden, device=self.device, dtype=self.dtype)
+                if not self.keep_source_weights:
+                    self.w_qkv = self.w_o = self.w_gu = self.w_d = None
+                    if self.lm_head is not self.embed:
+                        self.lm_head = None
+            elif self.pack_weights:
                 # MFMA-fragment order: every fragment 1 KB contiguous.  The
                 # projections of few 16-row tiles (q/k/v, o, down: 96-120 at
                 # the 1.5B shape) in 8-row tiles when the batch allows (<= 8
@@ -262,13 +292,17 @@ class SagaDecoder:
         def buf(n):
             return torch.empty(max(int(n), 256), dtype=torch.uint8, device=self.device)
 
-        self.ws["atopn"] = buf(max(ops.atopn_workspace_bytes(B, s.n_q, s.n_k, L, d, self.top_n, cal)
-                                   for cal in (True, False)))
-        self.ws["dense"] = buf(lib.saga_dense_workspace_bytes(B, s.n_q, L, d))
+        if self.kv_bits == 4:
+            self.ws["dense_q4"] = buf(lib.saga_dense_q4_workspace_bytes(B, s.n_q, L, d))
+        else:
+            self.ws["atopn"] = buf(max(ops.atopn_workspace_bytes(B, s.n_q, s.n_k, L, d, self.top_n, cal)
+                                       for cal in (True, False)))
+            self.ws["dense"] = buf(lib.saga_dense_workspace_bytes(B, s.n_q, L, d))
         if self.use_gemv:
             shapes = ((s.qkv_width, s.hidden), (s.hidden, s.n_q * d), (2 * s.intermediate, s.hidden),
                       (s.hidden, s.intermediate), (s.vocab, s.hidden))
-            self.ws["gemv"] = buf(max(lib.saga_gemv_workspace_bytes(B, n, k) for n, k in shapes))
+            need = lib.saga_gemv_q4_workspace_bytes if self.weight_bits == 4 else lib.saga_gemv_workspace_bytes
+            self.ws["gemv"] = buf(max(need(B, n, k) for n, k in shapes))
             self.ws["argmax"] = buf(lib.saga_argmax_workspace_bytes(B, s.vocab))
 
     def _prefill_layer(self, l: int):
@@ -277,6 +311,10 @@ class SagaDecoder:
         once released, the decode copies unpacked (norms folded in); w_gu None
         where ops.prompt_mlp takes the packed copy."""
         s = self.shape
+        if self.weight_bits == 4:  # the model that the decode step runs
+            w_qkv, w_o, w_d, w_gu = ops.unpack_gemv_q4([self.kw_qkv[l], self.kw_o[l], self.kw_d[l], self.kw_gu[l]],
+                                                       [None, None, None, (1, 2 * s.intermediate)])
+            return self._ones, w_qkv, w_o, self._ones, w_gu, w_d
         if self.w_qkv is not None:
             return self.ln1[l], self.w_qkv[l], self.w_o[l], self.ln2[l], self.w_gu[l], self.w_d[l]
         weights = [self.kw_qkv[l], self.kw_o[l], self.kw_d[l]]
@@ -303,15 +341,21 @@ class SagaDecoder:
         x = self.embed.index_select(0, prompt.to(self.device).reshape(-1))
         pos = torch.arange(T, device=self.device, dtype=torch.int32)
         zeros = torch.zeros(T, device=self.device, dtype=torch.int32)
+        table = ops.rope_table(pos, d, s.rope_theta) if self.kv_bits == 4 else None
         mod = _HeadGroups()
         for l in range(s.layers):
             n1, w_qkv, w_o, n2, w_gu, w_d = self._prefill_layer(l)
             h = ops.rmsnorm(x, n1, s.eps)
             qkv = torch.addmm(self.b_qkv[l], h, w_qkv.t())
-            q = ops.rope_kv_append(qkv, s.n_q, s.n_k, s.n_v, s.rope_theta, pos, self.k_cache[l], self.v_cache[l],
-                                   batch=zeros)
-            k = self.k_cache[l, 0:1, :, :T]
-            v = self.v_cache[l, 0:1, :, :T]
+            if self.kv_bits == 4:
+                cache = self.kv.layer(l)
+                q = ops.rope_kv_append_q4(qkv, s.n_q, table, pos, cache, batch=zeros)
+                k, v = (t.transpose(0, 1).unsqueeze(0) for t in ops.read_kv_q4(cache, pos, zeros, dtype=self.dtype))
+            else:
+                q = ops.rope_kv_append(qkv, s.n_q, s.n_k, s.n_v, s.rope_theta, pos, self.k_cache[l], self.v_cache[l],
+                                       batch=zeros)
+                k = self.k_cache[l, 0:1, :, :T]
+                v = self.v_cache[l, 0:1, :, :T]
             # the HIP prefill kernel when ops.prefill_supported holds for these
             # operands, else torch SDPA (attention/attention.py:13-53)
             o, _ = sdpa_attention_forward(mod, q.transpose(0, 1).unsqueeze(0), k, v, None, is_causal=True)
@@ -322,7 +366,9 @@ class SagaDecoder:
                 act = ops.prompt_mlp(h, self.kw_gu[l]) if w_gu is None else ops.silu_mul(torch.mm(h, w_gu.t()))
                 xc.addmm_(act, w_d.t())
             del w_qkv, w_o, w_gu, w_d
-        if self.lm_head is not None:
+        if self.weight_bits == 4:
+            first = ops.gemv_q4(x[-1:], self.kw_lm, rms_eps=s.eps, split_k=False).argmax(dim=-1)
+        elif self.lm_head is not None:
             last = ops.rmsnorm(x[-1:], self.ln_f, s.eps)
             head = self.lm_head
             if head.dtype == torch.bfloat16 and head.is_contiguous() and head.data_ptr() % 16 == 0 \
@@ -334,8 +380,8 @@ class SagaDecoder:
         else:
             # the packed head as the decode step reads it: one row needs no row-major copy of the vocabulary
             first = ops.gemv(x[-1:], self.kw_lm, rms_eps=s.eps, workspace=self.ws.get("gemv")).argmax(dim=-1)
-        self.k_cache[:, 1:, :, :T] = self.k_cache[:, 0:1, :, :T]
-        self.v_cache[:, 1:, :, :T] = self.v_cache[:, 0:1, :, :T]
+        for c in self.kv.tensors:
+            c[:, 1:, :, :T] = c[:, 0:1, :, :T]
         self.prompt_len = T
         self.reset()
         self._first_token = first
@@ -346,12 +392,25 @@ class SagaDecoder:
         """Fill the cache with N(0,1) keys/values of prompt_len positions
         instead of a prefill (tests and kernel-level runs)."""
         g = torch.Generator(device=self.device).manual_seed(seed)
-        for c in (self.k_cache, self.v_cache):
+        if self.kv_bits == 4:
+            self._fill_synthetic_q4(prompt_len, g)
+        for c in (self.k_cache, self.v_cache) if self.kv_bits == 16 else ():
             c[..., :prompt_len, :] = torch.randn(c[..., :prompt_len, :].shape, generator=g, device=self.device,
                                                  dtype=torch.float32).to(self.dtype)
         self.prompt_len = prompt_len
         self._first_token = torch.zeros(1, dtype=torch.int64, device=self.device)
         self.reset()
+
+    def _fill_synthetic_q4(self, prompt_len: int, g: torch.Generator) -> None:
+        s, d, B = self.shape, self.shape.head_dim, self.batch
+        for l in range(s.layers):
+            for p0 in range(0, prompt_len, 4096):
+                n = min(4096, prompt_len - p0)
+                pos = (torch.arange(n, device=self.device, dtype=torch.int32) + p0).repeat(B)
+                rows = torch.arange(B, device=self.device, dtype=torch.int32).repeat_interleave(n)
+                x = torch.randn(B * n, (1 + s.n_k + s.n_v) * d, generator=g, device=self.device).to(self.dtype)
+                unrotated = torch.tensor([1.0, 0.0], device=self.device).expand(B * n, d // 2, 2).contiguous()
+                ops.rope_kv_append_q4(x, 1, unrotated, pos, self.kv.layer(l), batch=rows)
 
     def reset(self) -> None:
         """Rewind the decode state to just after the prompt."""
@@ -369,7 +428,8 @@ class SagaDecoder:
         x = self._x
         # the token rows' embeddings and their rotations (once for all layers)
         ops.embed_rope(self.tokens, self.embed, x, self.pos, d, s.rope_theta,
-                       rope_table=self._rope if self.fuse_rope else None)
+                       rope_table=self._rope if self.fuse_rope or self.kv_bits == 4 else None)
+        gemv = ops.gemv_q4 if self.weight_bits == 4 else ops.gemv
         q4 = self._q.view(B, s.n_q, 1, d)
         for l in range(s.layers):
             if self.fuse_rope:
@@ -378,27 +438,23 @@ class SagaDecoder:
                                  rope_table=self._rope)
             else:
                 if self.use_gemv:
-                    ops.gemv(x, self.kw_qkv[l], bias=self.b_qkv[l], rms_eps=s.eps, out=self._qkv, workspace=ws.get("gemv"))
+                    gemv(x, self.kw_qkv[l], bias=self.b_qkv[l], rms_eps=s.eps, out=self._qkv, workspace=ws.get("gemv"))
                 else:
                     ops.rmsnorm(x, self.ln1[l], s.eps, out=self._h)
                     torch.addmm(self.b_qkv[l], self._h, self.w_qkv[l].t(), out=self._qkv)
-                ops.rope_kv_append(self._qkv, s.n_q, s.n_k, s.n_v, s.rope_theta, self.pos, self.k_cache[l],
-                                   self.v_cache[l], q_out=self._q)
-            K, V = self.k_cache[l], self.v_cache[l]
-            if self.mode == "vanilla":
-                self._vanilla_attention(q4, K, V)
-            elif self.mode == "dense" or l in self.exempt:
-                ops.dense_decode(q4, K, V, kv_len=self.kv_len, out=self._attn, workspace=ws["dense"])
-            elif calibrate:
-                ops.atopn_calibrate(q4, K, V, self.top_n, self.table[l], kv_len=self.kv_len, out=self._attn,
-                                    workspace=ws["atopn"])
+                if self.kv_bits == 4:
+                    ops.rope_kv_append_q4(self._qkv, s.n_q, self._rope, self.pos, self.kv.layer(l), q_out=self._q)
+                else:
+                    ops.rope_kv_append(self._qkv, s.n_q, s.n_k, s.n_v, s.rope_theta, self.pos, self.k_cache[l],
+                                       self.v_cache[l], q_out=self._q)
+            if self.kv_bits == 4:
+                ops.dense_decode_q4(q4, self.kv.layer(l), kv_len=self.kv_len, out=self._attn, workspace=ws["dense_q4"])
             else:
-                ops.atopn_decode(q4, K, V, self.table[l], self.top_n, kv_len=self.kv_len, out=self._attn,
-                                 workspace=ws["atopn"], k2_variant=self.k2_variant)
+                self._attention(l, q4, calibrate)
             if self.use_gemv:
-                ops.gemv(self._attn.view(B, s.n_q * d), self.kw_o[l], epilogue="add", out=x, workspace=ws["gemv"])
-                ops.gemv(x, self.kw_gu[l], rms_eps=s.eps, epilogue="silu_pairs", out=self._act, workspace=ws["gemv"])
-                ops.gemv(self._act, self.kw_d[l], epilogue="add", out=x, workspace=ws["gemv"])
+                gemv(self._attn.view(B, s.n_q * d), self.kw_o[l], epilogue="add", out=x, workspace=ws["gemv"])
+                gemv(x, self.kw_gu[l], rms_eps=s.eps, epilogue="silu_pairs", out=self._act, workspace=ws["gemv"])
+                gemv(self._act, self.kw_d[l], epilogue="add", out=x, workspace=ws["gemv"])
             else:
                 x.addmm_(self._attn.view(B, s.n_q * d), self.w_o[l].t())
                 ops.rmsnorm(x, self.ln2[l], s.eps, out=self._h)
@@ -406,13 +462,27 @@ class SagaDecoder:
                 ops.silu_mul(self._gu, out=self._act)
                 x.addmm_(self._act, self.w_d[l].t())
         if self.use_gemv:
-            ops.gemv(x, self.kw_lm, rms_eps=s.eps, out=self._logits, workspace=ws["gemv"])
+            gemv(x, self.kw_lm, rms_eps=s.eps, out=self._logits, workspace=ws["gemv"])
             ops.argmax_rows(self._logits, out=self.tokens, workspace=ws["argmax"])
         else:
             ops.rmsnorm(x, self.ln_f, s.eps, out=self._h)
             torch.mm(self._h, self.lm_head.t(), out=self._logits)
             torch.argmax(self._logits, dim=-1, out=self.tokens)
         ops.advance_positions(self.pos, self.kv_len)
+
+    def _attention(self, l: int, q4: torch.Tensor, calibrate: bool) -> None:
+        """Layer l's attention over its 16-bit caches."""
+        K, V, ws = self.k_cache[l], self.v_cache[l], self.ws
+        if self.mode == "vanilla":
+            self._vanilla_attention(q4, K, V)
+        elif self.mode == "dense" or l in self.exempt:
+            ops.dense_decode(q4, K, V, kv_len=self.kv_len, out=self._attn, workspace=ws["dense"])
+        elif calibrate:
+            ops.atopn_calibrate(q4, K, V, self.top_n, self.table[l], kv_len=self.kv_len, out=self._attn,
+                                workspace=ws["atopn"])
+        else:
+            ops.atopn_decode(q4, K, V, self.table[l], self.top_n, kv_len=self.kv_len, out=self._attn,
+                             workspace=ws["atopn"], k2_variant=self.k2_variant)
 
     def _vanilla_attention(self, q4: torch.Tensor, K: torch.Tensor, V: torch.Tensor) -> None:
         """speedup.py:76-83, vanilla mode: the decode step through the base

@@ -11,6 +11,10 @@ kind: K [layers, B, k_h, Lmax, d] and V [layers, B, v_h, Lmax, d].
   * one allocation per kind: the 28 layers of a 1.5B-shaped model at batch
     8 and 32k context are two tensors of 1.9 and 3.8 GB.
 
+With bits=4 a cache holds 4-bit codes with an f16 scale and offset per group
+of 32 or 64 dims (ops.KVQ4 per layer): 4.5 or 5 bits a value, so 3.2 to 3.6
+times the positions.
+
 plan_capacity() answers how long a context, or how large a batch, fits on one
 GPU next to the decode weights and workspaces: an MI355X has 288 GB of HBM3E.
 """
@@ -28,16 +32,27 @@ def _es(dtype) -> int:
     return torch.tensor([], dtype=dtype).element_size()
 
 
-def kv_cache_bytes(shape, batch: int, max_len: int, dtype=torch.bfloat16) -> int:
-    """Bytes of the K and V caches of every layer."""
-    return shape.layers * batch * (shape.n_k + shape.n_v) * max_len * shape.head_dim * _es(dtype)
+def _check_bits(name: str, bits: int) -> None:
+    if bits not in (4, 16):
+        raise ValueError(f"{name} must be 16 or 4, got {bits}")
 
 
-def decode_weight_bytes(shape, dtype=torch.bfloat16, decode_copies: bool = True) -> int:
+def kv_cache_bytes(shape, batch: int, max_len: int, dtype=torch.bfloat16, bits: int = 16, group: int = 64) -> int:
+    """Bytes of the K and V caches of every layer; bits 4: codes and the scales of groups of `group` dims."""
+    _check_bits("bits", bits)
+    d = shape.head_dim
+    row = d * _es(dtype) if bits == 16 else d // 2 + 4 * (d // group)
+    return shape.layers * batch * (shape.n_k + shape.n_v) * max_len * row
+
+
+def decode_weight_bytes(shape, dtype=torch.bfloat16, decode_copies: bool = True, bits: int = 16,
+                        group: int = 64) -> int:
     """Weights of a decoder of this shape: embedding (tied LM head), per-layer
     q/k/v (+ bias), o, gate/up and down projections, norms.  decode_copies:
     plus the decode-layout copies the skinny GEMM reads (norm-folded q/k/v and
-    gate/up, packed o and down, normed LM head)."""
+    gate/up, packed o and down, normed LM head), with bits=4 in codes and
+    scales (rows padded to 128 columns)."""
+    _check_bits("bits", bits)
     es = _es(dtype)
     s = shape
     per_layer = (s.qkv_width * s.hidden + s.qkv_width + s.hidden * s.n_q * s.head_dim + 2 * s.intermediate * s.hidden
@@ -45,19 +60,27 @@ def decode_weight_bytes(shape, dtype=torch.bfloat16, decode_copies: bool = True)
     base = (s.vocab * s.hidden + s.layers * per_layer + s.hidden) * es
     if not decode_copies:
         return base
-    copies = (s.layers * (s.qkv_width * s.hidden + 2 * s.intermediate * s.hidden + s.hidden * s.n_q * s.head_dim
-                          + s.hidden * s.intermediate) + s.vocab * s.hidden) * es
+    def copy(n, k):
+        return n * k * es if bits == 16 else n * ((k + 127) // 128 * 64 + 4 * (k // group))
+
+    copies = (s.layers * (copy(s.qkv_width, s.hidden) + copy(2 * s.intermediate, s.hidden)
+                          + copy(s.hidden, s.n_q * s.head_dim) + copy(s.hidden, s.intermediate))
+              + copy(s.vocab, s.hidden))
     return base + copies
 
 
-def decode_workspace_bytes(shape, batch: int, max_len: int, top_n: int) -> int:
+def decode_workspace_bytes(shape, batch: int, max_len: int, top_n: int, kv_bits: int = 16) -> int:
     """Atop-N and dense decode workspaces of one layer call (shared by all
-    layers) plus the per-step activations and the threshold table."""
+    layers; a 4-bit cache: its dense workspace) plus the per-step activations
+    and the threshold table."""
     from . import _lib
     lib = _lib.load()
     s = shape
-    ws = lib.saga_atopn_workspace_bytes(batch, s.n_q, s.n_k, max_len, s.head_dim, min(2 * top_n, max_len))
-    ws += lib.saga_dense_workspace_bytes(batch, s.n_q, max_len, s.head_dim)
+    if kv_bits == 4:
+        ws = lib.saga_dense_q4_workspace_bytes(batch, s.n_q, max_len, s.head_dim)
+    else:
+        ws = lib.saga_atopn_workspace_bytes(batch, s.n_q, s.n_k, max_len, s.head_dim, min(2 * top_n, max_len))
+        ws += lib.saga_dense_workspace_bytes(batch, s.n_q, max_len, s.head_dim)
     ws += lib.saga_gemv_workspace_bytes(batch, s.hidden, s.intermediate)
     ws += s.layers * batch * s.n_q * 4
     ws += batch * (3 * s.hidden + s.qkv_width + 2 * s.intermediate + s.vocab) * 2
@@ -86,23 +109,24 @@ class CapacityPlan:
 
 def plan_capacity(shape, batch: Optional[int] = None, max_len: Optional[int] = None, budget_bytes: Optional[int] = None,
                   reserve_fraction: float = 0.05, top_n: int = 512, dtype=torch.bfloat16,
-                  align: int = 256) -> CapacityPlan:
+                  align: int = 256, kv_bits: int = 16, weight_bits: int = 16, group: int = 64) -> CapacityPlan:
     """The largest max_len for a given batch, or the largest batch for a given
     max_len (give exactly one), that fits budget_bytes (default: the current
     device's total memory, else 288 GB) minus reserve_fraction, next to the
     decode weights (with their decode copies) and workspaces.  max_len is
-    rounded down to a multiple of `align` positions."""
+    rounded down to a multiple of `align` positions.  kv_bits, weight_bits:
+    caches and decode copies in 4 bits (groups of `group`)."""
     if (batch is None) == (max_len is None):
         raise ValueError("give exactly one of batch and max_len")
     if budget_bytes is None:
         budget_bytes = (torch.cuda.get_device_properties(0).total_memory if torch.cuda.is_available()
                         else HBM_BYTES_MI355X)
     avail = int(budget_bytes * (1 - reserve_fraction))
-    wbytes = decode_weight_bytes(shape, dtype)
+    wbytes = decode_weight_bytes(shape, dtype, bits=weight_bits, group=group)
 
     def fits(b: int, L: int) -> Optional[CapacityPlan]:
-        kv = kv_cache_bytes(shape, b, L, dtype)
-        ws = decode_workspace_bytes(shape, b, L, top_n)
+        kv = kv_cache_bytes(shape, b, L, dtype, kv_bits, group)
+        ws = decode_workspace_bytes(shape, b, L, top_n, kv_bits)
         if kv + wbytes + ws > avail:
             return None
         return CapacityPlan(b, L, kv, wbytes, ws, budget_bytes)
@@ -138,25 +162,44 @@ def plan_capacity(shape, batch: Optional[int] = None, max_len: Optional[int] = N
 class KVCache:
     """K [layers, B, k_h, Lmax, d] and V [layers, B, v_h, Lmax, d], zero-filled;
     layer(l) returns the reference-layout views (k [B, k_h, Lmax, d],
-    v [B, v_h, Lmax, d])."""
+    v [B, v_h, Lmax, d]).  bits=4: 4-bit codes and scales (zeros) of groups of
+    `group` dims; layer(l) returns ops.KVQ4 and k, v are None."""
 
     def __init__(self, shape, batch: int, max_len: int, device="cuda", dtype=torch.bfloat16,
-                 check_free: bool = True):
+                 check_free: bool = True, bits: int = 16, group: int = 64):
         dev = torch.device(device)
-        need = kv_cache_bytes(shape, batch, max_len, dtype)
+        d = shape.head_dim
+        _check_bits("bits", bits)
+        if bits == 4 and (d not in (64, 128) or group not in (32, 64)):
+            raise ValueError(f"a 4-bit cache needs a head dim of 64 or 128 and groups of 32 or 64, got {d} and {group}")
+        need = kv_cache_bytes(shape, batch, max_len, dtype, bits, group)
         if check_free and dev.type == "cuda":
             free, _ = torch.cuda.mem_get_info(dev)
             if need > 0.8 * free:
                 raise MemoryError(f"KV cache of {need / 2**30:.1f} GiB does not fit in {free / 2**30:.1f} GiB free "
                                   f"HBM (plan_capacity() gives the largest batch / context)")
-        d = shape.head_dim
-        self.k = torch.zeros(shape.layers, batch, shape.n_k, max_len, d, device=dev, dtype=dtype)
-        self.v = torch.zeros(shape.layers, batch, shape.n_v, max_len, d, device=dev, dtype=dtype)
-        self.batch, self.max_len = batch, max_len
+        if bits == 4:
+            from .ops import KVQ4
+
+            def zeros(heads, row, dt):
+                return torch.zeros(shape.layers, batch, heads, max_len, row, device=dev, dtype=dt)
+
+            self.k = self.v = None
+            self.q4 = KVQ4(*(zeros(h, row, dt) for h in (shape.n_k, shape.n_v)
+                             for row, dt in ((d // 2, torch.uint8), (2 * d // group, torch.float16))))
+        else:
+            self.k = torch.zeros(shape.layers, batch, shape.n_k, max_len, d, device=dev, dtype=dtype)
+            self.v = torch.zeros(shape.layers, batch, shape.n_v, max_len, d, device=dev, dtype=dtype)
+            self.q4 = None
+        self.batch, self.max_len, self.bits = batch, max_len, bits
+
+    @property
+    def tensors(self):
+        return self.q4 if self.bits == 4 else (self.k, self.v)
 
     @property
     def nbytes(self) -> int:
-        return self.k.numel() * self.k.element_size() + self.v.numel() * self.v.element_size()
+        return sum(t.numel() * t.element_size() for t in self.tensors)
 
     def layer(self, l: int):
-        return self.k[l], self.v[l]
+        return type(self.q4)(*(t[l] for t in self.q4)) if self.bits == 4 else (self.k[l], self.v[l])

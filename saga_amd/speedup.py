@@ -43,6 +43,9 @@ What it mirrors (speedup.py:447-700):
                         configuration named as the reference names them
                         (speedup.py:640-661).
 
+Beyond the reference: --kv_bits 4 decodes `full` over 4-bit caches and
+--weight_bits 4 with 4-bit projections and LM head (SagaDecoder's options).
+
 Models: `--model_path` is a local checkpoint directory (config.json +
 safetensors, loaded by saga_amd.checkpoint; merge mode averages its key heads
 down to --new_heads unless the checkpoint already has num_key_heads) or the
@@ -82,7 +85,7 @@ def _label(mode: str, param: Optional[int]) -> str:
 
 
 def build_decoder(model_path: str, merge: bool, new_heads: int, batch: int, max_len: int, mode: str,
-                  top_n: int, exempt, dtype):
+                  top_n: int, exempt, dtype, **options):
     """The decoder of one configuration (random-init built-in shape or a
     checkpoint directory)."""
     from saga_amd.decoder import (QWEN25_15B_GQA, QWEN25_15B_SAGA, SMOLLM2_360M_GQA, SMOLLM2_360M_SAGA,
@@ -92,13 +95,13 @@ def build_decoder(model_path: str, merge: bool, new_heads: int, batch: int, max_
         saga, gqa = ((QWEN25_15B_SAGA, QWEN25_15B_GQA) if model_path == "qwen2.5-1.5b"
                      else (SMOLLM2_360M_SAGA, SMOLLM2_360M_GQA))
         shape = replace(saga, n_k=new_heads) if merge else gqa
-        return SagaDecoder(shape, batch, max_len, mode=dmode, top_n=top_n, exempt_layers=exempt, dtype=dtype)
+        return SagaDecoder(shape, batch, max_len, mode=dmode, top_n=top_n, exempt_layers=exempt, dtype=dtype, **options)
     from saga_amd.checkpoint import load_checkpoint, read_config
     cfg = read_config(model_path)
     num_key_heads = new_heads if merge and "num_key_heads" not in cfg else None
     shape, weights = load_checkpoint(model_path, num_key_heads=num_key_heads, dtype=dtype)
     return SagaDecoder(shape, batch, max_len, mode=dmode, top_n=top_n, exempt_layers=exempt, dtype=dtype,
-                       weights=weights)
+                       weights=weights, **options)
 
 
 def trace_name(profile_output: str, merge: bool, mode: str, param: Optional[int], batch: int, seq_len: int) -> str:
@@ -116,7 +119,7 @@ def run_config(args, mode: str, param: Optional[int], batch: int, seq_len: int, 
     exempt = tuple(int(x) for x in args.exempt_layers.split(",") if x.strip())
     n_new = args.num_new_tokens
     m = build_decoder(args.model_path, merge, args.new_heads, batch, seq_len + n_new, mode, param or 512, exempt,
-                      dtype)
+                      dtype, kv_bits=getattr(args, "kv_bits", 16), weight_bits=getattr(args, "weight_bits", 16))
     torch.manual_seed(0)
     m.prefill(torch.randint(0, m.shape.vocab, (seq_len,), dtype=torch.int64))
     graphs = bool(getattr(args, "cuda_graph", True))
@@ -165,6 +168,9 @@ def _sub_cmd(args, mode, param, batch, seq_len, merge_mode) -> List[str]:
            "--num_new_tokens", str(args.num_new_tokens), "--num_iterations", str(args.num_iterations),
            "--num_warmup", str(args.num_warmup), "--dtype", args.dtype, "--new_heads", str(args.new_heads),
            "--merge_mode", merge_mode, "--_subprocess_json"]
+    for flag in ("kv_bits", "weight_bits"):
+        if getattr(args, flag, 16) != 16:
+            cmd += ["--" + flag, str(getattr(args, flag))]
     if args.exempt_layers:
         cmd += ["--exempt_layers", args.exempt_layers]
     if getattr(args, "cuda_graph", False):
@@ -207,6 +213,10 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--merge_mode", default="merge", help="merge, baseline or both (comma-separated)")
     ap.add_argument("--attention", default="full", help="full, vanilla, atopn:N, atopn_amortized:N (comma-separated)")
     ap.add_argument("--exempt_layers", default="", help="comma-separated layers that keep dense attention")
+    ap.add_argument("--kv_bits", type=int, default=16, choices=[16, 4],
+                    help="bits of a cached key / value element (4: full attention only)")
+    ap.add_argument("--weight_bits", type=int, default=16, choices=[16, 4],
+                    help="bits of a projection weight in the decode step (4: bfloat16, batch at most 32)")
     ap.add_argument("--no_compile", action="store_true",
                     help="accepted (no-op): the decode step is hand-written HIP kernels, not torch.compile output")
     ap.add_argument("--compile_mode", default="default", choices=["default", "reduce-overhead", "max-autotune"],
@@ -234,6 +244,8 @@ def main(argv=None) -> int:
         if mm not in ("merge", "baseline"):
             raise ValueError(f"Unknown merge mode: {mm}")
     modes = parse_attention(args.attention)
+    if args.kv_bits == 4 and any(m != "full" for m, _ in modes):
+        raise ValueError("--kv_bits 4 decodes with --attention full")
 
     if args._subprocess_json:  # one configuration, JSON on stdout
         (mode, param), = modes

@@ -212,3 +212,45 @@ def test_workspace_sizes():
         assert lib.saga_dense_q4_workspace_bytes(*bad) == 0
     for bad in ((0, 64, 64), (33, 64, 64), (1, 0, 64), (1, 64, 0), (1, 1 << 40, 64), (1, 64, 1 << 40)):
         assert lib.saga_gemv_q4_workspace_bytes(*bad) == 0
+
+
+def test_decoder_and_planner_options():
+    from saga_amd.decoder import QWEN25_15B_SAGA, DecoderShape, SagaDecoder
+    from saga_amd.kv_cache import HBM_BYTES_MI355X, KVCache, decode_weight_bytes, kv_cache_bytes, plan_capacity
+    s = QWEN25_15B_SAGA
+    assert kv_cache_bytes(s, 8, 33024, bits=4, group=64) == 28 * 8 * 3 * 33024 * (64 + 8)
+    assert kv_cache_bytes(s, 8, 33024, bits=4, group=32) == 28 * 8 * 3 * 33024 * (64 + 16)
+    assert decode_weight_bytes(s, bits=4) < decode_weight_bytes(s) < 2 * decode_weight_bytes(s, bits=4)
+    wide = plan_capacity(s, batch=8, budget_bytes=HBM_BYTES_MI355X)
+    q4 = plan_capacity(s, batch=8, budget_bytes=HBM_BYTES_MI355X, kv_bits=4, weight_bits=4)
+    assert q4.total_bytes <= HBM_BYTES_MI355X * 0.95
+    # 3.556 times by the rows' bytes (256 against 72); what weights and workspaces leave is at most 3 % apart
+    assert 3.4 < q4.max_len / wide.max_len < 3.7
+    tiny = DecoderShape(2, 64, 4, 1, 2, 64, 128, 256, 1e4, 1e-6)
+    c = KVCache(tiny, 3, 16, device="cpu", bits=4, group=32)
+    assert c.nbytes == kv_cache_bytes(tiny, 3, 16, bits=4, group=32) and c.k is None
+    assert [tuple(t.shape) for t in c.layer(1)] == [(3, 1, 16, 32), (3, 1, 16, 4), (3, 2, 16, 32), (3, 2, 16, 4)]
+    with pytest.raises(ValueError, match="groups of 32 or 64"):
+        KVCache(tiny, 3, 16, device="cpu", bits=4, group=128)
+    with pytest.raises(ValueError, match="16 or 4"):
+        KVCache(tiny, 3, 16, device="cpu", bits=8)
+    for kw, needle in ((dict(kv_bits=8), "16 or 4"), (dict(kv_bits=4), "mode 'dense'"),
+                       (dict(kv_bits=4, mode="dense", dtype=torch.float32), "bf16 or f16"),
+                       (dict(weight_bits=4, weight_group=16), "weight_group"),
+                       (dict(weight_bits=4, weight_group=128), "multiples of weight_group"),
+                       (dict(weight_bits=4, mode="dense", dtype=torch.float16), "needs bf16")):
+        with pytest.raises(ValueError, match=needle):
+            SagaDecoder(tiny, 2, 32, device="cpu", **kw)
+
+
+def test_command_line_options():
+    import argparse
+    from saga_amd import speedup
+    args = speedup.build_parser().parse_args(["--kv_bits", "4", "--weight_bits", "4"])
+    cmd = " ".join(speedup._sub_cmd(args, "full", None, 8, 4096, "merge"))
+    assert "--kv_bits 4" in cmd and "--weight_bits 4" in cmd
+    plain = " ".join(speedup._sub_cmd(speedup.build_parser().parse_args([]), "full", None, 8, 4096, "merge"))
+    assert "bits" not in plain
+    with pytest.raises(ValueError, match="full"):
+        speedup.main(["--attention", "full,atopn:64", "--kv_bits", "4"])
+    assert isinstance(args, argparse.Namespace)
