@@ -1180,6 +1180,10 @@ int check_kv_q4(const saga_kv_q4* c, KvQ4& kv) {
   const int64_t ng2 = ks.shape[3];
   if (ng2 != 2 * d / 32 && ng2 != 2 * d / 64)
     return fail(SAGA_ERR_UNSUPPORTED, "cache: groups of 32 or 64 dims, scales [B, heads, Lmax, 2 d / group] required");
+  // (32 rows within 2^31 bytes: the kernels' lane offsets)
+  if (kc.stride[2] >= (1LL << 26) || ks.stride[2] >= (1LL << 25) || vc.stride[2] >= (1LL << 26) ||
+      vs.stride[2] >= (1LL << 25))
+    return fail(SAGA_ERR_UNSUPPORTED, "cache: positions more than 64 MB apart");
   if (kc.shape[2] >= kMaxLen || n_k > 65535 || n_v > 65535) return fail(SAGA_ERR_UNSUPPORTED, "cache: sizes too large");
   kv = KvQ4{};
   kv.kc = static_cast<const char*>(kc.data);
@@ -1226,7 +1230,7 @@ int check_q4_weight(const saga_q4_weight* w, int64_t K, int64_t* N, int64_t* gro
   if (*group != 32 && *group != 64 && *group != 128)
     return fail(SAGA_ERR_UNSUPPORTED, "w: groups of %lld columns not built (32, 64, 128)", (long long)*group);
   *N = c.shape[0] * 16;
-  if (K >= (1LL << 30) || *N >= (1LL << 27)) return fail(SAGA_ERR_UNSUPPORTED, "w: sizes too large");
+  if (K >= (1LL << 30) || *N >= (1LL << 25)) return fail(SAGA_ERR_UNSUPPORTED, "w: sizes too large");
   return SAGA_OK;
 }
 
@@ -1332,6 +1336,11 @@ int saga_dense_decode_q4(const saga_tensor* query, const saga_kv_q4* cache, cons
     if ((mask->shape[0] != 1 && mask->shape[0] != s.b) || (mask->shape[1] != 1 && mask->shape[1] != s.q_h) ||
         mask->shape[2] != 1 || mask->shape[3] < s.L)
       return fail(SAGA_ERR_INVALID, "mask: shape does not broadcast to [b, q_h, 1, L=%lld]", (long long)s.L);
+    const int64_t span = (mask->shape[1] - 1) * mask->stride[1] + (s.L - 1) * mask->stride[3];
+    if (span * elt_size(mask->dtype) >= (1LL << 31) - 64)
+      return fail(SAGA_ERR_UNSUPPORTED, "mask: a batch row of more than 2 GB");
+    if (elt_size(mask->dtype) > 1 && reinterpret_cast<uintptr_t>(mask->data) % elt_size(mask->dtype))
+      return fail(SAGA_ERR_INVALID, "mask: data pointer must be aligned to its type");
     p.mask = mask->data;
     p.mask_dt = mask->dtype;
     p.m_sb = mask->shape[0] == 1 ? 0 : mask->stride[0];
@@ -1361,14 +1370,12 @@ int saga_dense_decode_q4(const saga_tensor* query, const saga_kv_q4* cache, cons
   p.o_sb = out->stride[0];
   p.o_sh = out->stride[1];
   p.part = static_cast<float*>(workspace);
-  p.nsplit = static_cast<int32_t>(ns);
-  p.split_len = static_cast<int32_t>(sl);
   if ((rc = hip_status(launch_dense_decode_q4(p, static_cast<hipStream_t>(stream)), "dense_decode_q4 launch"))) return rc;
   return ok();
 }
 
 size_t saga_gemv_q4_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M < 1 || M > 32 || N < 16 || K < 32 || N >= (1LL << 27) || K >= (1LL << 30)) return 0;
+  if (M < 1 || M > 32 || N < 16 || K < 32 || N >= (1LL << 25) || K >= (1LL << 30)) return 0;
   return static_cast<size_t>(gemv_q4_workspace_bytes(M, N, K));
 }
 

@@ -365,7 +365,7 @@ struct DenseQ4Params {
   const int32_t* kv_len;
   int32_t b, q_h, L;
   int32_t g, g_v;  // query heads per key head and per value head
-  int32_t nseg;    // blocks of query heads per batch row (set at launch)
+  int32_t nseg;    // units of query heads per batch row (set at launch, with the splits)
   float scale;
   void* out;
   int32_t out_dt;
@@ -373,7 +373,7 @@ struct DenseQ4Params {
   float* part;  // [b * q_h][nsplit][2 + d]
   int32_t nsplit, split_len;
 };
-void dense_q4_plan(int64_t b, int64_t L, int64_t* nsplit, int64_t* split_len);
+void dense_q4_plan(int64_t units, int64_t L, int64_t* nsplit, int64_t* split_len);
 hipError_t launch_dense_decode_q4(DenseQ4Params& p, hipStream_t st);
 
 struct GemvQ4Params {
@@ -388,9 +388,12 @@ struct GemvQ4Params {
   int32_t rms;
   float eps;
   int32_t epilogue;
+  int32_t splits;  // ranges of K (set at launch, with the fields below)
+  float* part;     // [splits][N / 16][token tiles][64][4]
+  float* part_sq;  // [splits][32]
 };
 int64_t gemv_q4_workspace_bytes(int64_t M, int64_t N, int64_t K);
-hipError_t launch_gemv_q4(const GemvQ4Params& p, void* ws, hipStream_t st);
+hipError_t launch_gemv_q4(GemvQ4Params& p, void* ws, hipStream_t st);
 
 struct UnpackQ4Params {
   struct Item {
