@@ -31,18 +31,18 @@ _RETIRED: list = []     # replaced workspaces that a captured graph may use, ali
 
 
 def _need_gpu(*ts: Optional[torch.Tensor]) -> torch.device:
-    dev = None
+    first, index = None, -1
     for t in ts:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError(
                 f"saga_amd: tensors must be on a ROCm GPU (got {t.device}); the decode path has no CPU fallback")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"saga_amd: tensors on different devices ({dev}, {t.device})")
-    return dev
+        if first is None:
+            first, index = t, t.get_device()
+        elif t.get_device() != index:
+            raise RuntimeError(f"saga_amd: tensors on different devices ({first.device}, {t.device})")
+    return None if first is None else first.device
 
 
 def _device(device) -> torch.device:
@@ -76,10 +76,8 @@ def workspace(device: torch.device, kind: str, nbytes: int, stream: Optional[tor
     workspace too small for a call is replaced by one at least 1.5x larger;
     the old one stays allocated until clear_workspaces() if a graph was
     captured while it was handed out, else it is freed."""
-    dev = _device(device)
-    if stream is None:
-        stream = torch.cuda.current_stream(dev)
-    key = (dev, stream.cuda_stream, kind)
+    dev = device if type(device) is torch.device and device.index is not None else _device(device)
+    key = (dev, _lib.raw_stream(dev.index) if stream is None else stream.cuda_stream, kind)
     ws = _WORKSPACES.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = _replace(key, ws, nbytes, lambda n: torch.empty(n, dtype=torch.uint8, device=dev))
@@ -777,7 +775,7 @@ def unpack_gemv_q4(weights, heads=None):
 
 def _indices(pos, batch, n: int) -> None:
     for t, name in ((pos, "pos"), (batch, "batch")):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.shape != (n,)):
+        if t is not None and (t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous()):
             raise ValueError(f"saga_amd: {name} must be a contiguous int32 [{n}] tensor")
 
 
