@@ -171,6 +171,160 @@ __global__ void __launch_bounds__(WAVES * 64) gemv_q4_kernel(GemvQ4Params p) {
   }
 }
 
+// Weights of many tiles and short rows (the LM head): a workgroup keeps its x in
+// registers, with its sums per group, and streams pairs of tiles (64-byte pieces of y rows),
+// the next tile's codes in flight under a tile's products.  Its waves split K (UPW units
+// each) and join through LDS, two buffers, a barrier per tile; a wave then finishes tokens
+// 4 s + r of a token tile.  Here every code is 16 + c, so that one sum of x serves both corrections:
+//   sum x w = s D + (z - 16 s) sum x.
+template <int EPI, int G, int MT, int WAVES, int UPW>
+__global__ void __launch_bounds__(WAVES * 64, 8 / WAVES) gemv_q4_stream_kernel(GemvQ4Params p) {
+  constexpr int NG = 128 / G;
+  __shared__ float red[2][WAVES][MT][4][64];
+  __shared__ float rsq[WAVES][16 * MT];
+  constexpr int NF = (4 * MT + WAVES - 1) / WAVES;  // (token tile, r) that a wave finishes: w, w + WAVES, ...
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, s = lane >> 4;
+  const int units = (p.K + 127) / 128, steps = p.K / 32, groups = p.K / G, tiles = p.N / 16;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  const u32x4 ones = {kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones};
+  const Q4Const qc;
+
+  struct Tile {
+    u32x4 c[UPW];
+    uint32_t sz[UPW][NG];
+  };
+  int64_t coff[UPW], soff[UPW][NG];  // units and groups past the row repeat its last (their x is zero)
+#pragma unroll
+  for (int u = 0; u < UPW; ++u) {
+    const int J = min(w + WAVES * u, units - 1);
+    coff[u] = static_cast<int64_t>(J) * 1024 + lane * 16;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) soff[u][g] = static_cast<int64_t>(min(J * NG + g, groups - 1)) * 64 + col * 4;
+  }
+  // pairs blockIdx.x, + gridDim.x, ... of tiles: the workgroups read one region at a time
+  const int pairs = (tiles + 1) / 2, grid = static_cast<int>(gridDim.x), b0 = static_cast<int>(blockIdx.x);
+  const int mine = (pairs - b0 + grid - 1) / grid * 2;
+  auto tile_of = [&](int i) { return ((i >> 1) * grid + b0) * 2 + (i & 1); };
+  auto load_tile = [&](Tile& t, int tile) {
+    const int at = min(tile, tiles - 1);
+    const char* code = static_cast<const char*>(p.codes) + static_cast<int64_t>(at) * units * 1024;
+    const char* scale = static_cast<const char*>(p.scales) + static_cast<int64_t>(at) * groups * 64;
+#pragma unroll
+    for (int u = 0; u < UPW; ++u) {
+      t.c[u] = ld16(code + coff[u]);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) t.sz[u][g] = *reinterpret_cast<const uint32_t*>(scale + soff[u][g]);
+    }
+  };
+  Tile ta, tb;
+  load_tile(ta, tile_of(0));
+
+  u32x4 xf[UPW][MT][4];
+  f32x4 xs[UPW][NG][MT];
+  {
+    f32x4 sq[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      sq[mt] = zero;
+      const bool row = col + 16 * mt < p.M;  // rows past the last token repeat the first: not stored
+      const char* xrow = static_cast<const char*>(p.x) + (static_cast<int64_t>(row ? col + 16 * mt : 0) * p.x_ld + 8 * s) * 2;
+#pragma unroll
+      for (int u = 0; u < UPW; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = 4 * (w + WAVES * u) + j;
+          xf[u][mt][j] = ld16(xrow + static_cast<int64_t>(min(k, steps - 1)) * 64);
+          if (k >= steps) xf[u][mt][j] = u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int u = 0; u < UPW; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int g = j * 32 / G;
+          xs[u][g][mt] = mfma_bf16(xf[u][mt][j], ones, j * 32 % G == 0 ? zero : xs[u][g][mt]);
+          if (p.rms) sq[mt] = mfma_bf16(xf[u][mt][j], xf[u][mt][j], sq[mt]);
+        }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)  // the diagonal of x x^T
+        if (col == 4 * s + r) rsq[w][16 * mt + col] = sq[mt][r];
+    }
+  }
+  lds_sync();
+  float scl[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    const int i = min(w + f * WAVES, 4 * MT - 1);
+    scl[f] = 1.f;
+    if (p.rms) {
+      float q2 = 0.f;
+#pragma unroll
+      for (int q = 0; q < WAVES; ++q) q2 += rsq[q][16 * (i / 4) + 4 * s + i % 4];
+      scl[f] = rsqrtf(q2 / static_cast<float>(p.K) + p.eps);
+    }
+  }
+
+  auto use_tile = [&](const Tile& t, int tile, int buf) {
+    f32x4 acc[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) acc[mt] = zero;
+#pragma unroll
+    for (int u = 0; u < UPW; ++u)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        f32x4 d[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) d[mt] = zero;
+#pragma unroll
+        for (int j = g * (G / 32); j < (g + 1) * (G / 32); ++j) {
+          const u32x4 b = q4_frag16(t.c[u][j], qc);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) d[mt] = mfma_bf16(xf[u][mt][j], b, d[mt]);
+        }
+        const float sc = q4_lo(t.sz[u][g]), zo = __builtin_fmaf(-16.f, sc, q4_hi(t.sz[u][g]));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            acc[mt][r] = __builtin_fmaf(sc, d[mt][r], __builtin_fmaf(zo, xs[u][g][mt][r], acc[mt][r]));
+      }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) red[buf][w][mt][r][lane] = acc[mt][r];
+    lds_sync();
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const int i = w + f * WAVES;
+      if (i >= 4 * MT) break;
+      float o = 0.f;
+#pragma unroll
+      for (int q = 0; q < WAVES; ++q) o += red[buf][q][i / 4][i % 4][lane];
+      o *= scl[f];
+      const int m = 16 * (i / 4) + 4 * s + i % 4, n = tile * 16 + col;
+      uint16_t* y = static_cast<uint16_t*>(p.y) + static_cast<int64_t>(m) * p.y_ld;
+      if constexpr (EPI == SAGA_GEMV_SILU_PAIRS) {
+        const float up = __shfl_xor(o, 1);
+        if (m < p.M && (n & 1) == 0 && tile < tiles) y[n / 2] = f32_to_bf16_bits(o / (1.0f + expf(-o)) * up);
+      } else {
+        if (m < p.M && tile < tiles) y[n] = f32_to_bf16_bits(o);
+      }
+    }
+  };
+  for (int i = 0; i < mine; i += 2) {
+    load_tile(tb, tile_of(i + 1));
+    __builtin_amdgcn_sched_barrier(0);
+    use_tile(ta, tile_of(i), 0);
+    if (i + 1 >= mine) break;
+    load_tile(ta, tile_of(i + 2));
+    __builtin_amdgcn_sched_barrier(0);
+    use_tile(tb, tile_of(i + 1), 1);
+  }
+}
+
 // Adds up the ranges, one wave per (tile, token tile).
 template <int EPI>
 __global__ void __launch_bounds__(64) gemv_q4_join_kernel(GemvQ4Params p, int mts) {
@@ -219,9 +373,34 @@ static void launch_gemv_q4_shape(const GemvQ4Params& p, hipStream_t st) {
   else hipLaunchKernelGGL((gemv_q4_kernel<EPI, G, MT, WAVES, TPW, U, false>), grid, dim3(WAVES * 64), 0, st, p);
 }
 
+// Two workgroups of 4 waves per CU, or one of 8 where the rows need more registers (x and
+// its sums: 24 per unit and token tile, 32 with groups of 32).  Measured against workgroups
+// of a few tiles (us, 8192 tiles, groups of 64; 8 and 32 rows of x): K 960 15.5, 22.6 against
+// 17.6, 29.6; K 2048 -, 41.9 against 34.2, 52.2 (8 rows, streamed: 35.3); K 2944 -, 53.9
+// against 47.6, 72.6.
+template <int EPI, int G, int MT>
+static void launch_gemv_q4_stream(const GemvQ4Params& p, int units, hipStream_t st) {
+  if constexpr (EPI != SAGA_GEMV_ADD) {
+    constexpr bool wide = MT == 2 && G == 32;
+    if (units <= 4) {
+      hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 1>), dim3(512), dim3(256), 0, st, p);
+    } else if (units <= 8) {
+      hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 2>), dim3(512), dim3(256), 0, st, p);
+    } else if (units <= 12 && !wide) {
+      if constexpr (!wide) hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 3>), dim3(512), dim3(256), 0, st, p);
+    } else if (units <= 16) {
+      if constexpr (MT == 2) hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 8, 2>), dim3(256), dim3(512), 0, st, p);
+    } else {
+      if constexpr (MT == 2 && !wide)
+        hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 8, 3>), dim3(256), dim3(512), 0, st, p);
+    }
+  }
+}
+
 // Tiles per workgroup share its reads of x and their sums, workgroups share the CUs.
 // Measured (us; 1, 8 and 32 rows of x; waves x tiles x units in flight):
-//   9496 tiles, K 1536: 4x4x1 29.8, 33.9, 51.7; 4x2x1 32.3, 36.2, 67.3; 4x1x3 -, 42, 127
+//   9496 tiles, K 1536: 4x4x1 29.8, 33.9, 51.7; 4x2x1 32.3, 36.2, 67.3; 4x1x3 -, 42, 127;
+//     streamed with x in registers 28.0, 29.5, 37.5 (tiles one by one 27.5, 28.9, 42.5)
 //   1120 tiles, K 1536: 4x2x1 8.0, 9.1, 14.8; 8x2x1 8.0, 9.6, 14.7; 4x4x1 8.8, 10.4, 14.9; 4x1x3 7.9, 9.3, 20
 //   96 tiles, K 1536: 4x1x3 3.8 (8 rows), 4x2x3 4.4, 16x1x1 4.2
 //   96 tiles, K 8960, five ranges: 8x2x2 7.7 and 10.5 (32 rows), 8x2x1 7.9 and 10.2, 4x1x3 8.4
@@ -231,6 +410,8 @@ static void launch_gemv_q4_rows(const GemvQ4Params& p, hipStream_t st) {
   if (p.splits > 1) {
     if (tiles % 2 == 0) launch_gemv_q4_shape<EPI, G, MT, 8, 2, 1>(p, st);
     else launch_gemv_q4_shape<EPI, G, MT, 8, 1, 1>(p, st);
+  } else if (tiles >= 4096 && units <= (MT == 1 ? 12 : G == 32 ? 16 : 24) && !p.bias && EPI != SAGA_GEMV_ADD) {
+    launch_gemv_q4_stream<EPI, G, MT>(p, units, st);
   } else if (tiles >= 2048 && tiles % 4 == 0) {
     launch_gemv_q4_shape<EPI, G, MT, 4, 4, 1>(p, st);
   } else if (tiles >= 512 && tiles % 2 == 0) {

@@ -34,6 +34,11 @@ __device__ __forceinline__ u32x4 q4_frag(uint32_t w, const Q4Const& c) {
   return u32x4{q4_pair<0>(w, c), q4_pair<1>(w, c), q4_pair<2>(w, c), q4_pair<3>(w, c)};
 }
 
+// The same with b = 16 in every slot.
+__device__ __forceinline__ u32x4 q4_frag16(uint32_t w, const Q4Const& c) {
+  return u32x4{((w << 3) & c.mask) | c.base, q4_pair<1>(w, c), q4_pair<2>(w, c), q4_pair<3>(w, c)};
+}
+
 // -b of each slot of q4_frag.
 __device__ __forceinline__ u32x4 q4_minus_base() { return u32x4{0xc300c300u, 0xc180c180u, 0xc180c180u, 0xc180c180u}; }
 
