@@ -426,8 +426,8 @@ int saga_prefill_attention(const saga_tensor* query, const saga_tensor* key, con
  *          stride 1, rows aligned to 4 * d / group bytes
  * Nibbles of a code row: keys have dim 32 j + 8 s + e (s < 4, e < 8) in nibble
  * 8 (s * d / 32 + j) + e; values have dim 16 e + c (c < 16) in nibble
- * c * d / 16 + e.  Rows of any strides (batch rows and heads may overlap for
- * reading). */
+ * c * d / 16 + e.  Batch and head strides are free, positions less than 64 MB
+ * apart (batch rows and heads may overlap for reading). */
 typedef struct saga_kv_q4 {
   saga_tensor k_codes, k_scales, v_codes, v_scales;
 } saga_kv_q4;
@@ -452,8 +452,8 @@ int saga_kv_q4_read(const saga_kv_q4* cache, const int32_t* pos, const int32_t* 
                     saga_tensor* v, saga_stream_t stream);
 
 /* saga_dense_decode over a 4-bit cache: query [b, q_h, 1, d] bf16 or f16, b and
- * the heads of the cache's, L its positions; mask, kv_len, scale and out as
- * there.  Any number of query heads per key head.  Scores, softmax and sums in
+ * the heads of the cache's, L its positions; mask (a batch row of it within
+ * 2 GB), kv_len, scale and out as there; a row without keys is NaN.  Any number of query heads per key head.  Scores, softmax and sums in
  * fp32; a softmax weight enters the second product with 16 bits. */
 size_t saga_dense_q4_workspace_bytes(int64_t b, int64_t q_h, int64_t L, int64_t d);
 int saga_dense_decode_q4(const saga_tensor* query, const saga_kv_q4* cache, const saga_tensor* mask,
@@ -472,7 +472,8 @@ typedef struct saga_q4_weight {
 } saga_q4_weight;
 
 /* saga_gemv for a weight in 4 bits: x [M <= 32, K] bf16, the same epilogues,
- * bias and fused RMSNorm.  Products with the codes are exact, sums in fp32.
+ * bias and fused RMSNorm.  Products with the codes are exact, sums in fp32; a row
+ * of x that holds an infinity or a NaN gives NaN, other rows are not touched by it.
  * workspace: as saga_gemv's, of saga_gemv_q4_workspace_bytes(M, N, K) bytes (the
  * size may be 0; without it results are equal to rounding). */
 size_t saga_gemv_q4_workspace_bytes(int64_t M, int64_t N, int64_t K);

@@ -443,7 +443,7 @@ static void launch_gemv_q4_epi(const GemvQ4Params& p, hipStream_t st) {
 hipError_t launch_gemv_q4(GemvQ4Params& p, void* ws, hipStream_t st) {
   p.splits = ws ? gemv_q4_splits(p.M, p.N, p.K) : 1;
   p.part = static_cast<float*>(ws);
-  p.part_sq = p.part + p.splits * static_cast<int64_t>(p.N) * 16 * (p.M > 16 ? 2 : 1);
+  if (p.splits > 1) p.part_sq = p.part + p.splits * static_cast<int64_t>(p.N) * 16 * (p.M > 16 ? 2 : 1);
   if (p.epilogue == SAGA_GEMV_ADD) launch_gemv_q4_epi<SAGA_GEMV_ADD>(p, st);
   else if (p.epilogue == SAGA_GEMV_SILU_PAIRS) launch_gemv_q4_epi<SAGA_GEMV_SILU_PAIRS>(p, st);
   else launch_gemv_q4_epi<SAGA_GEMV_STORE>(p, st);

@@ -1,7 +1,5 @@
 // The 4-bit key / value cache around its attention: rotary embedding with the
 // append of new tokens, and rows read back as values.  Formats: saga_amd.h.
-#include <algorithm>
-
 #include "kernels.h"
 #include "q4.cuh"
 
@@ -176,7 +174,7 @@ __global__ void __launch_bounds__(256) rope_kv_append_q4_kernel(RopeQ4Params p) 
 template <int D, int G>
 static void launch_rope_kv_append_q4_typed(const RopeQ4Params& p, hipStream_t st) {
   const int passes = (p.n_q + p.kv.n_k + p.kv.n_v + 64 / (D / 16) - 1) / (64 / (D / 16));
-  const dim3 grid(static_cast<unsigned>((p.N + 3) / 4), p.N < 1024 ? std::min(passes, 1024) : 1);
+  const dim3 grid(static_cast<unsigned>((p.N + 3) / 4), p.N < 1024 ? passes : 1);
   hipLaunchKernelGGL((rope_kv_append_q4_kernel<D, G>), grid, dim3(256), 0, st, p);
 }
 

@@ -716,6 +716,9 @@ def quantize_gemv_weight(w: torch.Tensor, group: int = 64) -> Q4Weight:
         raise ValueError(f"saga_amd: 4-bit weights need [N, K] with N % 16 == 0 and K a multiple of the group "
                          f"(32, 64 or 128), got {tuple(w.shape)} and {group}")
     n, k = w.shape
+    if n > 16384:  # (temporaries of a large head, one run of rows at a time)
+        parts = [quantize_gemv_weight(w[r:r + 16384], group) for r in range(0, n, 16384)]
+        return Q4Weight(torch.cat([q.codes for q in parts]), torch.cat([q.scales for q in parts]), group)
     x = w.float().reshape(n, k // group, group)
     lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
     if not bool((torch.maximum(lo.abs(), hi.abs()) <= 65504).all()):
@@ -730,6 +733,14 @@ def quantize_gemv_weight(w: torch.Tensor, group: int = 64) -> Q4Weight:
     return Q4Weight(c[..., 0] | (c[..., 1] << 4), scales, group)
 
 
+def _on_device(dev: torch.device, entry, *args) -> int:
+    """entry(*args) with dev current: a null stream handle means the current device's null stream."""
+    if torch.cuda.current_device() == dev.index:
+        return entry(*args)
+    with torch.cuda.device(dev):
+        return entry(*args)
+
+
 def _q4_weight(w: Q4Weight):
     return _lib.descriptors(_lib.Q4Weight, w.codes, w.scales)
 
@@ -741,21 +752,22 @@ def _check_group(w: Q4Weight, K: int) -> None:
 
 
 def gemv_q4(x, w: Q4Weight, bias=None, rms_eps=None, epilogue="store", out=None, split_k=True, workspace=None):
-    """gemv for a weight in 4 bits (x [M <= 32, K] bf16): the same epilogues, bias and fused RMSNorm."""
-    _need_gpu(x, w.codes, w.scales, bias, out)
+    """gemv for a weight in 4 bits (x [M <= 32, K] bf16): the same epilogues, bias and fused RMSNorm.  split_k: pass
+    the cached workspace, so that few tiles of long rows are read split over K; workspace: a caller's own."""
+    dev = _need_gpu(x, w.codes, w.scales, bias, out)
     code = {"store": _lib.GEMV_STORE, "add": _lib.GEMV_ADD, "silu_pairs": _lib.GEMV_SILU_PAIRS}[epilogue]
     M, N = x.shape[0], w.codes.shape[0] * 16
     _check_group(w, x.shape[1])
     if out is None:
         if code == _lib.GEMV_ADD:
             raise ValueError("saga_amd: epilogue 'add' needs out")
-        out = torch.empty(M, N // 2 if code == _lib.GEMV_SILU_PAIRS else N, dtype=x.dtype, device=x.device)
+        out = torch.empty(M, N // 2 if code == _lib.GEMV_SILU_PAIRS else N, dtype=x.dtype, device=dev)
     lib = _lib.load()
     need = lib.saga_gemv_q4_workspace_bytes(M, N, x.shape[1]) if split_k else 0
-    ws = _take_workspace(workspace, x.device, "gemv_q4", need) if need else None
-    _lib.check(lib.saga_gemv_q4(_lib.tensor(x), _q4_weight(w), _lib.tensor(bias),
-                                -1.0 if rms_eps is None else float(rms_eps), code, _lib.tensor(out), _lib.ptr(ws),
-                                ws.numel() if ws is not None else 0, _lib.stream_of(x)), "gemv_q4")
+    ws = _take_workspace(workspace, dev, "gemv_q4", need) if need else None
+    _lib.check(_on_device(dev, lib.saga_gemv_q4, _lib.tensor(x), _q4_weight(w), _lib.tensor(bias),
+                          -1.0 if rms_eps is None else float(rms_eps), code, _lib.tensor(out), _lib.ptr(ws),
+                          ws.numel() if ws is not None else 0, _lib.stream_of(x)), "gemv_q4")
     return out
 
 
@@ -768,8 +780,8 @@ def unpack_gemv_q4(weights, heads=None):
         rot, rows = h if h is not None else (0, 0)
         items.append(_lib.UnpackQ4Item(_q4_weight(w), _lib.descriptor(out), rot, rows))
         outs.append(out)
-    _lib.check(_lib.load().saga_unpack_gemv_q4((_lib.UnpackQ4Item * len(items))(*items), len(items),
-                                               _lib.stream_of(outs[0])), "unpack_gemv_q4")
+    _lib.check(_on_device(dev, _lib.load().saga_unpack_gemv_q4, (_lib.UnpackQ4Item * len(items))(*items), len(items),
+                          _lib.stream_of(outs[0])), "unpack_gemv_q4")
     return outs
 
 
@@ -794,9 +806,9 @@ def rope_kv_append_q4(qkv, n_q, rope_table, pos, cache: KVQ4, batch=None, q_out=
         raise ValueError("saga_amd: rope_table must be a contiguous float32 [N, d/2, 2] tensor")
     if q_out is None:
         q_out = torch.empty(n, n_q, d, dtype=qkv.dtype, device=dev)
-    _lib.check(_lib.load().saga_rope_kv_append_q4(_lib.tensor(qkv), n_q, _lib.ptr(rope_table), _lib.ptr(pos),
-                                                  _lib.ptr(batch), _lib.tensor(q_out), _kv_q4(cache),
-                                                  _lib.stream_of(qkv)), "rope_kv_append_q4")
+    _lib.check(_on_device(dev, _lib.load().saga_rope_kv_append_q4, _lib.tensor(qkv), n_q, _lib.ptr(rope_table),
+                          _lib.ptr(pos), _lib.ptr(batch), _lib.tensor(q_out), _kv_q4(cache), _lib.stream_of(qkv)),
+               "rope_kv_append_q4")
     return q_out
 
 
@@ -807,8 +819,8 @@ def read_kv_q4(cache: KVQ4, pos, batch=None, dtype=torch.bfloat16):
     _indices(pos, batch, pos.shape[0])
     d = cache.k_codes.shape[-1] * 2
     k, v = (torch.empty(pos.shape[0], t.shape[1], d, dtype=dtype, device=dev) for t in (cache.k_codes, cache.v_codes))
-    _lib.check(_lib.load().saga_kv_q4_read(_kv_q4(cache), _lib.ptr(pos), _lib.ptr(batch), _lib.tensor(k),
-                                           _lib.tensor(v), _lib.stream_of(pos)), "read_kv_q4")
+    _lib.check(_on_device(dev, _lib.load().saga_kv_q4_read, _kv_q4(cache), _lib.ptr(pos), _lib.ptr(batch),
+                          _lib.tensor(k), _lib.tensor(v), _lib.stream_of(pos)), "read_kv_q4")
     return k, v
 
 
@@ -828,7 +840,7 @@ def dense_decode_q4(query, cache: KVQ4, attention_mask=None, scaling=None, kv_le
         out = torch.empty(b, q_h, 1, d, dtype=out_dtype or query.dtype, device=dev)
     lib = _lib.load()
     ws = _take_workspace(workspace, dev, "dense_q4", lib.saga_dense_q4_workspace_bytes(b, q_h, L, d))
-    _lib.check(lib.saga_dense_decode_q4(_lib.tensor(query), _kv_q4(cache), _lib.tensor(mask), _lib.ptr(_kv_len(kv_len)),
-                                        _scale(query, scaling), _lib.tensor(out), _lib.ptr(ws), ws.numel(),
-                                        _lib.stream_of(query)), "dense_decode_q4")
+    _lib.check(_on_device(dev, lib.saga_dense_decode_q4, _lib.tensor(query), _kv_q4(cache), _lib.tensor(mask),
+                          _lib.ptr(_kv_len(kv_len)), _scale(query, scaling), _lib.tensor(out), _lib.ptr(ws), ws.numel(),
+                          _lib.stream_of(query)), "dense_decode_q4")
     return out

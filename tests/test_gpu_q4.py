@@ -404,3 +404,118 @@ def test_chain_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(held[3], eager[3]))
     q, v = ops.read_kv_q4(held[3], held[1] - 1)
     assert q.isfinite().all() and v.isfinite().all()
+
+
+# ------------------------------------------------------------------- large offsets, workspaces, streams
+
+@pytest.mark.parametrize("kind", ["batch", "position"])
+def test_cache_offsets_past_32_bits(kind):
+    """Caches whose batch rows, or whose positions, lie more than 4 GB apart: the same results as compact ones."""
+    g = _gen(31)
+    b, L = (2, 40) if kind == "batch" else (1, 75)
+    q_h, k_h, v_h, d = 12, 1, 2, 128
+    compact = Q.random_cache(g, b, k_h, v_h, L, d, 64)
+    big = torch.empty((1 << 32) + (1 << 30), dtype=torch.uint8, device="cuda")
+    halves = torch.empty((1 << 31) + (1 << 29), dtype=torch.float16, device="cuda")
+
+    def spread(t, base, off):
+        n, row = t.shape[1], t.shape[-1]
+        if kind == "batch":
+            strides = ((1 << 32) // base.element_size() + 4096, L * row, row, 1)
+        else:
+            strides = (16, row, 60_000_000 // base.element_size(), 1)
+        return base.as_strided(t.shape, strides, off)
+
+    far = ops.KVQ4(spread(compact[0], big, 0), spread(compact[1], halves, 0), spread(compact[2], big, 65536),
+                   spread(compact[3], halves, 65536))
+    for t, c in zip(far, compact):
+        t.copy_(c)
+    q = _randn(g, b, q_h, 1, d, dtype=torch.bfloat16)
+    assert torch.equal(ops.dense_decode_q4(q, far), ops.dense_decode_q4(q, compact))
+    pos = torch.full((b,), L - 1, dtype=torch.int32, device="cuda")
+    qkv = _tokens(g, b, q_h, k_h, v_h, d, torch.bfloat16)
+    table = ops.rope_table(pos, d, 1e4)
+    for cache in (far, compact):
+        ops.rope_kv_append_q4(qkv, q_h, table, pos, cache)
+    assert all(torch.equal(t, c) for t, c in zip(far, compact))
+    assert all(torch.equal(x, y) for x, y in zip(ops.read_kv_q4(far, pos), ops.read_kv_q4(compact, pos)))
+
+
+@pytest.mark.parametrize("N,K", [(1 << 20, 8704), ((1 << 23) + 512, 1024)])
+def test_weight_offsets_past_32_bits(N, K):
+    """Codes of more than 4 GB: the first and the last rows against 64 bits."""
+    g = _gen(32)
+    codes = torch.empty(N // 16, (K + 127) // 128, 1024, dtype=torch.uint8, device="cuda").random_(0, 256, generator=g)
+    scales = torch.empty(N // 16, K // 128, 16, 2, dtype=torch.float16, device="cuda").uniform_(0.01, 0.02, generator=g)
+    w = ops.Q4Weight(codes, scales, 128)
+    x = _randn(g, 3, K, dtype=torch.bfloat16)
+    got = ops.gemv_q4(x, w)
+    for part in (slice(0, 4), slice(N // 16 - 4, N // 16)):
+        ref, size = _gemv_ref(x, ops.Q4Weight(codes[part], scales[part], 128), None)
+        rows = slice(16 * part.start, 16 * part.stop)
+        _close(got[:, rows], ref, HALF[torch.bfloat16] * (ref.abs() + size) + size)
+    assert got.isfinite().all()
+
+
+def test_gemv_q4_workspaces():
+    """Split over K or not, in the cached workspace or the caller's: within the bound of each; a workspace of another
+    type, size or device is refused."""
+    g = _gen(33)
+    x = _randn(g, 8, 8960, dtype=torch.bfloat16)
+    w = ops.quantize_gemv_weight(0.05 * _randn(g, 256, 8960), 64)
+    need = ops._lib.load().saga_gemv_q4_workspace_bytes(8, 256, 8960)
+    assert need > 0
+    ref, size = _gemv_ref(x, w, 1e-6)
+    own = torch.empty(need, dtype=torch.uint8, device="cuda")
+    a, b, c = (ops.gemv_q4(x, w, rms_eps=1e-6, **kw) for kw in ({}, {"workspace": own}, {"split_k": False}))
+    assert torch.equal(a, b)
+    for got in (a, c):
+        _close(got, ref, HALF[torch.bfloat16] * (ref.abs() + size) + size)
+    for bad in (own[:-1], own.view(torch.int8), torch.empty(need)):
+        with pytest.raises(ValueError, match="workspace"):
+            ops.gemv_q4(x, w, workspace=bad)
+
+
+def test_python_refusals():
+    g = _gen(34)
+    cache = Q.random_cache(g, 2, 1, 1, 8, 64, 32)
+    w = ops.quantize_gemv_weight(torch.zeros(16, 128, device="cuda"), 64)
+    x = torch.zeros(2, 192, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="does not meet"):
+        ops.gemv_q4(x, w)
+    with pytest.raises(ValueError, match="needs out"):
+        ops.gemv_q4(x[:, :128].contiguous(), w, epilogue="add")
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    table = ops.rope_table(pos, 64, 1e4)
+    for kw, needle in ((dict(pos=pos.long()), "pos"), (dict(pos=pos[:1]), "pos"), (dict(batch=pos.long()), "batch"),
+                       (dict(rope_table=table[:1]), "rope_table"), (dict(rope_table=table.double()), "rope_table")):
+        a = dict(rope_table=table, pos=pos, batch=pos)
+        a.update(kw)
+        with pytest.raises(ValueError, match=needle):
+            ops.rope_kv_append_q4(x, 1, cache=cache, **a)
+    q = torch.zeros(2, 1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="kv_len"):
+        ops.dense_decode_q4(q, cache, kv_len=pos[:1])
+    with pytest.raises(ValueError, match="kv_len"):
+        ops.dense_decode_q4(q, cache, kv_len=pos.long())
+    with pytest.raises(NotImplementedError, match="l_q"):
+        ops.dense_decode_q4(q.expand(2, 1, 2, 64), cache)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        ops.dense_decode_q4(q, cache._replace(k_codes=cache.k_codes.cpu()))
+
+
+def test_another_stream():
+    """Calls on a stream of their own, each with the workspace of that stream, beside calls on the default one."""
+    g = _gen(35)
+    cache = Q.random_cache(g, 2, 1, 2, 3000, 128, 64)
+    qs = [_randn(g, 2, 12, 1, 128, dtype=torch.bfloat16) for _ in range(2)]
+    want = [ops.dense_decode_q4(q, cache) for q in qs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = [[], []]
+    for _ in range(8):
+        got[0].append(ops.dense_decode_q4(qs[0], cache))
+        with torch.cuda.stream(side):
+            got[1].append(ops.dense_decode_q4(qs[1], cache))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
