@@ -375,24 +375,28 @@ static void launch_gemv_q4_shape(const GemvQ4Params& p, hipStream_t st) {
 
 // Two workgroups of 4 waves per CU, or one of 8 where the rows need more registers (x and
 // its sums: 24 per unit and token tile, 32 with groups of 32).  Measured against workgroups
-// of a few tiles (us, 8192 tiles, groups of 64; 8 and 32 rows of x): K 960 15.5, 22.6 against
-// 17.6, 29.6; K 2048 -, 41.9 against 34.2, 52.2 (8 rows, streamed: 35.3); K 2944 -, 53.9
-// against 47.6, 72.6.
+// of a few tiles (us, groups of 64; 1, 8 and 32 rows of x): 8192 tiles, K 960 14.3, 15.5, 22.6
+// against 16.7, 17.6, 29.6; K 2048 -, -, 41.9 against 31.8, 34.2, 52.2 (8 rows, streamed:
+// 35.3); K 2944 -, -, 53.9 against 44.1, 47.6, 72.6; K 1536 with 1280 tiles 8.0, 8.1, 13.0
+// against 8.7, 9.3, 16.1, 768 6.6, 7.2, 11.4 against 7.0, 7.8, 10.9, 320 4.9, 5.5, 8.9 against
+// 4.7, 5.8, 9.6.
 template <int EPI, int G, int MT>
 static void launch_gemv_q4_stream(const GemvQ4Params& p, int units, hipStream_t st) {
   if constexpr (EPI != SAGA_GEMV_ADD) {
     constexpr bool wide = MT == 2 && G == 32;
+    const int pairs = (p.N / 16 + 1) / 2;
+    const dim3 two(std::min(pairs, 512)), one(std::min(pairs, 256));
     if (units <= 4) {
-      hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 1>), dim3(512), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 1>), two, dim3(256), 0, st, p);
     } else if (units <= 8) {
-      hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 2>), dim3(512), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 2>), two, dim3(256), 0, st, p);
     } else if (units <= 12 && !wide) {
-      if constexpr (!wide) hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 3>), dim3(512), dim3(256), 0, st, p);
+      if constexpr (!wide) hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 3>), two, dim3(256), 0, st, p);
     } else if (units <= 16) {
-      if constexpr (MT == 2) hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 8, 2>), dim3(256), dim3(512), 0, st, p);
+      if constexpr (MT == 2) hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 8, 2>), one, dim3(512), 0, st, p);
     } else {
       if constexpr (MT == 2 && !wide)
-        hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 8, 3>), dim3(256), dim3(512), 0, st, p);
+        hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 8, 3>), one, dim3(512), 0, st, p);
     }
   }
 }
@@ -401,7 +405,8 @@ static void launch_gemv_q4_stream(const GemvQ4Params& p, int units, hipStream_t 
 // Measured (us; 1, 8 and 32 rows of x; waves x tiles x units in flight):
 //   9496 tiles, K 1536: 4x4x1 29.8, 33.9, 51.7; 4x2x1 32.3, 36.2, 67.3; 4x1x3 -, 42, 127;
 //     streamed with x in registers 28.0, 29.5, 37.5 (tiles one by one 27.5, 28.9, 42.5)
-//   1120 tiles, K 1536: 4x2x1 8.0, 9.1, 14.8; 8x2x1 8.0, 9.6, 14.7; 4x4x1 8.8, 10.4, 14.9; 4x1x3 7.9, 9.3, 20
+//   1120 tiles, K 1536: 4x2x1 8.0, 9.1, 14.8; 8x2x1 8.0, 9.6, 14.7; 4x4x1 8.8, 10.4, 14.9; 4x1x3 7.9, 9.3, 20;
+//     streamed 7.7, 8.0, 13.1
 //   96 tiles, K 1536: 4x1x3 3.8 (8 rows), 4x2x3 4.4, 16x1x1 4.2
 //   96 tiles, K 8960, five ranges: 8x2x2 7.7 and 10.5 (32 rows), 8x2x1 7.9 and 10.2, 4x1x3 8.4
 template <int EPI, int G, int MT>
@@ -410,7 +415,7 @@ static void launch_gemv_q4_rows(const GemvQ4Params& p, hipStream_t st) {
   if (p.splits > 1) {
     if (tiles % 2 == 0) launch_gemv_q4_shape<EPI, G, MT, 8, 2, 1>(p, st);
     else launch_gemv_q4_shape<EPI, G, MT, 8, 1, 1>(p, st);
-  } else if (tiles >= 4096 && units <= (MT == 1 ? 12 : G == 32 ? 16 : 24) && !p.bias && EPI != SAGA_GEMV_ADD) {
+  } else if (tiles >= 256 && units <= (MT == 1 ? 12 : G == 32 ? 16 : 24) && !p.bias && EPI != SAGA_GEMV_ADD) {
     launch_gemv_q4_stream<EPI, G, MT>(p, units, st);
   } else if (tiles >= 2048 && tiles % 4 == 0) {
     launch_gemv_q4_shape<EPI, G, MT, 4, 4, 1>(p, st);

@@ -47,7 +47,8 @@ def _gemv_ref(x, w, rms):
 SHAPES = [(1, 16, 32, 32), (8, 1536, 1536, 64), (5, 64, 960, 64), (16, 1920, 1536, 128), (17, 960, 2560, 32), (32, 48, 128, 128),
           (3, 1536, 8960, 64), (32, 4096, 96, 32), (2, 8192, 256, 64), (9, 32, 12416, 64), (1, 151936, 128, 128),
           (32, 17920, 192, 64), (20, 64, 8960, 128), (7, 112, 1600, 64), (9, 65552, 320, 64), (32, 65568, 960, 32),
-          (18, 65552, 1536, 32), (2, 65536, 2048, 128), (31, 65552, 2944, 64)]
+          (18, 65552, 1536, 32), (2, 65536, 2048, 128), (31, 65552, 2944, 64),
+          (6, 4096, 1536, 64), (25, 4112, 512, 128), (16, 5120, 960, 32), (24, 12304, 1600, 64), (1, 32768, 3200, 128)]
 
 
 @pytest.mark.parametrize("M,N,K,group", SHAPES)
@@ -66,7 +67,7 @@ def test_gemv_q4_store_and_bias(M, N, K, group, rms):
     assert torch.equal(got, again)  # no order that changes
 
 
-@pytest.mark.parametrize("M,N,K,group", SHAPES[:8] + SHAPES[-5:])
+@pytest.mark.parametrize("M,N,K,group", SHAPES[:8] + SHAPES[-10:])
 def test_gemv_q4_add_and_silu(M, N, K, group):
     g = _gen(N + K)
     xs = _randn(g, M, K + 8, dtype=torch.bfloat16)
