@@ -110,15 +110,14 @@ _SIGS = {
     "saga_argmax_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
     "saga_argmax": (ctypes.c_int, [_T, _P, _P, ctypes.c_size_t, _P]),
     "saga_prefill_attention": (ctypes.c_int, [_T, _T, _T, _T, ctypes.c_float, ctypes.c_int32, ctypes.c_int64, _T, _P]),
-    "saga_rope_kv_append_q4": (ctypes.c_int, [_T, _I64, _P, _P, _P, _T, ctypes.POINTER(KvQ4), _P]),
-    "saga_kv_q4_read": (ctypes.c_int, [ctypes.POINTER(KvQ4), _P, _P, _T, _T, _P]),
+    # (descriptors as addresses: a call passes their bytes, packed(), without a structure around them)
+    "saga_rope_kv_append_q4": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P]),
+    "saga_kv_q4_read": (ctypes.c_int, [_P, _P, _P, _P, _P, _P]),
     "saga_dense_q4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64]),
-    "saga_dense_decode_q4": (ctypes.c_int, [_T, ctypes.POINTER(KvQ4), _T, _P, ctypes.c_float, _T, _P, ctypes.c_size_t,
-                                            _P]),
+    "saga_dense_decode_q4": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_float, _P, _P, ctypes.c_size_t, _P]),
     "saga_gemv_q4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
-    "saga_gemv_q4": (ctypes.c_int, [_T, ctypes.POINTER(Q4Weight), _T, ctypes.c_float, ctypes.c_int32, _T, _P,
-                                    ctypes.c_size_t, _P]),
-    "saga_unpack_gemv_q4": (ctypes.c_int, [ctypes.POINTER(UnpackQ4Item), ctypes.c_int32, _P]),
+    "saga_gemv_q4": (ctypes.c_int, [_P, _P, _P, ctypes.c_float, ctypes.c_int32, _P, _P, ctypes.c_size_t, _P]),
+    "saga_unpack_gemv_q4": (ctypes.c_int, [_P, ctypes.c_int32, _P]),
 }
 GEMV_STORE, GEMV_ADD, GEMV_SILU_PAIRS = 0, 1, 2
 K2_AUTO, K2_ROW_BLOCK, K2_SLICE_ROW = 0, 1, 2
@@ -161,28 +160,25 @@ def dtype_code(dt: torch.dtype) -> int:
         raise TypeError(f"saga_amd: unsupported dtype {dt}") from None
 
 
-def _packed(t: torch.Tensor) -> bytes:
+def packed(t: torch.Tensor) -> bytes:
+    """The bytes of a tensor's saga_tensor descriptor."""
     n = t.dim()
     if n > 4:
         raise ValueError("saga_amd: at most 4 dims")
     code = dtype_code(t.dtype)
     if n == 4:
         return _PACK(t.data_ptr(), code, 4, *t.shape, *t.stride())
+    if n == 3:
+        return _PACK(t.data_ptr(), code, 3, *t.shape, 0, *t.stride(), 0)
     if n == 2:
         return _PACK(t.data_ptr(), code, 2, *t.shape, 0, 0, *t.stride(), 0, 0)
-    pad = (0,) * (4 - max(n, 1))
-    shape, stride = (tuple(t.shape), t.stride()) if n else ((1,), (1,))
-    return _PACK(t.data_ptr(), code, max(n, 1), *shape, *pad, *stride, *pad)
+    shape, stride = (t.shape[0], t.stride(0)) if n else (1, 1)
+    return _PACK(t.data_ptr(), code, 1, shape, 0, 0, 0, stride, 0, 0, 0)
 
 
 def descriptor(t: torch.Tensor) -> SagaTensor:
     """saga_tensor descriptor of a torch tensor."""
-    return SagaTensor.from_buffer_copy(_packed(t))
-
-
-def descriptors(kind, *ts: torch.Tensor):
-    """A structure of saga_tensor descriptors (KvQ4, Q4Weight)."""
-    return kind.from_buffer_copy(b"".join(map(_packed, ts)))
+    return SagaTensor.from_buffer_copy(packed(t))
 
 
 def tensor(t: torch.Tensor | None):
@@ -195,9 +191,12 @@ def ptr(t: torch.Tensor | None):
 
 
 # The handle of a device's current stream by its index: torch.cuda.current_stream builds a
-# Stream object around it (1.9 us; an eager dense_decode_q4 call 20.8 -> 16.5 us with this,
+# Stream object around it (1.9 us; an eager dense_decode_q4 call 20.8 -> 16.3 us with this,
 # where it was asked for twice, and _need_gpu's integer comparison).
 raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def stream_of(t: torch.Tensor):

@@ -19,6 +19,7 @@ because the graph still holds its address; any other is freed at once.
 from __future__ import annotations
 
 import math
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -733,41 +734,48 @@ def quantize_gemv_weight(w: torch.Tensor, group: int = 64) -> Q4Weight:
     return Q4Weight(c[..., 0] | (c[..., 1] << 4), scales, group)
 
 
-def _on_device(dev: torch.device, entry, *args) -> int:
-    """entry(*args) with dev current: a null stream handle means the current device's null stream."""
-    if torch.cuda.current_device() == dev.index:
-        return entry(*args)
-    with torch.cuda.device(dev):
-        return entry(*args)
+_HEADS_PACK = struct.Struct("=2q").pack  # rot_heads, head_rows of a saga_unpack_q4_item
+_EPILOGUES = {"store": _lib.GEMV_STORE, "add": _lib.GEMV_ADD, "silu_pairs": _lib.GEMV_SILU_PAIRS}
 
 
-def _q4_weight(w: Q4Weight):
-    return _lib.descriptors(_lib.Q4Weight, w.codes, w.scales)
+def _on_device(dev: torch.device, what: str, entry, *args) -> None:
+    """entry(*args, stream) on dev's current stream, with dev current: a null handle means the current device's stream."""
+    if _lib.current_device() == dev.index:
+        rc = entry(*args, _lib.raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, _lib.raw_stream(dev.index))
+    _lib.check(rc, what)
 
 
-def _check_group(w: Q4Weight, K: int) -> None:
-    if w.scales.shape[1] * w.group != K:
-        raise ValueError(f"saga_amd: a 4-bit weight of {w.scales.shape[1]} groups of {w.group} columns does not meet "
-                         f"{K} columns")
+def _packed(t: Optional[torch.Tensor]):
+    return None if t is None else _lib.packed(t)
+
+
+def _address(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def gemv_q4(x, w: Q4Weight, bias=None, rms_eps=None, epilogue="store", out=None, split_k=True, workspace=None):
     """gemv for a weight in 4 bits (x [M <= 32, K] bf16): the same epilogues, bias and fused RMSNorm.  split_k: pass
     the cached workspace, so that few tiles of long rows are read split over K; workspace: a caller's own."""
-    dev = _need_gpu(x, w.codes, w.scales, bias, out)
-    code = {"store": _lib.GEMV_STORE, "add": _lib.GEMV_ADD, "silu_pairs": _lib.GEMV_SILU_PAIRS}[epilogue]
-    M, N = x.shape[0], w.codes.shape[0] * 16
-    _check_group(w, x.shape[1])
+    codes, scales, group = w
+    dev = _need_gpu(x, codes, scales, bias, out)
+    code = _EPILOGUES[epilogue]
+    M, K = x.shape
+    N = codes.size(0) * 16
+    if scales.size(1) * group != K:
+        raise ValueError(f"saga_amd: a 4-bit weight of {scales.size(1)} groups of {group} columns does not meet {K} columns")
     if out is None:
         if code == _lib.GEMV_ADD:
             raise ValueError("saga_amd: epilogue 'add' needs out")
-        out = torch.empty(M, N // 2 if code == _lib.GEMV_SILU_PAIRS else N, dtype=x.dtype, device=dev)
+        out = x.new_empty(M, N // 2 if code == _lib.GEMV_SILU_PAIRS else N)
     lib = _lib.load()
-    need = lib.saga_gemv_q4_workspace_bytes(M, N, x.shape[1]) if split_k else 0
+    need = lib.saga_gemv_q4_workspace_bytes(M, N, K) if split_k else 0
     ws = _take_workspace(workspace, dev, "gemv_q4", need) if need else None
-    _lib.check(_on_device(dev, lib.saga_gemv_q4, _lib.tensor(x), _q4_weight(w), _lib.tensor(bias),
-                          -1.0 if rms_eps is None else float(rms_eps), code, _lib.tensor(out), _lib.ptr(ws),
-                          ws.numel() if ws is not None else 0, _lib.stream_of(x)), "gemv_q4")
+    _on_device(dev, "gemv_q4", lib.saga_gemv_q4, _lib.packed(x), _lib.packed(codes) + _lib.packed(scales), _packed(bias),
+               -1.0 if rms_eps is None else float(rms_eps), code, _lib.packed(out), _address(ws),
+               0 if ws is None else ws.numel())
     return out
 
 
@@ -777,11 +785,9 @@ def unpack_gemv_q4(weights, heads=None):
     outs, items = [], []
     for w, h in zip(weights, heads or [None] * len(weights)):
         out = torch.empty(w.shape, dtype=torch.bfloat16, device=dev)
-        rot, rows = h if h is not None else (0, 0)
-        items.append(_lib.UnpackQ4Item(_q4_weight(w), _lib.descriptor(out), rot, rows))
+        items += (_lib.packed(w.codes), _lib.packed(w.scales), _lib.packed(out), _HEADS_PACK(*(h or (0, 0))))
         outs.append(out)
-    _lib.check(_on_device(dev, _lib.load().saga_unpack_gemv_q4, (_lib.UnpackQ4Item * len(items))(*items), len(items),
-                          _lib.stream_of(outs[0])), "unpack_gemv_q4")
+    _on_device(dev, "unpack_gemv_q4", _lib.load().saga_unpack_gemv_q4, b"".join(items), len(outs))
     return outs
 
 
@@ -791,8 +797,8 @@ def _indices(pos, batch, n: int) -> None:
             raise ValueError(f"saga_amd: {name} must be a contiguous int32 [{n}] tensor")
 
 
-def _kv_q4(cache: KVQ4):
-    return _lib.descriptors(_lib.KvQ4, *cache)
+def _kv_q4(cache: KVQ4) -> bytes:
+    return b"".join(map(_lib.packed, cache))
 
 
 def rope_kv_append_q4(qkv, n_q, rope_table, pos, cache: KVQ4, batch=None, q_out=None):
@@ -800,15 +806,14 @@ def rope_kv_append_q4(qkv, n_q, rope_table, pos, cache: KVQ4, batch=None, q_out=
     [batch, :, pos] (batch None: token n is batch row n), each pair (batch, pos) at most once per call.
     qkv [N, (n_q+n_k+n_v)*d]; rope_table: rope_table(pos, d, theta) of these tokens.  Returns q_out [N, n_q, d]."""
     dev = _need_gpu(qkv, rope_table, pos, batch, q_out, *cache)
-    n, d = qkv.shape[0], cache.k_codes.shape[-1] * 2
+    n, d = qkv.size(0), cache.k_codes.size(-1) * 2
     _indices(pos, batch, n)
-    if rope_table.dtype != torch.float32 or not rope_table.is_contiguous() or tuple(rope_table.shape) != (n, d // 2, 2):
+    if rope_table.dtype is not torch.float32 or rope_table.shape != (n, d // 2, 2) or not rope_table.is_contiguous():
         raise ValueError("saga_amd: rope_table must be a contiguous float32 [N, d/2, 2] tensor")
     if q_out is None:
-        q_out = torch.empty(n, n_q, d, dtype=qkv.dtype, device=dev)
-    _lib.check(_on_device(dev, _lib.load().saga_rope_kv_append_q4, _lib.tensor(qkv), n_q, _lib.ptr(rope_table),
-                          _lib.ptr(pos), _lib.ptr(batch), _lib.tensor(q_out), _kv_q4(cache), _lib.stream_of(qkv)),
-               "rope_kv_append_q4")
+        q_out = qkv.new_empty(n, n_q, d)
+    _on_device(dev, "rope_kv_append_q4", _lib.load().saga_rope_kv_append_q4, _lib.packed(qkv), n_q,
+               rope_table.data_ptr(), pos.data_ptr(), _address(batch), _lib.packed(q_out), _kv_q4(cache))
     return q_out
 
 
@@ -816,11 +821,11 @@ def read_kv_q4(cache: KVQ4, pos, batch=None, dtype=torch.bfloat16):
     """What a 4-bit cache holds at [batch, :, pos] (batch None: row n): k [N, n_k, d] and v [N, n_v, d] of `dtype`,
     NaN where an index is out of range.  Transposed to [1, heads, N, d] they are prefill_attention's operands."""
     dev = _need_gpu(pos, batch, *cache)
-    _indices(pos, batch, pos.shape[0])
-    d = cache.k_codes.shape[-1] * 2
-    k, v = (torch.empty(pos.shape[0], t.shape[1], d, dtype=dtype, device=dev) for t in (cache.k_codes, cache.v_codes))
-    _lib.check(_on_device(dev, _lib.load().saga_kv_q4_read, _kv_q4(cache), _lib.ptr(pos), _lib.ptr(batch),
-                          _lib.tensor(k), _lib.tensor(v), _lib.stream_of(pos)), "read_kv_q4")
+    n, d = pos.size(0), cache.k_codes.size(-1) * 2
+    _indices(pos, batch, n)
+    k, v = (torch.empty(n, t.size(1), d, dtype=dtype, device=dev) for t in (cache.k_codes, cache.v_codes))
+    _on_device(dev, "read_kv_q4", _lib.load().saga_kv_q4_read, _kv_q4(cache), pos.data_ptr(), _address(batch),
+               _lib.packed(k), _lib.packed(v))
     return k, v
 
 
@@ -832,15 +837,14 @@ def dense_decode_q4(query, cache: KVQ4, attention_mask=None, scaling=None, kv_le
     b, q_h, l_q, d = query.shape
     if l_q != 1:
         raise NotImplementedError("saga_amd: the HIP decode kernels take l_q == 1")
-    L = cache.k_codes.shape[2]
+    L = cache.k_codes.size(2)
     mask = _mask_view(attention_mask, L)
     if kv_len is not None and kv_len.shape != (b,):
         raise ValueError("saga_amd: kv_len must be a contiguous int32 tensor [b]")
     if out is None:
-        out = torch.empty(b, q_h, 1, d, dtype=out_dtype or query.dtype, device=dev)
+        out = query.new_empty(b, q_h, 1, d, dtype=out_dtype)
     lib = _lib.load()
     ws = _take_workspace(workspace, dev, "dense_q4", lib.saga_dense_q4_workspace_bytes(b, q_h, L, d))
-    _lib.check(_on_device(dev, lib.saga_dense_decode_q4, _lib.tensor(query), _kv_q4(cache), _lib.tensor(mask),
-                          _lib.ptr(_kv_len(kv_len)), _scale(query, scaling), _lib.tensor(out), _lib.ptr(ws), ws.numel(),
-                          _lib.stream_of(query)), "dense_decode_q4")
+    _on_device(dev, "dense_decode_q4", lib.saga_dense_decode_q4, _lib.packed(query), _kv_q4(cache), _packed(mask),
+               _address(_kv_len(kv_len)), _scale(query, scaling), _lib.packed(out), ws.data_ptr(), ws.numel())
     return out
