@@ -307,6 +307,34 @@ def test_dense_q4_lengths(L, b):
     assert torch.equal(got, ops.dense_decode_q4(q, cache, kv_len=kv, out_dtype=torch.float32, scaling=0.3))
 
 
+@pytest.mark.parametrize("q_h,k_h,v_h,d", LAYOUTS)
+@pytest.mark.parametrize("dtype,group", [(torch.bfloat16, 64), (torch.bfloat16, 32), (torch.float16, 64)])
+def test_dense_q4_layouts_split(q_h, k_h, v_h, d, dtype, group):
+    """More positions than one block of a unit takes: splits without a key, with one, and full ones are joined."""
+    g = _gen(q_h * d + group + 1)
+    b, L = 4, 777
+    cache = Q.random_cache(g, b, k_h, v_h, L, d, group)
+    q = _randn(g, b, q_h, 1, d, dtype=dtype)
+    kv = torch.tensor([777, 0, 129, 640], dtype=torch.int32, device="cuda")
+    ref, tol = _dense_ref(q, cache, None, kv, 1 / math.sqrt(d))
+    got = ops.dense_decode_q4(q, cache, kv_len=kv, out_dtype=torch.float32)
+    assert got[1].isnan().all()
+    keep = [0, 2, 3]
+    _close(got[keep], ref[keep], tol[keep] + U32 * ref[keep].abs())
+
+
+@pytest.mark.parametrize("q_h,k_h,v_h,d", [(12, 1, 2, 128), (15, 1, 5, 64)])
+@pytest.mark.parametrize("L", [255, 257, 511, 512, 513, 8192, 8193, 16416, 70001])
+def test_dense_q4_one_row_splits(q_h, k_h, v_h, d, L):
+    """One row: one block to 512 positions, 64 splits at 8192, 65 (joined by blocks of 32 dims) and more past it."""
+    g = _gen(L + d)
+    cache = Q.random_cache(g, 1, k_h, v_h, L, d, 64)
+    q = _randn(g, 1, q_h, 1, d, dtype=torch.bfloat16)
+    ref, tol = _dense_ref(q, cache, None, None, 0.2)
+    got = ops.dense_decode_q4(q, cache, out_dtype=torch.float32, scaling=0.2)
+    _close(got, ref, tol + U32 * ref.abs())
+
+
 @pytest.mark.parametrize("mdt", [torch.bool, torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("per_head", [False, True])
 def test_dense_q4_masks(mdt, per_head):

@@ -102,6 +102,17 @@ def test_decoder_graphs_equal_eager(dtype, batch, weight_bits):
     assert torch.equal(m.generate(ids, 12), eager) and torch.equal(m.generate(ids, 12), eager)
 
 
+@pytest.mark.parametrize("batch", [1, 8, 32])
+def test_atopn_with_4_bit_weights(batch):
+    """4-bit weights beside Atop-N attention over 16-bit caches."""
+    s = SHAPES["qwen"]
+    m = SagaDecoder(s, batch, 2048, mode="atopn", top_n=256, weight_bits=4, seed=4)
+    ids = torch.randint(0, s.vocab, (1500,), generator=torch.Generator().manual_seed(6))
+    eager = m.generate(ids, 10, graphs=False)
+    assert m._logits.isfinite().all()
+    assert all(torch.equal(m.generate(ids, 10), eager) for _ in range(3))
+
+
 def test_fill_synthetic_q4():
     s = SHAPES["llama"]
     m = SagaDecoder(s, 2, 5000, mode="dense", kv_bits=4, weight_bits=4)
