@@ -183,9 +183,13 @@ __global__ void __launch_bounds__(WAVES * 64) gemv_q4_kernel(GemvQ4Params p) {
 // each) and join through LDS, two buffers, a barrier per tile; a wave then finishes tokens
 // 4 s + r of a token tile.  Here every code is 16 + c, so that one sum of x serves both corrections:
 //   sum x w = s D + (z - 16 s) sum x.
+// With two token tiles and groups of 32 (SUMS) the second term is a product of its own, fp32
+// MFMAs over four groups each: a register per four groups and token tile in place of 16, and
+// an instruction in place of 16 (LM head, 32 rows, 60 -> 49 us; with larger groups 5 % slower).
 template <int EPI, int G, int MT, int WAVES, int UPW>
 __global__ void __launch_bounds__(WAVES * 64, 8 / WAVES) gemv_q4_stream_kernel(GemvQ4Params p) {
-  constexpr int NG = 128 / G;
+  constexpr int NG = 128 / G, NS = UPW * NG, NC = (NS + 3) / 4;  // groups of a wave, in fours
+  constexpr bool SUMS = MT == 2 && G == 32;
   __shared__ float red[2][WAVES][MT][4][64];
   __shared__ float rsq[WAVES][16 * MT];
   constexpr int NF = (4 * MT + WAVES - 1) / WAVES;  // (token tile, r) that a wave finishes: w, w + WAVES, ...
@@ -227,7 +231,10 @@ __global__ void __launch_bounds__(WAVES * 64, 8 / WAVES) gemv_q4_stream_kernel(G
   load_tile(ta, tile_of(0));
 
   u32x4 xf[UPW][MT][4];
-  f32x4 xs[UPW][NG][MT];
+  f32x4 xs[SUMS ? 1 : UPW][NG][MT];
+  float xa[NC][MT];  // SUMS: the sum over group 4 c + s of token `col`, an A operand of four groups
+  float* xsum = &red[0][w][0][0][0];  // SUMS: [MT][4 NC][16 tokens]
+  static_assert(!SUMS || 4 * NC * 16 <= 256, "a wave's sums of x fit its part of red");
   {
     f32x4 sq[MT];
 #pragma unroll
@@ -251,7 +258,9 @@ __global__ void __launch_bounds__(WAVES * 64, 8 / WAVES) gemv_q4_stream_kernel(G
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int g = j * 32 / G;
-          xs[u][g][mt] = mfma_bf16(xf[u][mt][j], ones, j * 32 % G == 0 ? zero : xs[u][g][mt]);
+          f32x4& sum = xs[SUMS ? 0 : u][g][mt];  // tokens 4 s + r, in every column
+          sum = mfma_bf16(xf[u][mt][j], ones, j * 32 % G == 0 ? zero : sum);
+          if (SUMS && col == 0) *reinterpret_cast<f32x4*>(xsum + (mt * 4 * NC + u * NG + g) * 16 + 4 * s) = sum;
           if (p.rms) sq[mt] = mfma_bf16(xf[u][mt][j], xf[u][mt][j], sq[mt]);
         }
 #pragma unroll
@@ -260,6 +269,12 @@ __global__ void __launch_bounds__(WAVES * 64, 8 / WAVES) gemv_q4_stream_kernel(G
     }
   }
   lds_sync();
+  if constexpr (SUMS) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) xa[c][mt] = xsum[(mt * 4 * NC + 4 * c + s) * 16 + col];
+  }
   float scl[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
@@ -277,6 +292,17 @@ __global__ void __launch_bounds__(WAVES * 64, 8 / WAVES) gemv_q4_stream_kernel(G
     f32x4 acc[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) acc[mt] = zero;
+    if constexpr (SUMS) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {  // (NG 4: the groups of unit c)
+        uint32_t sz = t.sz[c][0];  // of this lane's group
+#pragma unroll
+        for (int g = 1; g < NG; ++g) sz = s == g ? t.sz[c][g] : sz;
+        const float zo = __builtin_fmaf(-16.f, q4_lo(sz), q4_hi(sz));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(xa[c][mt], zo, acc[mt], 0, 0, 0);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < UPW; ++u)
 #pragma unroll
@@ -294,8 +320,10 @@ __global__ void __launch_bounds__(WAVES * 64, 8 / WAVES) gemv_q4_stream_kernel(G
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            acc[mt][r] = __builtin_fmaf(sc, d[mt][r], __builtin_fmaf(zo, xs[u][g][mt][r], acc[mt][r]));
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (SUMS) acc[mt][r] = __builtin_fmaf(sc, d[mt][r], acc[mt][r]);
+            else acc[mt][r] = __builtin_fmaf(sc, d[mt][r], __builtin_fmaf(zo, xs[u][g][mt][r], acc[mt][r]));
+          }
       }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -380,7 +408,7 @@ static void launch_gemv_q4_shape(const GemvQ4Params& p, hipStream_t st) {
 }
 
 // Two workgroups of 4 waves per CU, or one of 8 where the rows need more registers (x and
-// its sums: 24 per unit and token tile, 32 with groups of 32).  Measured against workgroups
+// its sums: 24 per unit and token tile; groups of 32: 32 with one token tile, 17 with two).  Measured against workgroups
 // of a few tiles (us, groups of 64; 1, 8 and 32 rows of x): 8192 tiles, K 960 14.3, 15.5, 22.6
 // against 16.7, 17.6, 29.6; K 2048 -, -, 41.9 against 31.8, 34.2, 52.2 (8 rows, streamed:
 // 35.3); K 2944 -, -, 53.9 against 44.1, 47.6, 72.6; K 1536 with 1280 tiles 8.0, 8.1, 13.0
@@ -389,19 +417,18 @@ static void launch_gemv_q4_shape(const GemvQ4Params& p, hipStream_t st) {
 template <int EPI, int G, int MT>
 static void launch_gemv_q4_stream(const GemvQ4Params& p, int units, hipStream_t st) {
   if constexpr (EPI != SAGA_GEMV_ADD) {
-    constexpr bool wide = MT == 2 && G == 32;
     const int pairs = (p.N / 16 + 1) / 2;
     const dim3 two(std::min(pairs, 512)), one(std::min(pairs, 256));
     if (units <= 4) {
       hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 1>), two, dim3(256), 0, st, p);
     } else if (units <= 8) {
       hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 2>), two, dim3(256), 0, st, p);
-    } else if (units <= 12 && !wide) {
-      if constexpr (!wide) hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 3>), two, dim3(256), 0, st, p);
+    } else if (units <= 12) {
+      hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 4, 3>), two, dim3(256), 0, st, p);
     } else if (units <= 16) {
       if constexpr (MT == 2) hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 8, 2>), one, dim3(512), 0, st, p);
     } else {
-      if constexpr (MT == 2 && !wide)
+      if constexpr (MT == 2 && G > 32)
         hipLaunchKernelGGL((gemv_q4_stream_kernel<EPI, G, MT, 8, 3>), one, dim3(512), 0, st, p);
     }
   }

@@ -89,6 +89,24 @@ def test_gemv_q4_add_and_silu(M, N, K, group):
     _close(ops.gemv_q4(x, w, rms_eps=1e-6, epilogue="silu_pairs"), want, HALF[torch.bfloat16] * (want.abs() + tol) + tol)
 
 
+@pytest.mark.parametrize("M,N,K", [(32, 4144, 1824), (19, 4112, 1280), (17, 4096, 1536), (24, 8208, 480), (31, 4112, 2048)])
+def test_gemv_q4_streamed_32_rows(M, N, K):
+    """Groups of 32 under 17 to 32 rows: sums of x as operands; NaN stays in its row of x and its row of W."""
+    g = _gen(N + K + 1)
+    x = _randn(g, M, K, dtype=torch.bfloat16)
+    w = ops.quantize_gemv_weight(0.05 * _randn(g, N, K) + 0.02, 32)
+    ref, size = _gemv_ref(x, w, 1e-6)
+    got = ops.gemv_q4(x, w, rms_eps=1e-6)
+    _close(got, ref, HALF[torch.bfloat16] * (ref.abs() + size) + size)
+    w.scales[N // 16 - 1, K // 32 - 1, 5] = float("nan")
+    x[M - 1, 3] = float("nan")
+    bad = ops.gemv_q4(x, w, rms_eps=1e-6)
+    n = N - 16 + 5
+    assert bad[:, n].isnan().all() and bad[M - 1].isnan().all()
+    keep = torch.arange(N, device="cuda") != n
+    assert torch.equal(bad[: M - 1][:, keep], got[: M - 1][:, keep])
+
+
 def test_gemv_q4_special_values():
     """Rows of x do not meet each other; constant, tiny and one-sided groups; a NaN offset reaches its own row."""
     g = _gen(3)
