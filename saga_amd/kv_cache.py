@@ -37,10 +37,17 @@ def _check_bits(name: str, bits: int) -> None:
         raise ValueError(f"{name} must be 16 or 4, got {bits}")
 
 
+def _check_q4_rows(d: int, group: int) -> None:
+    if d not in (64, 128) or group not in (32, 64):
+        raise ValueError(f"a 4-bit cache needs a head dim of 64 or 128 and groups of 32 or 64, got {d} and {group}")
+
+
 def kv_cache_bytes(shape, batch: int, max_len: int, dtype=torch.bfloat16, bits: int = 16, group: int = 64) -> int:
     """Bytes of the K and V caches of every layer; bits 4: codes and the scales of groups of `group` dims."""
     _check_bits("bits", bits)
     d = shape.head_dim
+    if bits == 4:
+        _check_q4_rows(d, group)
     row = d * _es(dtype) if bits == 16 else d // 2 + 4 * (d // group)
     return shape.layers * batch * (shape.n_k + shape.n_v) * max_len * row
 
@@ -53,6 +60,8 @@ def decode_weight_bytes(shape, dtype=torch.bfloat16, decode_copies: bool = True,
     gate/up, packed o and down, normed LM head), with bits=4 in codes and
     scales (rows padded to 128 columns)."""
     _check_bits("bits", bits)
+    if bits == 4 and group not in (32, 64, 128):
+        raise ValueError(f"4-bit weights need groups of 32, 64 or 128 columns, got {group}")
     es = _es(dtype)
     s = shape
     per_layer = (s.qkv_width * s.hidden + s.qkv_width + s.hidden * s.n_q * s.head_dim + 2 * s.intermediate * s.hidden
@@ -170,8 +179,6 @@ class KVCache:
         dev = torch.device(device)
         d = shape.head_dim
         _check_bits("bits", bits)
-        if bits == 4 and (d not in (64, 128) or group not in (32, 64)):
-            raise ValueError(f"a 4-bit cache needs a head dim of 64 or 128 and groups of 32 or 64, got {d} and {group}")
         need = kv_cache_bytes(shape, batch, max_len, dtype, bits, group)
         if check_free and dev.type == "cuda":
             free, _ = torch.cuda.mem_get_info(dev)

@@ -243,6 +243,17 @@ def test_decoder_and_planner_options():
             SagaDecoder(tiny, 2, 32, device="cpu", **kw)
 
 
+def test_sizes_of_layouts_without_kernels_are_refused():
+    from saga_amd.decoder import QWEN25_15B_SAGA, DecoderShape
+    from saga_amd.kv_cache import decode_weight_bytes, kv_cache_bytes, plan_capacity
+    s, odd = QWEN25_15B_SAGA, DecoderShape(2, 96, 3, 1, 1, 32, 128, 256, 1e4, 1e-6)
+    for call in (lambda: kv_cache_bytes(s, 8, 64, bits=4, group=128), lambda: kv_cache_bytes(odd, 8, 64, bits=4, group=32),
+                 lambda: plan_capacity(s, batch=8, kv_bits=4, group=128), lambda: decode_weight_bytes(s, bits=4, group=16)):
+        with pytest.raises(ValueError, match="groups of 32"):
+            call()
+    assert plan_capacity(s, batch=8, weight_bits=4, group=128).max_len > 0
+
+
 def test_command_line_options():
     import argparse
     from saga_amd import speedup
