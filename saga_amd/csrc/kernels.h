@@ -370,7 +370,7 @@ struct DenseQ4Params {
   void* out;
   int32_t out_dt;
   int64_t o_sb, o_sh;
-  float* part;  // [b * q_h][nsplit][2 + d]
+  float* part;  // sums [b * q_h][nsplit][d], then (reference, sum of weights) [b * q_h][nsplit][2]
   int32_t nsplit, split_len;
 };
 void dense_q4_plan(int64_t units, int64_t L, int64_t* nsplit, int64_t* split_len);
