@@ -417,7 +417,8 @@ int saga_prefill_attention(const saga_tensor* query, const saga_tensor* key, con
  * (maximum - z) / 15 and c = (value - z) / s rounded to the nearest (ties to
  * even), so that a value is off by at most s / 2.  A group that holds a NaN, an
  * infinity or a magnitude above 65504 is stored as s = z = NaN: it reads back
- * as NaN.
+ * as NaN.  z + 15 s may pass 65504 by up to 15 steps of s: results of type f16
+ * computed from such values end at +-65504.
  *
  * A key / value cache of Lmax positions, groups along the head dim d (64 or
  * 128), all groups of one size (32 or 64) in k and v:

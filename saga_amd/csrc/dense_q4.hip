@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(256, 2) dense_q4_kernel(DenseQ4Params p) {
       a += Wo[(q * 16 + hh) * WROW + dd] * f;
     }
     if (p.nsplit == 1) {
-      store_from_f32(p.out, p.out_dt, bi * p.o_sb + static_cast<int64_t>(h0 + hh) * p.o_sh + dd, a / l);
+      store_from_f32(p.out, p.out_dt, bi * p.o_sb + static_cast<int64_t>(h0 + hh) * p.o_sh + dd, q4_in_range(a / l, p.out_dt));
     } else {
       const int64_t at = (static_cast<int64_t>(bi) * p.q_h + h0 + hh) * p.nsplit + split;
       p.part[at * D + dd] = a;
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(GR * JD) dense_q4_join_kernel(DenseQ4Params p)
     float t = og[0][i];
 #pragma unroll
     for (int q = 1; q < GR; ++q) t += og[q][i];
-    store_from_f32(p.out, p.out_dt, bi * p.o_sb + static_cast<int64_t>(h) * p.o_sh + d0 + i, t / l);
+    store_from_f32(p.out, p.out_dt, bi * p.o_sb + static_cast<int64_t>(h) * p.o_sh + d0 + i, q4_in_range(t / l, p.out_dt));
   }
 }
 

@@ -233,6 +233,8 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(KvQ4ReadParams p) {
       }
     }
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = q4_in_range(x[e], p.dt);
   if (is_v) store8(p.v, p.dt, static_cast<int64_t>(n) * p.v_sn + static_cast<int64_t>(h) * p.v_sh + 8 * t, p.vec, x);
   else store8(p.k, p.dt, static_cast<int64_t>(n) * p.k_sn + static_cast<int64_t>(h) * p.k_sh + 8 * t, p.vec, x);
 }

@@ -1,0 +1,49 @@
+"""Limits of the 4-bit forms on the GPU: values at the end of the range of f16."""
+import pytest
+import torch
+
+import q4_util as Q
+from saga_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("d,group", [(64, 32), (64, 64), (128, 32), (128, 64)])
+def test_values_at_the_end_of_the_f16_range_stay_finite(d, group):
+    """A scale is rounded up, so that a group from -60000 to 65504 (z -60000, s 8368, c 15) reads as 65520, which f16
+    would round to infinity: reads and attention of f16 stay at 65504."""
+    g = torch.Generator(device="cuda").manual_seed(d + group)
+    n, L = 3, 700
+    x = (torch.rand(n, 3, d, generator=g, device="cuda") * 100000 - 50000).half().float()
+    x[..., ::8], x[..., 3::8] = -60000.0, 65504.0
+    held = Q.values(*_grouped(x, group), torch.float32)
+    assert float(held.max()) == 65520.0 and not held.half().isfinite().all()
+    cache = Q.random_cache(g, n, 1, 1, L, d, group)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    table = torch.tensor([1.0, 0.0], device="cuda").expand(n, d // 2, 2).contiguous()  # no rotation
+    ops.rope_kv_append_q4(x.flatten(1).half(), 1, table, pos, cache)
+    for got, want in zip(ops.read_kv_q4(cache, pos, dtype=torch.float16), (held[:, 1:2], held[:, 2:3])):
+        assert torch.equal(got, want.clamp(max=65504.0).half())
+    for got, want in zip(ops.read_kv_q4(cache, pos, dtype=torch.float32), (held[:, 1:2], held[:, 2:3])):
+        assert torch.equal(got, want)
+    # attention over the one key that the mask leaves, in one block and in several splits; over none of them NaN
+    for length in (3, L):
+        part = ops.KVQ4(*(t[:, :, :length].contiguous() for t in cache))
+        mask = torch.full((n, 1, 1, length), float("-inf"), device="cuda")
+        for i in range(n - 1):
+            mask[i, 0, 0, i] = 0
+        for dtype in (torch.float16, torch.bfloat16):
+            q = torch.zeros(n, 2, 1, d, dtype=dtype, device="cuda")
+            out = ops.dense_decode_q4(q, part, attention_mask=mask, out_dtype=torch.float16)[:, :, 0]
+            want = held[:, 2].clamp(max=65504.0)
+            # a weight's terms keep 16 bits of p s c, the offset and the sums 2^-20 of p s (128 + c)
+            tol = 2.0 ** -11 * want.abs() + 2.0 ** -17 * 15 * 8368 + 2.0 ** -20 * 143 * 8368
+            assert bool(((out[:-1].float() - want[:-1, None]).abs() <= tol[:-1, None]).all())
+            assert out[:-1].isfinite().all() and out[-1].isnan().all()
+    cache.v_scales[0, 0, 0, 0] = float("inf")  # what is infinite stays so
+    assert not ops.read_kv_q4(cache, pos, dtype=torch.float16)[1][0, 0, :group].isfinite().any()
+
+
+def _grouped(x, group):
+    codes, sz = Q.quantise(x.cpu(), group)
+    return codes.cuda(), sz.cuda()
