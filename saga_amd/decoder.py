@@ -236,33 +236,41 @@ class SagaDecoder:
                                "(construct with keep_source_weights=True to fold new norm weights)")
         s = self.shape
         with torch.no_grad():
-            self.kw_qkv = [(self.w_qkv[l].float() * self.ln1[l].float()).to(self.dtype) for l in range(s.layers)]
+            def qkv(l):
+                w = (self.w_qkv[l].float() * self.ln1[l].float()).to(self.dtype)
+                return w if order is None else w.index_select(0, order).contiguous()
+
+            def gate_up(l):
+                w = (self.w_gu[l].float() * self.ln2[l].float()).to(self.dtype)
+                return torch.stack([w[:s.intermediate], w[s.intermediate:]], dim=1).reshape(2 * s.intermediate, s.hidden)
+
+            order = None
             self.kb_qkv = self.b_qkv
             if self.fuse_rope:
                 order = ops.rope_pair_order(s.n_q, s.n_k, s.n_v, s.head_dim, device=self.device)
-                self.kw_qkv = [w.index_select(0, order).contiguous() for w in self.kw_qkv]
                 self.kb_qkv = [b.index_select(0, order).contiguous() for b in self.b_qkv]
-            self.kw_gu = []
-            for l in range(s.layers):
-                w = (self.w_gu[l].float() * self.ln2[l].float()).to(self.dtype)
-                self.kw_gu.append(torch.stack([w[:s.intermediate], w[s.intermediate:]], dim=1)
-                                  .reshape(2 * s.intermediate, s.hidden).contiguous())
-            self.kw_lm = (self.lm_head.float() * self.ln_f.float()).to(self.dtype)
-            self.kw_o = list(self.w_o)
-            self.kw_d = list(self.w_d)
+            head = (self.lm_head.float() * self.ln_f.float()).to(self.dtype)
+            layers = range(s.layers)
             if self.weight_bits == 4:
+                # one folded weight at a time: beside the sources there is never more than the 4-bit
+                # copies, which is what plan_capacity counts
                 def q4(w):
                     return ops.quantize_gemv_weight(w, self.weight_group)
 
-                self.kw_qkv, self.kw_gu, self.kw_o, self.kw_d = (
-                    [q4(w) for w in ws] for ws in (self.kw_qkv, self.kw_gu, self.kw_o, self.kw_d))
-                self.kw_lm = q4(self.kw_lm)
+                self.kw_lm = q4(head)
+                del head
+                self.kw_qkv, self.kw_gu = [q4(qkv(l)) for l in layers], [q4(gate_up(l)) for l in layers]
+                self.kw_o, self.kw_d = [q4(w) for w in self.w_o], [q4(w) for w in self.w_d]
                 self._ones = torch.ones(s.hidden, device=self.device, dtype=self.dtype)
                 if not self.keep_source_weights:
                     self.w_qkv = self.w_o = self.w_gu = self.w_d = None
                     if self.lm_head is not self.embed:
                         self.lm_head = None
-            elif self.pack_weights:
+                return
+            self.kw_lm = head
+            self.kw_qkv, self.kw_gu = [qkv(l) for l in layers], [gate_up(l) for l in layers]
+            self.kw_o, self.kw_d = list(self.w_o), list(self.w_d)
+            if self.pack_weights:
                 # MFMA-fragment order: every fragment 1 KB contiguous.  The
                 # projections of few 16-row tiles (q/k/v, o, down: 96-120 at
                 # the 1.5B shape) in 8-row tiles when the batch allows (<= 8

@@ -1,4 +1,4 @@
-"""Limits of the 4-bit forms on the GPU: values at the end of the range of f16."""
+"""Limits of the 4-bit forms on the GPU: values at the end of the range of f16, the memory of a decoder's construction."""
 import pytest
 import torch
 
@@ -47,3 +47,22 @@ def test_values_at_the_end_of_the_f16_range_stay_finite(d, group):
 def _grouped(x, group):
     codes, sz = Q.quantise(x.cpu(), group)
     return codes.cuda(), sz.cuda()
+
+
+def test_a_decoder_is_built_within_its_planned_memory():
+    """Construction needs the source weights, the 4-bit copies, caches and workspaces that the planner counts, and
+    one weight's temporaries at a time: not the norm-folded bf16 copies of all layers (35 MB a layer here)."""
+    from saga_amd.decoder import DecoderShape, SagaDecoder
+    from saga_amd.kv_cache import plan_capacity
+    s = DecoderShape(40, 1024, 8, 1, 2, 64, 8192, 2048, 1e6, 1e-6, True)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    m = SagaDecoder(s, 4, 512, mode="dense", kv_bits=4, weight_bits=4)
+    peak = torch.cuda.max_memory_allocated() - before
+    plan = plan_capacity(s, batch=4, budget_bytes=1 << 37, kv_bits=4, weight_bits=4)
+    planned = plan.weight_bytes + plan.workspace_bytes + m.kv.nbytes
+    one = 4 * 2 * s.intermediate * s.hidden  # the largest weight in fp32
+    print(f"peak {peak / 1e6:.0f} MB, planned {planned / 1e6:.0f} MB, one weight {one / 1e6:.0f} MB", flush=True)
+    assert peak <= planned + 8 * one < planned + 40 * 35e6
