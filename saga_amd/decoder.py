@@ -32,7 +32,8 @@ import torch
 
 from . import ops
 from .attention.attention import sdpa_attention_forward
-from .kv_cache import KVCache, kv_cache_bytes  # noqa: F401  (kv_cache_bytes re-exported)
+from .kv_cache import (KVCache, check_q4_decoder, kv_cache_bytes, projection_shapes,  # noqa: F401  (kv_cache_bytes re-exported)
+                       skinny_gemm_supported)
 
 
 @dataclass(frozen=True)
@@ -107,12 +108,9 @@ class SagaDecoder:
                  weight_group: int = 64):
         if mode not in ("atopn", "dense", "vanilla"):
             raise ValueError(f"mode must be 'atopn', 'dense' or 'vanilla', got {mode!r}")
-        if kv_bits not in (4, 16) or weight_bits not in (4, 16):
-            raise ValueError(f"kv_bits and weight_bits must be 16 or 4, got {kv_bits} and {weight_bits}")
-        if kv_bits == 4 and (mode != "dense" or dtype not in (torch.bfloat16, torch.float16)):
-            raise ValueError("kv_bits=4 needs mode 'dense' and bf16 or f16")
-        if weight_bits == 4 and weight_group not in (32, 64, 128):
-            raise ValueError(f"weight_group must be 32, 64 or 128, got {weight_group}")
+        if kv_bits == 4 and mode != "dense":
+            raise ValueError("kv_bits=4 needs mode 'dense'")
+        check_q4_decoder(shape, batch, dtype, kv_bits, kv_group, weight_bits, weight_group)
         self.kv_bits, self.weight_bits, self.weight_group = kv_bits, weight_bits, weight_group
         self.shape, self.batch, self.max_len, self.mode, self.top_n = shape, batch, max_len, mode, top_n
         self.exempt = set(exempt_layers)
@@ -157,10 +155,7 @@ class SagaDecoder:
         self._act = torch.empty(batch, s.intermediate, device=self.device, dtype=dtype)
         self._logits = torch.empty(batch, s.vocab, device=self.device, dtype=dtype)
         # decode projections: the skinny-GEMM kernel for up to 32 token rows
-        self.use_gemv = (batch <= 32 and dtype == torch.bfloat16 and s.hidden % 32 == 0 and s.intermediate % 32 == 0
-                         and (s.n_q * d) % 32 == 0 and s.qkv_width % 16 == 0 and s.vocab % 16 == 0)
-        if weight_bits == 4 and (not self.use_gemv or any(k % weight_group for k in (s.hidden, s.n_q * d, s.intermediate))):
-            raise ValueError("weight_bits=4 needs bf16, a batch of at most 32 and widths that are multiples of weight_group")
+        self.use_gemv = skinny_gemm_supported(s, batch, dtype)
         # q/k/v projection, RoPE and cache append in one launch (pair-ordered rows)
         self.fuse_rope = fuse_rope and self.use_gemv and d % 16 == 0 and kv_bits == 16 and weight_bits == 16
         self.pack_weights = pack_weights
@@ -307,10 +302,8 @@ class SagaDecoder:
                                        for cal in (True, False)))
             self.ws["dense"] = buf(lib.saga_dense_workspace_bytes(B, s.n_q, L, d))
         if self.use_gemv:
-            shapes = ((s.qkv_width, s.hidden), (s.hidden, s.n_q * d), (2 * s.intermediate, s.hidden),
-                      (s.hidden, s.intermediate), (s.vocab, s.hidden))
             need = lib.saga_gemv_q4_workspace_bytes if self.weight_bits == 4 else lib.saga_gemv_workspace_bytes
-            self.ws["gemv"] = buf(max(need(B, n, k) for n, k in shapes))
+            self.ws["gemv"] = buf(max(need(B, n, k) for n, k in projection_shapes(s)))
             self.ws["argmax"] = buf(lib.saga_argmax_workspace_bytes(B, s.vocab))
 
     def _prefill_layer(self, l: int):

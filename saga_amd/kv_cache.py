@@ -42,6 +42,34 @@ def _check_q4_rows(d: int, group: int) -> None:
         raise ValueError(f"a 4-bit cache needs a head dim of 64 or 128 and groups of 32 or 64, got {d} and {group}")
 
 
+def projection_shapes(shape):
+    """(rows, columns) of a layer's q/k/v, o, gate/up and down projections, and of the LM head."""
+    s = shape
+    return ((s.qkv_width, s.hidden), (s.hidden, s.n_q * s.head_dim), (2 * s.intermediate, s.hidden),
+            (s.hidden, s.intermediate), (s.vocab, s.hidden))
+
+
+def skinny_gemm_supported(shape, batch: int, dtype) -> bool:
+    """Whether a decoder's projections run through the skinny GEMM (ops.gemv, ops.gemv_q4)."""
+    return (batch <= 32 and dtype == torch.bfloat16 and shape.hidden % 32 == 0 and shape.intermediate % 32 == 0
+            and (shape.n_q * shape.head_dim) % 32 == 0 and shape.qkv_width % 16 == 0 and shape.vocab % 16 == 0)
+
+
+def check_q4_decoder(shape, batch: int, dtype, kv_bits: int, kv_group: int, weight_bits: int, weight_group: int) -> None:
+    """ValueError for caches or weights in 4 bits that SagaDecoder does not take."""
+    _check_bits("kv_bits", kv_bits)
+    _check_bits("weight_bits", weight_bits)
+    if kv_bits == 4:
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("kv_bits=4 needs bf16 or f16")
+        _check_q4_rows(shape.head_dim, kv_group)
+    if weight_bits == 4:
+        if weight_group not in (32, 64, 128):
+            raise ValueError(f"weight_group: 4-bit weights need groups of 32, 64 or 128 columns, got {weight_group}")
+        if not skinny_gemm_supported(shape, batch, dtype) or any(k % weight_group for _, k in projection_shapes(shape)):
+            raise ValueError("weight_bits=4 needs bf16, a batch of at most 32 and widths that are multiples of weight_group")
+
+
 def kv_cache_bytes(shape, batch: int, max_len: int, dtype=torch.bfloat16, bits: int = 16, group: int = 64) -> int:
     """Bytes of the K and V caches of every layer; bits 4: codes and the scales of groups of `group` dims."""
     _check_bits("bits", bits)
@@ -58,10 +86,11 @@ def decode_weight_bytes(shape, dtype=torch.bfloat16, decode_copies: bool = True,
     q/k/v (+ bias), o, gate/up and down projections, norms.  decode_copies:
     plus the decode-layout copies the skinny GEMM reads (norm-folded q/k/v and
     gate/up, packed o and down, normed LM head), with bits=4 in codes and
-    scales (rows padded to 128 columns)."""
+    scales (rows padded to 128 columns).  A decoder releases the row-major
+    projections once its copies are made: both are there until then."""
     _check_bits("bits", bits)
-    if bits == 4 and group not in (32, 64, 128):
-        raise ValueError(f"4-bit weights need groups of 32, 64 or 128 columns, got {group}")
+    if bits == 4 and (group not in (32, 64, 128) or any(k % group for _, k in projection_shapes(shape))):
+        raise ValueError(f"4-bit weights need groups of 32, 64 or 128 columns that divide every width, got {group}")
     es = _es(dtype)
     s = shape
     per_layer = (s.qkv_width * s.hidden + s.qkv_width + s.hidden * s.n_q * s.head_dim + 2 * s.intermediate * s.hidden
@@ -69,19 +98,19 @@ def decode_weight_bytes(shape, dtype=torch.bfloat16, decode_copies: bool = True,
     base = (s.vocab * s.hidden + s.layers * per_layer + s.hidden) * es
     if not decode_copies:
         return base
+
     def copy(n, k):
         return n * k * es if bits == 16 else n * ((k + 127) // 128 * 64 + 4 * (k // group))
 
-    copies = (s.layers * (copy(s.qkv_width, s.hidden) + copy(2 * s.intermediate, s.hidden)
-                          + copy(s.hidden, s.n_q * s.head_dim) + copy(s.hidden, s.intermediate))
-              + copy(s.vocab, s.hidden))
-    return base + copies
+    *layer, head = (copy(n, k) for n, k in projection_shapes(s))
+    return base + s.layers * sum(layer) + head
 
 
-def decode_workspace_bytes(shape, batch: int, max_len: int, top_n: int, kv_bits: int = 16) -> int:
+def decode_workspace_bytes(shape, batch: int, max_len: int, top_n: int, kv_bits: int = 16,
+                           weight_bits: int = 16) -> int:
     """Atop-N and dense decode workspaces of one layer call (shared by all
-    layers; a 4-bit cache: its dense workspace) plus the per-step activations
-    and the threshold table."""
+    layers; a 4-bit cache: its dense workspace), the projections' (of 16- or
+    4-bit weights), plus the per-step activations and the threshold table."""
     from . import _lib
     lib = _lib.load()
     s = shape
@@ -90,7 +119,10 @@ def decode_workspace_bytes(shape, batch: int, max_len: int, top_n: int, kv_bits:
     else:
         ws = lib.saga_atopn_workspace_bytes(batch, s.n_q, s.n_k, max_len, s.head_dim, min(2 * top_n, max_len))
         ws += lib.saga_dense_workspace_bytes(batch, s.n_q, max_len, s.head_dim)
-    ws += lib.saga_gemv_workspace_bytes(batch, s.hidden, s.intermediate)
+    if weight_bits == 4:
+        ws += max(lib.saga_gemv_q4_workspace_bytes(batch, n, k) for n, k in projection_shapes(s))
+    else:
+        ws += lib.saga_gemv_workspace_bytes(batch, s.hidden, s.intermediate)
     ws += s.layers * batch * s.n_q * 4
     ws += batch * (3 * s.hidden + s.qkv_width + 2 * s.intermediate + s.vocab) * 2
     return int(ws)
@@ -118,24 +150,31 @@ class CapacityPlan:
 
 def plan_capacity(shape, batch: Optional[int] = None, max_len: Optional[int] = None, budget_bytes: Optional[int] = None,
                   reserve_fraction: float = 0.05, top_n: int = 512, dtype=torch.bfloat16,
-                  align: int = 256, kv_bits: int = 16, weight_bits: int = 16, group: int = 64) -> CapacityPlan:
+                  align: int = 256, kv_bits: int = 16, weight_bits: int = 16, group: int = 64,
+                  kv_group: Optional[int] = None, weight_group: Optional[int] = None) -> CapacityPlan:
     """The largest max_len for a given batch, or the largest batch for a given
     max_len (give exactly one), that fits budget_bytes (default: the current
     device's total memory, else 288 GB) minus reserve_fraction, next to the
     decode weights (with their decode copies) and workspaces.  max_len is
     rounded down to a multiple of `align` positions.  kv_bits, weight_bits:
-    caches and decode copies in 4 bits (groups of `group`)."""
+    caches and decode copies in 4 bits, in groups of kv_group and weight_group
+    (`group` where not given); what SagaDecoder refuses is refused, and a
+    batch searched for ends at the 32 rows that 4-bit weights take."""
     if (batch is None) == (max_len is None):
         raise ValueError("give exactly one of batch and max_len")
+    kv_group, weight_group = kv_group or group, weight_group or group
+    check_q4_decoder(shape, batch or 1, dtype, kv_bits, kv_group, weight_bits, weight_group)
     if budget_bytes is None:
         budget_bytes = (torch.cuda.get_device_properties(0).total_memory if torch.cuda.is_available()
                         else HBM_BYTES_MI355X)
     avail = int(budget_bytes * (1 - reserve_fraction))
-    wbytes = decode_weight_bytes(shape, dtype, bits=weight_bits, group=group)
+    wbytes = decode_weight_bytes(shape, dtype, bits=weight_bits, group=weight_group)
 
     def fits(b: int, L: int) -> Optional[CapacityPlan]:
-        kv = kv_cache_bytes(shape, b, L, dtype, kv_bits, group)
-        ws = decode_workspace_bytes(shape, b, L, top_n, kv_bits)
+        if weight_bits == 4 and b > 32:
+            return None
+        kv = kv_cache_bytes(shape, b, L, dtype, kv_bits, kv_group)
+        ws = decode_workspace_bytes(shape, b, L, top_n, kv_bits, weight_bits)
         if kv + wbytes + ws > avail:
             return None
         return CapacityPlan(b, L, kv, wbytes, ws, budget_bytes)
