@@ -1256,7 +1256,8 @@ int saga_rope_kv_append_q4(const saga_tensor* qkv, int64_t n_q, const float* rop
   if (qkv->shape[1] < heads * d) return fail(SAGA_ERR_INVALID, "qkv: row shorter than (n_q + n_k + n_v) * d");
   if (qkv->stride[1] != 1 || q_out->stride[2] != 1) return fail(SAGA_ERR_INVALID, "innermost strides must be 1");
   if (!batch && N > p.kv.B) return fail(SAGA_ERR_INVALID, "without batch indices N must be <= B");
-  if (N >= (1LL << 26)) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");  // a launch holds less than 2^32 threads
+  // (four tokens a block of 256 threads; a launch holds less than 2^32 threads)
+  if (N > (1LL << 26) - 4) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
   p.qkv = qkv->data;
   p.qkv_ld = qkv->stride[0];
   p.q_out = q_out->data;

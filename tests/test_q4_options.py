@@ -55,3 +55,23 @@ def test_workspaces_of_4_bit_weights_are_the_4_bit_projections():
         rest = decode_workspace_bytes(s, batch, 4096, 512) - lib.saga_gemv_workspace_bytes(batch, s.hidden, s.intermediate)
         need = max(lib.saga_gemv_q4_workspace_bytes(batch, n, k) for n, k in projection_shapes(s))
         assert decode_workspace_bytes(s, batch, 4096, 512, weight_bits=4) == rest + need
+
+
+def _t(shape, dtype, strides):
+    d = _lib.SagaTensor()
+    d.data, d.dtype, d.ndim = 0x100000, dtype, len(shape)
+    for i, (n, s) in enumerate(zip(shape, strides)):
+        d.shape[i], d.stride[i] = n, s
+    return d
+
+
+def test_append_refuses_more_tokens_than_a_launch_holds():
+    """Four tokens a block of 256 threads, less than 2^32 threads: at most 2^26 - 4 tokens."""
+    import ctypes
+    cache = _lib.KvQ4(*(_t((2, 1, 48, n), dt, (48 * n, 48 * n, n, 1))
+                        for n, dt in ((64, _lib.DTYPE_U8), (4, _lib.DTYPE_F16)) * 2))
+    for n in ((1 << 26) - 3, (1 << 26) - 1, 1 << 26):
+        qkv, q = _t((n, 3 * 128), _lib.DTYPE_BF16, (0, 1)), _t((n, 1, 128), _lib.DTYPE_BF16, (128, 128, 1))
+        assert _lib.load().saga_rope_kv_append_q4(ctypes.byref(qkv), 1, 0x300000, 0x300000, 0x300000, ctypes.byref(q),
+                                                  ctypes.byref(cache), None) == -2, n
+        assert "sizes too large" in _lib.load().saga_last_error().decode()
