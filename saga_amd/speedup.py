@@ -84,6 +84,12 @@ def _label(mode: str, param: Optional[int]) -> str:
     return f"{mode}:{param}" if param is not None else mode
 
 
+def _bits(args) -> str:
+    """What of a configuration is held in 4 bits: "", "kv4", "w4" or "kv4-w4"."""
+    names = [n for n, flag in (("kv4", "kv_bits"), ("w4", "weight_bits")) if getattr(args, flag, 16) == 4]
+    return "-".join(names)
+
+
 def build_decoder(model_path: str, merge: bool, new_heads: int, batch: int, max_len: int, mode: str,
                   top_n: int, exempt, dtype, **options):
     """The decoder of one configuration (random-init built-in shape or a
@@ -104,11 +110,12 @@ def build_decoder(model_path: str, merge: bool, new_heads: int, batch: int, max_
                        weights=weights, **options)
 
 
-def trace_name(profile_output: str, merge: bool, mode: str, param: Optional[int], batch: int, seq_len: int) -> str:
-    """The decode trace file of one configuration (speedup.py:657-658)."""
+def trace_name(profile_output: str, merge: bool, mode: str, param: Optional[int], batch: int, seq_len: int,
+               bits: str = "") -> str:
+    """The decode trace file of one configuration (speedup.py:657-658), with what it holds in 4 bits."""
     merge_label = "merged" if merge else "baseline"
     return (f"{profile_output.replace('.json', '')}_{merge_label}_{_label(mode, param).replace(':', '_')}"
-            f"_bs{batch}_seq{seq_len}.json")
+            f"{'_' + bits if bits else ''}_bs{batch}_seq{seq_len}.json")
 
 
 def run_config(args, mode: str, param: Optional[int], batch: int, seq_len: int, merge: bool) -> dict:
@@ -153,7 +160,7 @@ def run_config(args, mode: str, param: Optional[int], batch: int, seq_len: int, 
             lat.append((time.perf_counter() - t0) * 1000.0)
             if prof is not None:
                 prof.stop()
-                trace = trace_name(args.profile_output, merge, mode, param, batch, seq_len)
+                trace = trace_name(args.profile_output, merge, mode, param, batch, seq_len, _bits(args))
                 prof.export_chrome_trace(trace)
                 prof = None  # the first measured generation is traced (one trace per configuration)
                 print(f"decode trace: {trace}", file=sys.stderr, flush=True)
@@ -187,6 +194,8 @@ def describe_flags(args) -> str:
              f"{', --no_compile' if args.no_compile else ''} accepted)",
              "CUDA graph: " + ("enabled (HIP graphs: calibration step, fast step)" if args.cuda_graph
                                else "disabled (kernels launched eagerly per step)")]
+    if _bits(args):
+        lines.append(f"Held in 4 bits: {_bits(args)} (kv4: caches; w4: projections and LM head)")
     if args.calibrate_during_measurement:
         lines.append("Calibration during measurement: on (every measured generation starts with it)")
     if args.profile_decode:
@@ -262,10 +271,11 @@ def main(argv=None) -> int:
     for merge_mode in merge_modes:
         merge_label = "merged" if merge_mode == "merge" else "baseline"
         for mode, param in modes:
-            print(f"\n### {merge_label} / {_label(mode, param)} ###", flush=True)
+            label = f"{_label(mode, param)} {_bits(args)}".strip()
+            print(f"\n### {merge_label} / {label} ###", flush=True)
             for batch in batch_sizes:
                 for seq_len in seq_lengths:
-                    key = (merge_label, _label(mode, param), batch, seq_len)
+                    key = (merge_label, label, batch, seq_len)
                     try:
                         r = subprocess.run(_sub_cmd(args, mode, param, batch, seq_len, merge_mode),
                                            capture_output=True, text=True, timeout=args.timeout, env=env, cwd=root)
@@ -291,10 +301,11 @@ def main(argv=None) -> int:
     print("\n" + "=" * 70)
     print("SUMMARY")
     print("=" * 70)
-    print(f"{'Merge':<10} {'Attention':<12} {'BS':<6} {'Seq':<8} {'Mean (ms)':<12} {'P50 (ms)':<12} {'tok/s':<10}")
-    print("-" * 72)
+    width = max([12, *(len(attn) for _, attn, _, _ in results)])
+    print(f"{'Merge':<10} {'Attention':<{width}} {'BS':<6} {'Seq':<8} {'Mean (ms)':<12} {'P50 (ms)':<12} {'tok/s':<10}")
+    print("-" * (60 + width))
     for (merge, attn, bs, seq), s in results.items():
-        print(f"{merge:<10} {attn:<12} {bs:<6} {seq:<8} {s['mean_ms']:<12.3f} {s['p50_ms']:<12.3f} "
+        print(f"{merge:<10} {attn:<{width}} {bs:<6} {seq:<8} {s['mean_ms']:<12.3f} {s['p50_ms']:<12.3f} "
               f"{s['tokens_per_s']:<10.0f}")
     if failures:
         print(f"\n{len(failures)} configuration(s) FAILED: {failures}")

@@ -75,3 +75,32 @@ def test_append_refuses_more_tokens_than_a_launch_holds():
         assert _lib.load().saga_rope_kv_append_q4(ctypes.byref(qkv), 1, 0x300000, 0x300000, 0x300000, ctypes.byref(q),
                                                   ctypes.byref(cache), None) == -2, n
         assert "sizes too large" in _lib.load().saga_last_error().decode()
+
+
+def test_traces_and_headings_tell_the_bits(tmp_path, monkeypatch, capsys):
+    """A configuration in 4 bits has a trace of its own, and its heading, settings and summary row say so; without
+    them the names are the reference's."""
+    import subprocess
+    from saga_amd import speedup
+    assert speedup.trace_name("t.json", True, "full", None, 8, 4096) == "t_merged_full_bs8_seq4096.json"
+    names = set()
+    for flags in ([], ["--kv_bits", "4"], ["--weight_bits", "4"], ["--kv_bits", "4", "--weight_bits", "4"]):
+        seen = []
+
+        def run(cmd, **kw):  # a configuration's subprocess: what it would write and print
+            args = speedup.build_parser().parse_args(cmd[3:])
+            (mode, param), = speedup.parse_attention(args.attention)
+            seen.append(speedup.trace_name("t.json", True, mode, param, 8, 4096, speedup._bits(args)))
+            line = '{"mean_ms": 1.5, "std_ms": 0, "p50_ms": 1.4, "p90_ms": 1.6, "tokens_per_s": 5333}'
+            return subprocess.CompletedProcess(cmd, 0, stdout=line, stderr="")
+
+        monkeypatch.setattr(speedup.subprocess, "run", run)
+        assert speedup.main(["--batch_sizes", "8", "--seq_lengths", "4096", *flags]) == 0
+        out = capsys.readouterr().out
+        bits = "-".join(n for n, f in (("kv4", "--kv_bits"), ("w4", "--weight_bits")) if f in flags)
+        label = f"full {bits}".strip()
+        assert f"### merged / {label} ###" in out and f"merged     {label:<12} 8 " in out
+        assert ("Held in 4 bits: " + bits in out) == bool(flags)
+        names.update(seen)
+    assert len(names) == 4
+    assert speedup.trace_name("t.json", False, "atopn", 512, 8, 4096, "w4") == "t_baseline_atopn_512_w4_bs8_seq4096.json"
