@@ -14,6 +14,8 @@ Operators (namespace "saga"):
     scaling, kv_len) -> out [b, q_h, 1, d]        (attention/attention.py:173-189)
   * dense_decode(query, key, value, attention_mask, scaling, kv_len)
     -> out [b, q_h, 1, d]                         (attention/attention.py:64-85)
+  * dense_decode_q4(query, k_codes, k_scales, v_codes, v_scales, attention_mask,
+    scaling, kv_len) -> out [b, q_h, 1, d]        (the same over the parts of an ops.KVQ4)
   * prefill_attention(query, key, value, attention_mask, scaling, is_causal)
     -> out [b, l_q, q_h, d]                       (attention/attention.py:13-53)
 """
@@ -64,6 +66,19 @@ def dense_decode(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 
 @dense_decode.register_fake
 def _dense_decode_fake(query, key, value, attention_mask=None, scaling=None, kv_len=None):
+    return _out_like(query)
+
+
+@torch.library.custom_op("saga::dense_decode_q4", mutates_args=())
+def dense_decode_q4(query: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+                    v_scales: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
+                    scaling: Optional[float] = None, kv_len: Optional[torch.Tensor] = None) -> torch.Tensor:
+    return ops.dense_decode_q4(query, ops.KVQ4(k_codes, k_scales, v_codes, v_scales), attention_mask, scaling,
+                               kv_len=kv_len)
+
+
+@dense_decode_q4.register_fake
+def _dense_decode_q4_fake(query, k_codes, k_scales, v_codes, v_scales, attention_mask=None, scaling=None, kv_len=None):
     return _out_like(query)
 
 
