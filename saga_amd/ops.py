@@ -787,7 +787,8 @@ def unpack_gemv_q4(weights, heads=None):
         out = torch.empty(w.shape, dtype=torch.bfloat16, device=dev)
         items += (_lib.packed(w.codes), _lib.packed(w.scales), _lib.packed(out), _HEADS_PACK(*(h or (0, 0))))
         outs.append(out)
-    _on_device(dev, "unpack_gemv_q4", _lib.load().saga_unpack_gemv_q4, b"".join(items), len(outs))
+    if outs:
+        _on_device(dev, "unpack_gemv_q4", _lib.load().saga_unpack_gemv_q4, b"".join(items), len(outs))
     return outs
 
 

@@ -104,3 +104,9 @@ def test_traces_and_headings_tell_the_bits(tmp_path, monkeypatch, capsys):
         names.update(seen)
     assert len(names) == 4
     assert speedup.trace_name("t.json", False, "atopn", 512, 8, 4096, "w4") == "t_baseline_atopn_512_w4_bs8_seq4096.json"
+
+
+def test_opening_no_weights_gives_none():
+    """As unpack_gemv_weights."""
+    from saga_amd import ops
+    assert ops.unpack_gemv_weights([]) == [] and ops.unpack_gemv_q4([]) == []
