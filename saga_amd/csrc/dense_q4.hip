@@ -511,25 +511,35 @@ void dense_q4_plan(int64_t units, int64_t L, int64_t* nsplit, int64_t* split_len
   *nsplit = (L + sl - 1) / sl;
 }
 
-template <int D, int G, int NV>
+// Whether masked calls take units of NV value heads.  With four groups of each row the registers of
+// two value heads spill: 8 x 30k positions, 12 / 1 / 2 heads, 41 us as two units against 62.
+constexpr bool dense_q4_masked(int D, int G, int NV) { return NV == 1 || D / G < 4; }
+
+template <int D, int G, int QT, int NV>
 static void launch_dense_q4_typed(const DenseQ4Params& p, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.b * p.nseg * p.nsplit));
-  if (p.q_dt == SAGA_DTYPE_BF16) {
-    if (p.mask) hipLaunchKernelGGL((dense_q4_kernel<D, G, 1, NV, true>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((dense_q4_kernel<D, G, 1, NV, false>), grid, dim3(256), 0, st, p);
-  } else {
-    if (p.mask) hipLaunchKernelGGL((dense_q4_kernel<D, G, 2, NV, true>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((dense_q4_kernel<D, G, 2, NV, false>), grid, dim3(256), 0, st, p);
+  if constexpr (dense_q4_masked(D, G, NV)) {
+    if (p.mask) {
+      hipLaunchKernelGGL((dense_q4_kernel<D, G, QT, NV, true>), grid, dim3(256), 0, st, p);
+      return;
+    }
   }
+  hipLaunchKernelGGL((dense_q4_kernel<D, G, QT, NV, false>), grid, dim3(256), 0, st, p);
+}
+
+template <int D, int G, int QT>
+static void launch_dense_q4_units(const DenseQ4Params& p, int nv, hipStream_t st) {
+  if constexpr (D == 64) {
+    if (nv == 5) return launch_dense_q4_typed<D, G, QT, 5>(p, st);
+  }
+  if (nv == 2) return launch_dense_q4_typed<D, G, QT, 2>(p, st);
+  launch_dense_q4_typed<D, G, QT, 1>(p, st);
 }
 
 template <int D, int G>
 static void launch_dense_q4_group(const DenseQ4Params& p, int nv, hipStream_t st) {
-  if constexpr (D == 64) {
-    if (nv == 5) return launch_dense_q4_typed<D, G, 5>(p, st);
-  }
-  if (nv == 2) return launch_dense_q4_typed<D, G, 2>(p, st);
-  launch_dense_q4_typed<D, G, 1>(p, st);
+  if (p.q_dt == SAGA_DTYPE_BF16) launch_dense_q4_units<D, G, 1>(p, nv, st);
+  else launch_dense_q4_units<D, G, 2>(p, nv, st);
 }
 
 hipError_t launch_dense_decode_q4(DenseQ4Params& p, hipStream_t st) {
@@ -538,9 +548,10 @@ hipError_t launch_dense_decode_q4(DenseQ4Params& p, hipStream_t st) {
   const int n_k = p.q_h / p.g;
   int nv = p.g % p.g_v == 0 && p.g <= 16 ? p.g / p.g_v : 1;
   if (nv != 2 && !(nv == 5 && p.kv.d == 64)) nv = 1;
-  // (with a mask and four groups of each row the registers of two value heads spill: 8 x 30k
-  // positions, 12 / 1 / 2 heads, 41 us as two units against 62)
-  if (p.mask && p.kv.d == 128 && p.kv.group == 32) nv = 1;
+  // (the units of five value heads spill with a mask too, 14 to 77 registers, and pay for it only with
+  // groups of 32: 8 x 32768 positions, 15 / 1 / 5 heads of 64, bf16 and f16, 54 and 63 us against 47 and
+  // 50 as five units, with groups of 64 28 and 38 against 41 and 45)
+  if (p.mask && !dense_q4_masked(p.kv.d, p.kv.group, nv)) nv = 1;
   int64_t ns, sl;
   if (nv > 1) {
     // (not where that leaves most CUs without a block)
