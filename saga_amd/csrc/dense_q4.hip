@@ -3,8 +3,8 @@
 // A block takes one batch row, one unit of query heads (at most 16, the columns of
 // every product) and one split of the positions; its waves step through 32 positions
 // each and meet in LDS.  A unit is a key head with its NV whole value heads, or a run
-// of heads that share both.  With the codes c as b + c (q4.cuh), all products of a
-// step are bf16 MFMAs with 32-bit sums:
+// of heads that share both.  With the codes c as b + c (q4.cuh), b = 16 everywhere, all
+// products of a step are bf16 MFMAs with 32-bit sums:
 //   * x[h, j] = sum_g s_jg (q_h . c_j)_g + z_jg (sum q_h)_g: key rows straight from
 //     memory as the A operand, a chain per group that starts at - sum q b;
 //   * softmax with a running reference and sum in fp32: the reference moves only when
@@ -12,6 +12,9 @@
 //   * o[h, i] = sum_j (p_hj s_jg) (b + c_ji) - b sum_j p_hj s_jg + sum_j p_hj z_jg:
 //     p s is split into two bf16 terms (16 bits), the first two sums are MFMAs over
 //     the same terms, so that what the split loses meets c alone, the third is fp32.
+//     The sums with b grow with the positions while what they leave cancels: with b 128
+//     in one slot of four, an instruction less, those dims were off by 2e-4 of the
+//     output over 65541 positions, the others by 3e-5 (relative norms, in the same time).
 //     A lane's words of 8 positions are turned into rows of codes in registers.  A
 //     column's p s are those of its own value head, whose sums alone it keeps.
 // The (s, z) of a step go through wave-private LDS.  Kernel 2 joins the splits.
@@ -215,21 +218,17 @@ __global__ void __launch_bounds__(256, 2) dense_q4_kernel(DenseQ4Params p) {
   // query fragments: slots (2 k, 2 k + 1) of step j are dims 32 j + 8 s + (k, k + 4)
   u32x4 qf[NJ][QT];
   float qs[NG];   // sums over the groups, for head `col`
-  f32x4 qb[NG];   // minus the sums with each slot's b, in every row of a tile
+  f32x4 qb[NG];   // - b of them, in every row of a tile
   {
-    float b[NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) qs[g] = b[g] = 0.f;
+    for (int g = 0; g < NG; ++g) qs[g] = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       float f[8];
       if constexpr (QT == 1) unpack16<SAGA_DTYPE_BF16>(qraw[j], f);
       else unpack16<SAGA_DTYPE_F16>(qraw[j], f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        qs[j * 32 / G] += f[e];
-        b[j * 32 / G] -= (e % 4 == 0 ? 128.f : 16.f) * f[e];
-      }
+      for (int e = 0; e < 8; ++e) qs[j * 32 / G] += f[e];
 #pragma unroll
       for (int t = 0; t < QT; ++t)
 #pragma unroll
@@ -239,9 +238,8 @@ __global__ void __launch_bounds__(256, 2) dense_q4_kernel(DenseQ4Params p) {
     for (int g = 0; g < NG; ++g) {
       qs[g] += __shfl_xor(qs[g], 16);
       qs[g] += __shfl_xor(qs[g], 32);
-      b[g] += __shfl_xor(b[g], 16);
-      b[g] += __shfl_xor(b[g], 32);
-      qb[g] = f32x4{b[g], b[g], b[g], b[g]};
+      const float b = -16.f * qs[g];
+      qb[g] = f32x4{b, b, b, b};
     }
   }
 
@@ -276,7 +274,7 @@ __global__ void __launch_bounds__(256, 2) dense_q4_kernel(DenseQ4Params p) {
         dg[g] = qb[g];
 #pragma unroll
         for (int j = g * (G / 32); j < (g + 1) * (G / 32); ++j) {
-          const u32x4 a = q4_frag(r.k[t].w[j], qc);
+          const u32x4 a = q4_frag16(r.k[t].w[j], qc);
 #pragma unroll
           for (int q = 0; q < QT; ++q) dg[g] = mfma_16b<SAGA_DTYPE_BF16>(a, qf[j][q], dg[g]);
         }
@@ -365,7 +363,7 @@ __global__ void __launch_bounds__(256, 2) dense_q4_kernel(DenseQ4Params p) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) o[u][e] = mfma_16b<SAGA_DTYPE_BF16>(a, pf[16 * e / G][k], o[u][e]);
         };
-        tile(4 * hv + 0, u32x4{q4_pair<0>(two[0], qc), q4_pair<0>(two[1], qc), q4_pair<0>(two[2], qc), q4_pair<0>(two[3], qc)});
+        tile(4 * hv + 0, u32x4{q4_pair16<0>(two[0], qc), q4_pair16<0>(two[1], qc), q4_pair16<0>(two[2], qc), q4_pair16<0>(two[3], qc)});
         tile(4 * hv + 1, u32x4{q4_pair<1>(two[0], qc), q4_pair<1>(two[1], qc), q4_pair<1>(two[2], qc), q4_pair<1>(two[3], qc)});
         tile(4 * hv + 2, u32x4{q4_pair<2>(two[0], qc), q4_pair<2>(two[1], qc), q4_pair<2>(two[2], qc), q4_pair<2>(two[3], qc)});
         tile(4 * hv + 3, u32x4{q4_pair<3>(two[0], qc), q4_pair<3>(two[1], qc), q4_pair<3>(two[2], qc), q4_pair<3>(two[3], qc)});
@@ -405,7 +403,7 @@ __global__ void __launch_bounds__(256, 2) dense_q4_kernel(DenseQ4Params p) {
 #pragma unroll
     for (int u = 1; u < NV; ++u) a = u_mine == u ? o[u][e] : a;
     const int g = 16 * e / G;
-    *reinterpret_cast<f32x4*>(Wo + (w * 16 + col) * WROW + 16 * e + 4 * s) = a + (corr[g] * (e % 4 == 0 ? 8.f : 1.f) + zo[g]);
+    *reinterpret_cast<f32x4*>(Wo + (w * 16 + col) * WROW + 16 * e + 4 * s) = a + (corr[g] + zo[g]);
   }
   __syncthreads();
 

@@ -35,8 +35,13 @@ __device__ __forceinline__ u32x4 q4_frag(uint32_t w, const Q4Const& c) {
 }
 
 // The same with b = 16 in every slot.
+template <int P>
+__device__ __forceinline__ uint32_t q4_pair16(uint32_t w, const Q4Const& c) {
+  if constexpr (P == 0) return ((w << 3) & c.mask) | c.base;
+  else return q4_pair<P>(w, c);
+}
 __device__ __forceinline__ u32x4 q4_frag16(uint32_t w, const Q4Const& c) {
-  return u32x4{((w << 3) & c.mask) | c.base, q4_pair<1>(w, c), q4_pair<2>(w, c), q4_pair<3>(w, c)};
+  return u32x4{q4_pair16<0>(w, c), q4_pair16<1>(w, c), q4_pair16<2>(w, c), q4_pair16<3>(w, c)};
 }
 
 // -b of each slot of q4_frag.

@@ -123,18 +123,16 @@ def _attention(q, cache, mask, kv_len, scale):
     in the errors (1 % for the rest).
 
     A score: at most 32 roundings (18 of a query's sums, 8 of a chain of products, 6 of scales, sums, the factor and
-    the mask) of partial sums of q (2 b + c) s and q z, b 128 for the dims 0 and 4 of every 8 and 16 for the others; the
-    mask's own rounding where it does not absorb the score, which is then exact in both.  An exponential: 2^-22 and 3
+    the mask) of partial sums of q (2 * 16 + c) s and q z; the mask's own rounding where it does not absorb the score,
+    which is then exact in both.  An exponential: 2^-22 and 3
     roundings of its argument, at most 8 above the distance from the maximum.  They move the output by what they move
     each weight times the distance of its value from it.  A weight's terms keep 16 bits of p s c; sums over the
     positions take at most 64 roundings (a split is at most two steps of a wave, at most 33 splits) of partial sums of
-    p s (2 b + c), b 128 for every fourth 16 dims, and p z."""
+    p s (2 * 16 + c) and p z."""
     b, q_h, _, d = q.shape
     k, v = Q.cache_values(cache)
     kz, vz = (t.unflatten(-1, (-1, 2)).double() for t in (cache.k_scales, cache.v_scales))
     group, L = d // kz.shape[-2], k.shape[2]
-    i = torch.arange(d, device=q.device)
-    kb, vb = (271 - 224 * (i % 4 != 0)).double(), (271 - 224 * (i // 16 % 4 != 0)).double()
     out, tol = (torch.empty(b, q_h, d, dtype=torch.float64, device=q.device) for _ in range(2))
     for r in range(b):
         n = L if kv_len is None else min(int(kv_len[r]), L)
@@ -142,7 +140,7 @@ def _attention(q, cache, mask, kv_len, scale):
             kh, vh = h * k.shape[1] // q_h, h * v.shape[1] // q_h
             qd, sk, zk = q[r, h, 0].double(), kz[r, kh, :n, :, 0], kz[r, kh, :n, :, 1].abs()
             x = k[r, kh, :n] @ qd * scale
-            e = (sk @ (qd.abs() * kb).reshape(-1, group).sum(-1) + zk @ qd.abs().reshape(-1, group).sum(-1)) * abs(scale) * 32 * U32
+            e = (47 * sk + zk) @ qd.abs().reshape(-1, group).sum(-1) * abs(scale) * 32 * U32
             if mask is not None:
                 m = mask[r % mask.shape[0], h % mask.shape[1], 0, :n].double()
                 absorbed = m.abs() > 2.0 ** 100  # (scores are below 2^20: half a unit there is 2^75)
@@ -155,7 +153,7 @@ def _attention(q, cache, mask, kv_len, scale):
             pz = (p @ vz[r, vh, :n, :, 1].abs()).repeat_interleave(group)
             out[r, h] = o
             tol[r, h] = (1.01 * (p * delta) @ (v[r, vh, :n] - o).abs() + 2.0 ** -17 * 15 * ps
-                         + 64 * U32 * (vb * ps + pz + o.abs()))
+                         + 64 * U32 * (47 * ps + pz + o.abs()))
     return out[:, :, None], tol[:, :, None]
 
 
