@@ -12,7 +12,8 @@
 // Bound by the weight stream from some 10 MB on (the LM head of 151936 x 1536, 131 MB,
 // 28-29 us at up to 16 rows of x, 4.6 TB/s); below by a launch and two round trips (960 x
 // 960 3.3 us in a graph), and with many rows by reading x: 96 tiles of K 8960 read 143 KB
-// of x per workgroup at 8 rows.
+// of x per workgroup at 8 rows.  Bias and residual are loaded behind the sums: 1536 x 1536 at
+// 8 rows 3.9 us stored, 4.3 with norm and bias, 5.1 added to y.
 #include <algorithm>
 
 #include "kernels.h"
@@ -413,7 +414,7 @@ static void launch_gemv_q4_shape(const GemvQ4Params& p, hipStream_t st) {
 // against 16.7, 17.6, 29.6; K 2048 -, -, 41.9 against 31.8, 34.2, 52.2 (8 rows, streamed:
 // 35.3); K 2944 -, -, 53.9 against 44.1, 47.6, 72.6; K 1536 with 1280 tiles 8.0, 8.1, 13.0
 // against 8.7, 9.3, 16.1, 768 6.6, 7.2, 11.4 against 7.0, 7.8, 10.9, 320 4.9, 5.5, 8.9 against
-// 4.7, 5.8, 9.6.
+// 4.7, 5.8, 9.6.  (1120 tiles are 560 pairs: 48 workgroups take two, the others one.)
 template <int EPI, int G, int MT>
 static void launch_gemv_q4_stream(const GemvQ4Params& p, int units, hipStream_t st) {
   if constexpr (EPI != SAGA_GEMV_ADD) {

@@ -85,9 +85,10 @@ __device__ __forceinline__ void quantise(const float (&x)[NW][8], uint32_t (&w)[
 // wave takes 64 / T heads of one token at a time, with the token's rotations in registers
 // for all of them; few tokens spread their heads over blocks (grid y).  A group's extremes
 // and a value row's transposition are lane exchanges.  4001 tokens of 15 heads, d 128
-// (31 MB): 11.0 us, bound by the quantisation's VALU work beside the projection's bytes (a
-// thread per 8 dims that read its rotations per head and divided per value: 16.8; heads
-// over blocks here too: 12.4); 8 tokens 4.7 us, a launch and two round trips.
+// (31 MB): 11.0 us, bound by the quantisation's VALU work beside the projection's bytes: of a
+// wave's second pass here (12 / 1 / 2 heads) 24 lanes hold keys or values and 40 queries or
+// repeats (a thread per 8 dims that read its rotations per head and divided per value: 16.8;
+// heads over blocks here too: 12.4); 8 tokens 4.7 us, a launch and two round trips.
 template <int D, int G>
 __global__ void __launch_bounds__(256) rope_kv_append_q4_kernel(RopeQ4Params p) {
   constexpr int T = D / 16, HW = 64 / T;
