@@ -53,7 +53,7 @@ extern "C" {
 #define SAGA_DTYPE_BOOL 3 /* one byte, 0 or 1; masks only */
 #define SAGA_DTYPE_I32 4
 #define SAGA_DTYPE_I64 5
-#define SAGA_DTYPE_U8 6 /* bytes of two 4-bit codes, the first in the low half */
+#define SAGA_DTYPE_U8 6 /* bytes: two 4-bit codes, the first in the low half, or one e4m3 number */
 
 #define SAGA_OK 0
 #define SAGA_ERR_INVALID (-1)     /* null pointer, bad shape/stride/dtype */
@@ -489,6 +489,114 @@ typedef struct saga_unpack_q4_item {
   int64_t rot_heads, head_rows;
 } saga_unpack_q4_item;
 int saga_unpack_gemv_q4(const saga_unpack_q4_item* items, int32_t n, saga_stream_t stream);
+
+/* ---- norms of queries and keys, a cache held in 8 bits ---- */
+
+/* New tokens into a cache, norms and rotation in one pass: per query head x
+ * y = x / sqrt(mean(x^2) + eps) * q_norm, per key head the same with k_norm (a
+ * null norm: y = x), then the pairs (y[i], y[i + d/2]) turned by the token's
+ * rotations; values as they are.  qkv [N, >= (n_q + n_k + n_v) * d] (bf16, f16
+ * or f32; d 64 or 128), norms [d] of its type, rope_table as saga_rope_table
+ * writes it for these tokens (required, 16-byte aligned; its positions need not
+ * be the rows').  q_out [N, n_q, d] receives the queries, the caches of qkv's type
+ * [B, n_k, Lmax, d] and [B, n_v, Lmax, d] the rows [batch[n], :, pos[n]] (batch
+ * == NULL: token n is batch row n).  A pos or batch index out of range writes no
+ * cache row and NaN queries.  The (batch, pos) of a call's tokens must differ
+ * from each other. */
+int saga_norm_rope_kv_append(const saga_tensor* qkv, int64_t n_q, const float* rope_table, const saga_tensor* q_norm,
+                             const saga_tensor* k_norm, float eps, const int32_t* pos, const int32_t* batch,
+                             saga_tensor* q_out, saga_tensor* k_cache, saga_tensor* v_cache, saga_stream_t stream);
+
+/* A key / value cache of Lmax positions in 8 bits: e4m3 numbers c (OCP form, no
+ * infinities, largest 448) and per head and block of 32, 64 or 128 consecutive
+ * positions one scale s: value = s * c.
+ *   codes  U8  [B, heads, Lmax, d] (d 64 or 128), innermost stride 1, rows
+ *          16-byte aligned, positions less than 64 MB apart
+ *   scales F32 [B, heads, ceil(Lmax / block)], innermost stride 1
+ * Batch and head strides are free (batch rows and heads may overlap for reading).
+ * What the library writes has scales that are powers of two, 2^(floor(log2 a) - 5)
+ * (at least 2^-100, 0 for a = 0) of the finite magnitude a that set it, and
+ * c = value / s rounded to the nearest, ties to even: off by at most 2^-4 of the
+ * value, or 2^-10 s.  An infinity or a NaN is held as NaN.  What is read may
+ * have any positive scales; results of type f16 end at +-65504, others read
+ * back at bf16's largest.  Attention sums in fp32: magnitudes whose sums over the
+ * positions pass 2^116 overflow there. */
+typedef struct saga_kv_fp8 {
+  saga_tensor k_codes, k_scales, v_codes, v_scales;
+  int64_t block;
+} saga_kv_fp8;
+
+/* saga_norm_rope_kv_append into an 8-bit cache, keys and values rounded from
+ * the exact operations on qkv's numbers (keys: from fp64).  Batch row i of the
+ * first `rows` takes tokens offsets[i] .. offsets[i + 1] - 1 (device int32
+ * [rows + 1], from 0 to N, ascending; NULL: N / rows tokens each) at positions
+ * start[i], start[i] + 1, ... (device int32 [rows]).  A token at a block's first
+ * position starts the block: its scale is set by the call's tokens in it.  Later
+ * tokens leave the scale while they are at most 448 s in magnitude; beyond,
+ * it is set anew by the call's tokens and the positions before them are
+ * rounded to it.  What a block holds behind a call's last token is lost.  A row
+ * whose positions are not all in [0, Lmax) writes nothing and NaN queries. */
+int saga_norm_rope_kv_append_fp8(const saga_tensor* qkv, int64_t n_q, const float* rope_table,
+                                 const saga_tensor* q_norm, const saga_tensor* k_norm, float eps,
+                                 const int32_t* start, const int32_t* offsets, int64_t rows, saga_tensor* q_out,
+                                 const saga_kv_fp8* cache, saga_stream_t stream);
+
+/* Rows of an 8-bit cache as values, as saga_kv_q4_read. */
+int saga_kv_fp8_read(const saga_kv_fp8* cache, const int32_t* pos, const int32_t* batch, saga_tensor* k,
+                     saga_tensor* v, saga_stream_t stream);
+
+/* saga_dense_decode over an 8-bit cache: operands, limits and results as
+ * saga_dense_decode_q4's (query bf16 or f16, any number of query heads per key
+ * head, a row without keys is NaN).  weights (optional): as saga_attention_weights
+ * writes them, G a common divisor of the cache's head counts. */
+size_t saga_dense_fp8_workspace_bytes(int64_t b, int64_t q_h, int64_t L, int64_t d, int32_t with_weights);
+int saga_dense_decode_fp8(const saga_tensor* query, const saga_kv_fp8* cache, const saga_tensor* mask,
+                          const int32_t* kv_len, float scale, saga_tensor* out, saga_tensor* weights,
+                          int32_t weights_add, void* workspace, size_t workspace_bytes, saga_stream_t stream);
+
+/* ---- a cache kept short ---- */
+
+/* The weight that every position gets from one decode step: weights f32 [b, G,
+ * >= L] (innermost stride 1), G a divisor of k_h; group u is the query heads
+ * [u q_h / G, (u + 1) q_h / G) and weights[i, u, j] is the sum of their softmax
+ * weights of position j.  add != 0: added to what is there below kv_len[i]; 0:
+ * written, 0 from kv_len[i] to L.  A head without a finite softmax (no position,
+ * a NaN score) adds nothing.  Operands as saga_qk_scores'. */
+size_t saga_attention_weights_workspace_bytes(int64_t b, int64_t q_h, int64_t k_h, int64_t L);
+int saga_attention_weights(const saga_tensor* query, const saga_tensor* key, const saga_tensor* mask,
+                           const int32_t* kv_len, float scale, saga_tensor* weights, int32_t add, void* workspace,
+                           size_t workspace_bytes, saga_stream_t stream);
+
+/* Eviction: of the n = kv_len[i] positions of batch row i `keep` are kept, where n
+ * is more than that: the last `recent` (0 to keep), and of the others the H = keep
+ * - recent of largest weight (equal ones: the lower position; NaN above all
+ * numbers).  weights f32 [B, G, >= Lmax] (innermost stride 1), G a common
+ * divisor of the key and value heads; each group of heads keeps positions of
+ * its own.  kept (device int32 [B, G, keep], contiguous) receives the position
+ * that each place now holds: a kept one below H keeps its place, the gaps below
+ * H take the kept ones from [H, n - recent) in their order, H + r is n - recent
+ * + r; -1 behind a row's n.  Rows and weights move along; kv_len is the caller's
+ * to cut to min(n, keep).
+ * In place (the *_out NULL): weights behind min(n, keep) become 0; rows behind
+ * it are left as they are.  Into other tensors (all *_out given; they must
+ * not overlap the inputs): k_out, v_out [B, heads, >= keep, d] of the caches' type,
+ * weights_out f32 [B, G, >= keep] (0 behind min(n, keep)); rows behind it are left.
+ * Caches [B, heads, Lmax, d] bf16, f16 or f32, 16-byte aligned rows.
+ * workspace: saga_evict_workspace_bytes of the sum of heads and a row's bytes. */
+size_t saga_evict_workspace_bytes(int64_t B, int64_t G, int64_t keep, int64_t recent, int64_t heads,
+                                  int64_t row_bytes, int32_t in_place);
+int saga_evict_kv(const saga_tensor* k_cache, const saga_tensor* v_cache, const saga_tensor* weights,
+                  const int32_t* kv_len, int64_t keep, int64_t recent, const saga_tensor* k_out,
+                  const saga_tensor* v_out, const saga_tensor* weights_out, int32_t* kept, void* workspace,
+                  size_t workspace_bytes, saga_stream_t stream);
+
+/* The same over an 8-bit cache (row_bytes: d).  A block of the result takes the
+ * largest of its rows' scales; rows from under a smaller one are rounded to it
+ * (powers of two: only numbers that turn subnormal change).  cache_out (NULL: in
+ * place): the same block, at least keep positions. */
+int saga_evict_kv_fp8(const saga_kv_fp8* cache, const saga_tensor* weights, const int32_t* kv_len, int64_t keep,
+                      int64_t recent, const saga_kv_fp8* cache_out, const saga_tensor* weights_out, int32_t* kept,
+                      void* workspace, size_t workspace_bytes, saga_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -60,6 +60,11 @@ class Q4Weight(ctypes.Structure):
     _fields_ = [("codes", SagaTensor), ("scales", SagaTensor)]
 
 
+class KvFp8(ctypes.Structure):
+    _fields_ = [("k_codes", SagaTensor), ("k_scales", SagaTensor), ("v_codes", SagaTensor), ("v_scales", SagaTensor),
+                ("block", ctypes.c_int64)]
+
+
 class UnpackQ4Item(ctypes.Structure):
     _fields_ = [("w", Q4Weight), ("out", SagaTensor), ("rot_heads", ctypes.c_int64), ("head_rows", ctypes.c_int64)]
 
@@ -118,6 +123,17 @@ _SIGS = {
     "saga_gemv_q4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "saga_gemv_q4": (ctypes.c_int, [_P, _P, _P, ctypes.c_float, ctypes.c_int32, _P, _P, ctypes.c_size_t, _P]),
     "saga_unpack_gemv_q4": (ctypes.c_int, [_P, ctypes.c_int32, _P]),
+    "saga_norm_rope_kv_append": (ctypes.c_int, [_P, _I64, _P, _P, _P, ctypes.c_float, _P, _P, _P, _P, _P, _P]),
+    "saga_norm_rope_kv_append_fp8": (ctypes.c_int, [_P, _I64, _P, _P, _P, ctypes.c_float, _P, _P, _I64, _P, _P, _P]),
+    "saga_kv_fp8_read": (ctypes.c_int, [_P, _P, _P, _P, _P, _P]),
+    "saga_dense_fp8_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, ctypes.c_int32]),
+    "saga_dense_decode_fp8": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_float, _P, _P, ctypes.c_int32, _P,
+                                             ctypes.c_size_t, _P]),
+    "saga_attention_weights_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64]),
+    "saga_attention_weights": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_float, _P, ctypes.c_int32, _P, ctypes.c_size_t, _P]),
+    "saga_evict_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I64, ctypes.c_int32]),
+    "saga_evict_kv": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "saga_evict_kv_fp8": (ctypes.c_int, [_P, _P, _P, _I64, _I64, _P, _P, _P, _P, ctypes.c_size_t, _P]),
 }
 GEMV_STORE, GEMV_ADD, GEMV_SILU_PAIRS = 0, 1, 2
 K2_AUTO, K2_ROW_BLOCK, K2_SLICE_ROW = 0, 1, 2

@@ -1209,6 +1209,23 @@ bool vec8(const saga_tensor* t) {
          (t->ndim < 3 || t->stride[1] % 8 == 0);
 }
 
+// An additive mask of the decode kernels with 4- and 8-bit caches.
+int check_mask_2gb(const saga_tensor* mask, const Shape& s) {
+  int rc;
+  if ((rc = check_tensor(mask, "mask", 4))) return rc;
+  if (!is_float(mask->dtype) && mask->dtype != SAGA_DTYPE_BOOL)
+    return fail(SAGA_ERR_INVALID, "mask: dtype must be f32, bf16, f16 or bool");
+  if ((mask->shape[0] != 1 && mask->shape[0] != s.b) || (mask->shape[1] != 1 && mask->shape[1] != s.q_h) ||
+      mask->shape[2] != 1 || mask->shape[3] < s.L)
+    return fail(SAGA_ERR_INVALID, "mask: shape does not broadcast to [b, q_h, 1, L=%lld]", (long long)s.L);
+  const int64_t span = (mask->shape[1] - 1) * mask->stride[1] + (s.L - 1) * mask->stride[3];
+  if (span * elt_size(mask->dtype) >= (1LL << 31) - 64)
+    return fail(SAGA_ERR_UNSUPPORTED, "mask: a batch row of more than 2 GB");
+  if (elt_size(mask->dtype) > 1 && reinterpret_cast<uintptr_t>(mask->data) % elt_size(mask->dtype))
+    return fail(SAGA_ERR_INVALID, "mask: data pointer must be aligned to its type");
+  return SAGA_OK;
+}
+
 // A 4-bit weight [N, K] of saga_gemv_q4 / saga_unpack_gemv_q4.
 int check_q4_weight(const saga_q4_weight* w, int64_t K, int64_t* N, int64_t* group) {
   int rc;
@@ -1331,17 +1348,7 @@ int saga_dense_decode_q4(const saga_tensor* query, const saga_kv_q4* cache, cons
   if (s.q_h > (1LL << 22) || s.b * s.q_h >= (1LL << 22)) return fail(SAGA_ERR_UNSUPPORTED, "b * q_h too large");
   if ((rc = check_vec_rows(query, "query")) || (rc = check_out(out, s))) return rc;
   if (mask) {
-    if ((rc = check_tensor(mask, "mask", 4))) return rc;
-    if (!is_float(mask->dtype) && mask->dtype != SAGA_DTYPE_BOOL)
-      return fail(SAGA_ERR_INVALID, "mask: dtype must be f32, bf16, f16 or bool");
-    if ((mask->shape[0] != 1 && mask->shape[0] != s.b) || (mask->shape[1] != 1 && mask->shape[1] != s.q_h) ||
-        mask->shape[2] != 1 || mask->shape[3] < s.L)
-      return fail(SAGA_ERR_INVALID, "mask: shape does not broadcast to [b, q_h, 1, L=%lld]", (long long)s.L);
-    const int64_t span = (mask->shape[1] - 1) * mask->stride[1] + (s.L - 1) * mask->stride[3];
-    if (span * elt_size(mask->dtype) >= (1LL << 31) - 64)
-      return fail(SAGA_ERR_UNSUPPORTED, "mask: a batch row of more than 2 GB");
-    if (elt_size(mask->dtype) > 1 && reinterpret_cast<uintptr_t>(mask->data) % elt_size(mask->dtype))
-      return fail(SAGA_ERR_INVALID, "mask: data pointer must be aligned to its type");
+    if ((rc = check_mask_2gb(mask, s))) return rc;
     p.mask = mask->data;
     p.mask_dt = mask->dtype;
     p.m_sb = mask->shape[0] == 1 ? 0 : mask->stride[0];
@@ -1452,6 +1459,492 @@ int saga_unpack_gemv_q4(const saga_unpack_q4_item* items, int32_t n, saga_stream
   }
   if ((rc = hip_status(launch_unpack_q4(p, static_cast<hipStream_t>(stream)), "unpack_q4 launch"))) return rc;
   return ok();
+}
+
+}  // extern "C"
+
+namespace {
+
+// The rows of a cache that a call writes must differ from each other.
+int check_distinct(const saga_tensor* t, const char* name) {
+  for (int i = 0; i + 1 < t->ndim; ++i)
+    if (t->shape[i] > 1 && t->stride[i] == 0) return fail(SAGA_ERR_INVALID, "%s: rows written must not share memory", name);
+  return SAGA_OK;
+}
+
+// One kind (codes + scales) of an 8-bit cache.
+int check_kv_fp8_kind(const saga_tensor* codes, const saga_tensor* scales, int64_t block, const char* name) {
+  int rc;
+  if ((rc = check_tensor(codes, name, 4)) || (rc = check_tensor(scales, name, 3))) return rc;
+  if (codes->dtype != SAGA_DTYPE_U8 || scales->dtype != SAGA_DTYPE_F32)
+    return fail(SAGA_ERR_INVALID, "%s: codes must be u8 and scales f32", name);
+  if (codes->shape[0] != scales->shape[0] || codes->shape[1] != scales->shape[1] ||
+      scales->shape[2] != (codes->shape[2] + block - 1) / block)
+    return fail(SAGA_ERR_INVALID, "%s: codes [B, heads, Lmax, d] and scales [B, heads, ceil(Lmax / block)] differ", name);
+  if ((rc = check_vec_rows(codes, name))) return rc;
+  if (scales->stride[2] != 1 && scales->shape[2] > 1)
+    return fail(SAGA_ERR_INVALID, "%s: scales need a unit innermost stride", name);
+  if (reinterpret_cast<uintptr_t>(scales->data) % 4)
+    return fail(SAGA_ERR_INVALID, "%s: scales must be aligned to their type", name);
+  return SAGA_OK;
+}
+
+int check_kv_fp8(const saga_kv_fp8* c, bool written, KvFp8& kv) {
+  if (!c) return fail(SAGA_ERR_INVALID, "cache: null");
+  if (c->block != 32 && c->block != 64 && c->block != 128)
+    return fail(SAGA_ERR_UNSUPPORTED, "cache: blocks of %lld positions not built (32, 64, 128)", (long long)c->block);
+  int rc;
+  const saga_tensor &kc = c->k_codes, &ks = c->k_scales, &vc = c->v_codes, &vs = c->v_scales;
+  if ((rc = check_kv_fp8_kind(&kc, &ks, c->block, "key cache")) || (rc = check_kv_fp8_kind(&vc, &vs, c->block, "value cache")))
+    return rc;
+  if (kc.shape[0] != vc.shape[0] || kc.shape[2] != vc.shape[2] || kc.shape[3] != vc.shape[3])
+    return fail(SAGA_ERR_INVALID, "cache: keys and values differ in batch, positions or head dim");
+  const int64_t d = kc.shape[3];
+  if (d != 64 && d != 128) return fail(SAGA_ERR_UNSUPPORTED, "cache: head_dim %lld not built (64, 128)", (long long)d);
+  // (32 rows within 2^31 bytes: the kernels' lane offsets)
+  if (kc.stride[2] >= (1LL << 26) || vc.stride[2] >= (1LL << 26))
+    return fail(SAGA_ERR_UNSUPPORTED, "cache: positions more than 64 MB apart");
+  if (kc.shape[2] >= kMaxLen || kc.shape[1] > 65535 || vc.shape[1] > 65535)
+    return fail(SAGA_ERR_UNSUPPORTED, "cache: sizes too large");
+  if (written)
+    for (const saga_tensor* t : {&kc, &ks, &vc, &vs})
+      if ((rc = check_distinct(t, "cache"))) return rc;
+  kv = KvFp8{};
+  kv.kc = static_cast<const char*>(kc.data);
+  kv.kc_sb = kc.stride[0], kv.kc_sh = kc.stride[1], kv.kc_sl = kc.stride[2];
+  kv.vc = static_cast<const char*>(vc.data);
+  kv.vc_sb = vc.stride[0], kv.vc_sh = vc.stride[1], kv.vc_sl = vc.stride[2];
+  kv.ks = static_cast<const float*>(ks.data);
+  kv.ks_sb = ks.stride[0], kv.ks_sh = ks.stride[1];
+  kv.vs = static_cast<const float*>(vs.data);
+  kv.vs_sb = vs.stride[0], kv.vs_sh = vs.stride[1];
+  kv.B = static_cast<int32_t>(kc.shape[0]);
+  kv.n_k = static_cast<int32_t>(kc.shape[1]);
+  kv.n_v = static_cast<int32_t>(vc.shape[1]);
+  kv.Lmax = static_cast<int32_t>(kc.shape[2]);
+  kv.d = static_cast<int32_t>(d);
+  kv.shift = c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
+  return SAGA_OK;
+}
+
+// What the appends with norms share: projection, norms, rotations and queries of head dim d beside n_k and n_v heads.
+int make_norm_rope(const saga_tensor* qkv, int64_t n_q, int64_t n_k, int64_t n_v, int64_t d, const float* rope_table,
+                   const saga_tensor* q_norm, const saga_tensor* k_norm, float eps, const saga_tensor* q_out,
+                   NormRopeParams& p) {
+  int rc;
+  if ((rc = check_tensor(qkv, "qkv", 2)) || (rc = check_tensor(q_out, "q_out", 3))) return rc;
+  if (!is_float(qkv->dtype) || q_out->dtype != qkv->dtype)
+    return fail(SAGA_ERR_INVALID, "qkv and q_out must share one float dtype");
+  if (!rope_table || reinterpret_cast<uintptr_t>(rope_table) % 16)
+    return fail(SAGA_ERR_INVALID, "rope_table must be given and 16-byte aligned");
+  if (d != 64 && d != 128) return fail(SAGA_ERR_UNSUPPORTED, "head_dim %lld not built (64, 128)", (long long)d);
+  const int64_t N = qkv->shape[0];
+  if (n_q < 1 || n_q + n_k + n_v > 65535) return fail(SAGA_ERR_INVALID, "head counts: 1 to 65535 in all required");
+  if (q_out->shape[0] != N || q_out->shape[1] != n_q || q_out->shape[2] != d)
+    return fail(SAGA_ERR_INVALID, "q_out: shape must be [N, n_q, d]");
+  if (qkv->shape[1] < (n_q + n_k + n_v) * d) return fail(SAGA_ERR_INVALID, "qkv: row shorter than (n_q + n_k + n_v) * d");
+  if (qkv->stride[1] != 1 || q_out->stride[2] != 1) return fail(SAGA_ERR_INVALID, "innermost strides must be 1");
+  if ((rc = check_distinct(q_out, "q_out"))) return rc;
+  p = NormRopeParams{};
+  p.vec = vec8(qkv) && vec8(q_out);
+  for (const saga_tensor* t : {q_norm, k_norm}) {
+    if (!t) continue;
+    if ((rc = check_tensor(t, "norm", 1))) return rc;
+    if (t->dtype != qkv->dtype || t->shape[0] != d || t->stride[0] != 1)
+      return fail(SAGA_ERR_INVALID, "norms must be contiguous [d] of qkv's dtype");
+    p.vec = p.vec && reinterpret_cast<uintptr_t>(t->data) % 16 == 0;
+  }
+  if ((q_norm || k_norm) && !(eps >= 0.f)) return fail(SAGA_ERR_INVALID, "eps must not be negative");
+  // (four tokens a block of 256 threads; a launch holds less than 2^32 threads)
+  if (N > (1LL << 26) - 4) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  p.qkv = qkv->data;
+  p.qkv_ld = qkv->stride[0];
+  p.q_out = q_out->data;
+  p.q_sn = q_out->stride[0];
+  p.q_sh = q_out->stride[1];
+  p.dt = qkv->dtype;
+  p.N = static_cast<int32_t>(N);
+  p.n_q = static_cast<int32_t>(n_q);
+  p.n_k = static_cast<int32_t>(n_k);
+  p.n_v = static_cast<int32_t>(n_v);
+  p.d = static_cast<int32_t>(d);
+  p.table = rope_table;
+  p.q_norm = q_norm ? q_norm->data : nullptr;
+  p.k_norm = k_norm ? k_norm->data : nullptr;
+  p.eps = eps;
+  return SAGA_OK;
+}
+
+// weights f32 [b, G, >= L] of groups of heads.
+int check_weights(const saga_tensor* w, const char* name, int64_t b, int64_t k_h, int64_t v_h, int64_t L, bool written) {
+  int rc;
+  if ((rc = check_tensor(w, name, 3))) return rc;
+  if (w->dtype != SAGA_DTYPE_F32 || w->shape[0] != b || w->shape[2] < L || w->stride[2] != 1)
+    return fail(SAGA_ERR_INVALID, "%s: f32 [b, G, >= %lld] with a unit innermost stride required", name, (long long)L);
+  if (k_h % w->shape[1] || v_h % w->shape[1])
+    return fail(SAGA_ERR_INVALID, "%s: %lld groups do not divide %lld key and %lld value heads", name, (long long)w->shape[1],
+                (long long)k_h, (long long)v_h);
+  return written ? check_distinct(w, name) : SAGA_OK;
+}
+
+WeightsParams make_weights(const saga_tensor* w, int32_t add, const int32_t* kv_len, int64_t b, int64_t q_h, int64_t L) {
+  WeightsParams p{};
+  p.kv_len = kv_len;
+  p.b = static_cast<int32_t>(b);
+  p.q_h = static_cast<int32_t>(q_h);
+  p.G = static_cast<int32_t>(w->shape[1]);
+  p.L = static_cast<int32_t>(L);
+  p.w = static_cast<float*>(w->data);
+  p.w_sb = w->stride[0];
+  p.w_sg = w->stride[1];
+  p.add = add ? 1 : 0;
+  return p;
+}
+
+// Byte offsets of an eviction's workspace.
+struct EvictLayout {
+  int64_t movers, held, stage, stage_s, total;
+};
+EvictLayout evict_layout(int64_t B, int64_t G, int64_t keep, int64_t recent, int64_t heads, int64_t row_bytes, bool in_place) {
+  EvictLayout o{};
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = off;
+    off = align256(off + bytes);
+    return at;
+  };
+  o.movers = take(B * G * keep * 4);
+  o.held = take(B * G * keep * 4);
+  const int64_t staged = in_place ? B * heads * std::min(keep, recent + 127) : 0;
+  o.stage = take(staged * row_bytes);
+  o.stage_s = take(staged * 4);
+  o.total = off;
+  return o;
+}
+
+// The shared body of the evictions: p.rows hold the tensors; out: whether other tensors take the result.
+int evict_run(EvictParams& p, const saga_tensor* weights, const int32_t* kv_len, int64_t keep, int64_t recent, bool out,
+              const saga_tensor* weights_out, int64_t B, int64_t k_h, int64_t v_h, int64_t L, int64_t row_bytes,
+              int32_t* kept, void* workspace, size_t workspace_bytes, saga_stream_t stream) {
+  int rc;
+  if (keep < 1 || keep >= kMaxLen || recent < 0 || recent > keep)
+    return fail(SAGA_ERR_INVALID, "keep >= 1 and 0 <= recent <= keep required, got %lld and %lld", (long long)keep, (long long)recent);
+  if (!kv_len || !kept) return fail(SAGA_ERR_INVALID, "kv_len or kept: null");
+  if ((rc = check_weights(weights, "weights", B, k_h, v_h, L, !out))) return rc;
+  const int64_t G = weights->shape[1], heads = k_h + v_h;
+  if (out && (rc = check_weights(weights_out, "weights_out", B, k_h, v_h, keep, true))) return rc;
+  if (out && weights_out->shape[1] != G) return fail(SAGA_ERR_INVALID, "weights_out: groups differ from weights");
+  const int64_t S = 1LL << p.shift, nblk = (keep + S - 1) / S;
+  // (a launch holds less than 2^32 threads)
+  if (B > (1LL << 22) / G - 1 || B * heads > ((1LL << 24) - 1) / nblk || B * G * keep > (1LL << 40))
+    return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  const EvictLayout lay = evict_layout(B, G, keep, recent, heads, row_bytes, !out);
+  if (!workspace || workspace_bytes < static_cast<size_t>(lay.total))
+    return fail(SAGA_ERR_WORKSPACE, "workspace of %zu bytes, need %lld", workspace_bytes, (long long)lay.total);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(SAGA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  const saga_tensor* wo = out ? weights_out : weights;
+  p.w = static_cast<const float*>(weights->data);
+  p.w_sb = weights->stride[0], p.w_sg = weights->stride[1];
+  p.w_out = static_cast<float*>(wo->data);
+  p.wo_sb = wo->stride[0], p.wo_sg = wo->stride[1], p.wo_len = wo->shape[2];
+  p.kv_len = kv_len;
+  p.kept = kept;
+  p.movers = reinterpret_cast<int32_t*>(ws + lay.movers);
+  p.held_w = reinterpret_cast<float*>(ws + lay.held);
+  p.B = static_cast<int32_t>(B);
+  p.G = static_cast<int32_t>(G);
+  p.Lmax = static_cast<int32_t>(L);
+  p.keep = static_cast<int32_t>(keep);
+  p.recent = static_cast<int32_t>(recent);
+  p.in_place = out ? 0 : 1;
+  p.staged0 = static_cast<int32_t>((keep - recent) / S * S);
+  const int64_t nstage = keep - p.staged0;
+  p.rows[0].stage = ws + lay.stage;
+  p.rows[0].stage_s = reinterpret_cast<float*>(ws + lay.stage_s);
+  p.rows[1].stage = p.rows[0].stage + B * k_h * nstage * row_bytes;
+  p.rows[1].stage_s = p.rows[0].stage_s + B * k_h * nstage;
+  p.rows[0].heads = static_cast<int32_t>(k_h);
+  p.rows[1].heads = static_cast<int32_t>(v_h);
+  p.rows[0].pieces = p.rows[1].pieces = static_cast<int32_t>(row_bytes / 16);
+  if ((rc = hip_status(launch_evict(p, static_cast<hipStream_t>(stream)), "evict launch"))) return rc;
+  return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+int saga_norm_rope_kv_append(const saga_tensor* qkv, int64_t n_q, const float* rope_table, const saga_tensor* q_norm,
+                             const saga_tensor* k_norm, float eps, const int32_t* pos, const int32_t* batch,
+                             saga_tensor* q_out, saga_tensor* k_cache, saga_tensor* v_cache, saga_stream_t stream) {
+  int rc;
+  NormRopeParams p;
+  if ((rc = check_tensor(k_cache, "k_cache", 4)) || (rc = check_tensor(v_cache, "v_cache", 4))) return rc;
+  const int64_t n_k = k_cache->shape[1], n_v = v_cache->shape[1], d = k_cache->shape[3];
+  if (n_k > 65535 || n_v > 65535 || n_q > 65535) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  if ((rc = make_norm_rope(qkv, n_q, n_k, n_v, d, rope_table, q_norm, k_norm, eps, q_out, p))) return rc;
+  if (!pos) return fail(SAGA_ERR_INVALID, "pos: null");
+  if (k_cache->dtype != qkv->dtype || v_cache->dtype != qkv->dtype)
+    return fail(SAGA_ERR_INVALID, "the caches must have the dtype of the projection");
+  if (v_cache->shape[0] != k_cache->shape[0] || v_cache->shape[2] != k_cache->shape[2] || v_cache->shape[3] != d)
+    return fail(SAGA_ERR_INVALID, "caches: shapes must be [B, n_k, Lmax, d] and [B, n_v, Lmax, d]");
+  if (k_cache->stride[3] != 1 || v_cache->stride[3] != 1) return fail(SAGA_ERR_INVALID, "innermost strides must be 1");
+  if ((rc = check_distinct(k_cache, "k_cache")) || (rc = check_distinct(v_cache, "v_cache"))) return rc;
+  if (!batch && p.N > k_cache->shape[0]) return fail(SAGA_ERR_INVALID, "without batch indices N must be <= B");
+  if (k_cache->shape[2] >= kMaxLen) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  for (const saga_tensor* t : {k_cache, v_cache})
+    p.vec = p.vec && vec8(t) && t->stride[2] % 8 == 0;
+  p.pos = pos;
+  p.batch = batch;
+  p.k_cache = k_cache->data;
+  p.k_sb = k_cache->stride[0], p.k_sh = k_cache->stride[1], p.k_sl = k_cache->stride[2];
+  p.v_cache = v_cache->data;
+  p.v_sb = v_cache->stride[0], p.v_sh = v_cache->stride[1], p.v_sl = v_cache->stride[2];
+  p.B = static_cast<int32_t>(k_cache->shape[0]);
+  p.Lmax = static_cast<int32_t>(k_cache->shape[2]);
+  if ((rc = hip_status(launch_norm_rope_kv_append(p, static_cast<hipStream_t>(stream)), "norm_rope_kv_append launch")))
+    return rc;
+  return ok();
+}
+
+int saga_norm_rope_kv_append_fp8(const saga_tensor* qkv, int64_t n_q, const float* rope_table,
+                                 const saga_tensor* q_norm, const saga_tensor* k_norm, float eps,
+                                 const int32_t* start, const int32_t* offsets, int64_t rows, saga_tensor* q_out,
+                                 const saga_kv_fp8* cache, saga_stream_t stream) {
+  int rc;
+  KvFp8 kv;
+  NormRopeParams p;
+  if ((rc = check_kv_fp8(cache, true, kv))) return rc;
+  if (n_q > 65535) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  if ((rc = make_norm_rope(qkv, n_q, kv.n_k, kv.n_v, kv.d, rope_table, q_norm, k_norm, eps, q_out, p))) return rc;
+  if (!start) return fail(SAGA_ERR_INVALID, "start: null");
+  if (rows < 1 || rows > kv.B) return fail(SAGA_ERR_INVALID, "rows: 1 to B required");
+  if (!offsets && p.N % rows) return fail(SAGA_ERR_INVALID, "without offsets N must be a multiple of rows");
+  if ((p.N >> kv.shift) + 2 * rows >= (1LL << 24)) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  p.kv = kv;
+  p.start = start;
+  p.offsets = offsets;
+  p.rows = static_cast<int32_t>(rows);
+  p.B = kv.B;
+  p.Lmax = kv.Lmax;
+  if ((rc = hip_status(launch_norm_rope_kv_append_fp8(p, static_cast<hipStream_t>(stream)), "norm_rope_kv_append_fp8 launch")))
+    return rc;
+  return ok();
+}
+
+int saga_kv_fp8_read(const saga_kv_fp8* cache, const int32_t* pos, const int32_t* batch, saga_tensor* k, saga_tensor* v,
+                     saga_stream_t stream) {
+  int rc;
+  KvFp8ReadParams p{};
+  if ((rc = check_kv_fp8(cache, false, p.kv)) || (rc = check_tensor(k, "k", 3)) || (rc = check_tensor(v, "v", 3))) return rc;
+  if (!pos) return fail(SAGA_ERR_INVALID, "pos: null");
+  if (!is_float(k->dtype) || v->dtype != k->dtype) return fail(SAGA_ERR_INVALID, "k and v must share one float dtype");
+  const int64_t N = k->shape[0], d = p.kv.d;
+  if (k->shape[1] != p.kv.n_k || k->shape[2] != d || v->shape[0] != N || v->shape[1] != p.kv.n_v || v->shape[2] != d)
+    return fail(SAGA_ERR_INVALID, "k and v: shapes must be [N, n_k, d] and [N, n_v, d]");
+  if (k->stride[2] != 1 || v->stride[2] != 1) return fail(SAGA_ERR_INVALID, "innermost strides must be 1");
+  if (!batch && N > p.kv.B) return fail(SAGA_ERR_INVALID, "without batch indices N must be <= B");
+  if (N * (p.kv.n_k + p.kv.n_v) * (d / 8) >= (1LL << 32) - 256) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  p.pos = pos;
+  p.batch = batch;
+  p.k = k->data;
+  p.k_sn = k->stride[0], p.k_sh = k->stride[1];
+  p.v = v->data;
+  p.v_sn = v->stride[0], p.v_sh = v->stride[1];
+  p.dt = k->dtype;
+  p.N = static_cast<int32_t>(N);
+  p.vec = vec8(k) && vec8(v);
+  if ((rc = hip_status(launch_kv_fp8_read(p, static_cast<hipStream_t>(stream)), "kv_fp8_read launch"))) return rc;
+  return ok();
+}
+
+size_t saga_dense_fp8_workspace_bytes(int64_t b, int64_t q_h, int64_t L, int64_t d, int32_t with_weights) {
+  if (b < 1 || q_h < 1 || L < 1 || L >= kMaxLen || d < 1 || d > 1024 || b > (1LL << 22) / q_h) return 0;
+  int64_t ns, sl;
+  dense_q4_plan(b, L, &ns, &sl);
+  const int64_t scores = with_weights ? b * q_h * ((L + 31) / 32 * 32) * 4 : 0;
+  return static_cast<size_t>(align256(b * q_h * ns * (2 + d) * 4) + scores);
+}
+
+int saga_dense_decode_fp8(const saga_tensor* query, const saga_kv_fp8* cache, const saga_tensor* mask,
+                          const int32_t* kv_len, float scale, saga_tensor* out, saga_tensor* weights,
+                          int32_t weights_add, void* workspace, size_t workspace_bytes, saga_stream_t stream) {
+  int rc;
+  DenseFp8Params p{};
+  if ((rc = check_tensor(query, "query", 4)) || (rc = check_kv_fp8(cache, false, p.kv))) return rc;
+  Shape s{};
+  s.b = query->shape[0];
+  s.q_h = query->shape[1];
+  s.d = query->shape[3];
+  s.L = p.kv.Lmax;
+  if (query->shape[2] != 1)
+    return fail(SAGA_ERR_UNSUPPORTED, "query: decode path needs l_q == 1, got %lld", (long long)query->shape[2]);
+  if (query->dtype != SAGA_DTYPE_BF16 && query->dtype != SAGA_DTYPE_F16)
+    return fail(SAGA_ERR_UNSUPPORTED, "query: dtype must be bf16 or f16");
+  if (p.kv.B != s.b || p.kv.d != s.d) return fail(SAGA_ERR_INVALID, "cache: batch or head dim differs from the query's");
+  if (s.q_h % p.kv.n_k) return fail(SAGA_ERR_INVALID, "q_h (%lld) not a multiple of k_h (%d)", (long long)s.q_h, p.kv.n_k);
+  if (s.q_h % p.kv.n_v) return fail(SAGA_ERR_INVALID, "q_h (%lld) not a multiple of v_h (%d)", (long long)s.q_h, p.kv.n_v);
+  if (s.q_h > (1LL << 22) || s.b * s.q_h >= (1LL << 22)) return fail(SAGA_ERR_UNSUPPORTED, "b * q_h too large");
+  if ((rc = check_vec_rows(query, "query")) || (rc = check_out(out, s))) return rc;
+  if (mask) {
+    if ((rc = check_mask_2gb(mask, s))) return rc;
+    p.mask = mask->data;
+    p.mask_dt = mask->dtype;
+    p.m_sb = mask->shape[0] == 1 ? 0 : mask->stride[0];
+    p.m_sh = mask->shape[1] == 1 ? 0 : mask->stride[1];
+    p.m_sl = mask->stride[3];
+  }
+  if (weights && (rc = check_weights(weights, "weights", s.b, p.kv.n_k, p.kv.n_v, s.L, true))) return rc;
+  int64_t ns, sl;
+  dense_q4_plan(s.b, s.L, &ns, &sl);
+  const int64_t part = align256(s.b * s.q_h * ns * (2 + s.d) * 4), ld = (s.L + 31) / 32 * 32;
+  const size_t need = static_cast<size_t>(part + (weights ? s.b * s.q_h * ld * 4 : 0));
+  const bool used = ns > 1 || weights;
+  if (used && (!workspace || workspace_bytes < need))
+    return fail(SAGA_ERR_WORKSPACE, "workspace of %zu bytes, need %zu", workspace_bytes, need);
+  if (used && reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(SAGA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  p.q = static_cast<const char*>(query->data);
+  p.q_sb = query->stride[0];
+  p.q_sh = query->stride[1];
+  p.q_dt = query->dtype;
+  p.kv_len = kv_len;
+  p.b = static_cast<int32_t>(s.b);
+  p.q_h = static_cast<int32_t>(s.q_h);
+  p.L = static_cast<int32_t>(s.L);
+  p.g = static_cast<int32_t>(s.q_h / p.kv.n_k);
+  p.g_v = static_cast<int32_t>(s.q_h / p.kv.n_v);
+  p.scale = scale;
+  p.out = out->data;
+  p.out_dt = out->dtype;
+  p.o_sb = out->stride[0];
+  p.o_sh = out->stride[1];
+  p.part = static_cast<float*>(workspace);
+  if (weights) {
+    p.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + part);
+    p.scores_ld = ld;
+  }
+  if ((rc = hip_status(launch_dense_decode_fp8(p, static_cast<hipStream_t>(stream)), "dense_decode_fp8 launch"))) return rc;
+  if (weights) {
+    WeightsParams w = make_weights(weights, weights_add, kv_len, s.b, s.q_h, s.L);
+    w.scores = p.scores;
+    w.s_ld = ld;
+    w.pm = p.part + s.b * s.q_h * p.nsplit * s.d;
+    w.ps = w.pm + 1;
+    w.pstride = 2;
+    w.nparts = p.nsplit;
+    if ((rc = hip_status(launch_attention_weights(w, static_cast<hipStream_t>(stream)), "attention_weights launch"))) return rc;
+  }
+  return ok();
+}
+
+size_t saga_attention_weights_workspace_bytes(int64_t b, int64_t q_h, int64_t k_h, int64_t L) {
+  if (b < 1 || q_h < 1 || k_h < 1 || k_h > q_h || L < 1 || L >= kMaxLen || b > (1LL << 22) / q_h) return 0;
+  const int64_t parts = align256(b * q_h * (qk_plan(b, k_h, L) / 4) * 4);
+  return static_cast<size_t>(2 * parts + b * q_h * ((L + 15) / 16 * 16) * 4);
+}
+
+int saga_attention_weights(const saga_tensor* query, const saga_tensor* key, const saga_tensor* mask,
+                           const int32_t* kv_len, float scale, saga_tensor* weights, int32_t add, void* workspace,
+                           size_t workspace_bytes, saga_stream_t stream) {
+  Shape s{};
+  int rc;
+  if ((rc = check_qk(query, key, mask, &s))) return rc;
+  if ((rc = check_weights(weights, "weights", s.b, s.k_h, s.k_h, s.L, true))) return rc;
+  if (s.b * s.q_h > (1LL << 22)) return fail(SAGA_ERR_UNSUPPORTED, "b * q_h too large");
+  const size_t need = saga_attention_weights_workspace_bytes(s.b, s.q_h, s.k_h, s.L);
+  if (!workspace || workspace_bytes < need)
+    return fail(SAGA_ERR_WORKSPACE, "workspace of %zu bytes, need %zu", workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(SAGA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  QKParams q = make_qk(query, key, mask, kv_len, scale, s);
+  if (s.b * s.k_h * static_cast<int64_t>(q.nparts) / 4 >= (1LL << 24)) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  const int64_t ld = (s.L + 15) / 16 * 16, parts = align256(s.b * s.q_h * (q.nparts / 4) * 4) / 4;
+  q.pmax = static_cast<float*>(workspace);
+  q.psum = q.pmax + parts;
+  q.scores = q.psum + parts;
+  q.s_sb = s.q_h * ld;
+  q.s_sh = ld;
+  q.vec_store = 1;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if ((rc = hip_status(launch_qk_scores(s.dt, static_cast<int>(s.d), q, st), "qk_scores launch"))) return rc;
+  WeightsParams w = make_weights(weights, add, kv_len, s.b, s.q_h, s.L);
+  w.scores = q.scores;
+  w.s_ld = ld;
+  w.pm = q.pmax;
+  w.ps = q.psum;
+  w.pstride = 1;
+  w.nparts = q.nparts / 4;
+  if ((rc = hip_status(launch_attention_weights(w, st), "attention_weights launch"))) return rc;
+  return ok();
+}
+
+size_t saga_evict_workspace_bytes(int64_t B, int64_t G, int64_t keep, int64_t recent, int64_t heads, int64_t row_bytes,
+                                  int32_t in_place) {
+  if (B < 1 || G < 1 || keep < 1 || keep >= kMaxLen || recent < 0 || recent > keep || heads < 1 || heads > 131070 ||
+      row_bytes < 1 || row_bytes > 4096 || B > (1LL << 22) / G || B * heads > (1LL << 24))
+    return 0;
+  return static_cast<size_t>(evict_layout(B, G, keep, recent, heads, row_bytes, in_place != 0).total);
+}
+
+int saga_evict_kv(const saga_tensor* k_cache, const saga_tensor* v_cache, const saga_tensor* weights,
+                  const int32_t* kv_len, int64_t keep, int64_t recent, const saga_tensor* k_out,
+                  const saga_tensor* v_out, const saga_tensor* weights_out, int32_t* kept, void* workspace,
+                  size_t workspace_bytes, saga_stream_t stream) {
+  int rc;
+  EvictParams p{};
+  const bool out = k_out || v_out || weights_out;
+  const saga_tensor *src[2] = {k_cache, v_cache}, *dst[2] = {out ? k_out : k_cache, out ? v_out : v_cache};
+  const char* names[2] = {"k_cache", "v_cache"};
+  for (int i = 0; i < 2; ++i) {
+    if ((rc = check_tensor(src[i], names[i], 4)) || (rc = check_vec_rows(src[i], names[i]))) return rc;
+    if ((rc = check_tensor(dst[i], "result", 4)) || (rc = check_vec_rows(dst[i], "result")) || (rc = check_distinct(dst[i], "result")))
+      return rc;
+    if (!is_float(src[i]->dtype) || src[i]->dtype != k_cache->dtype || dst[i]->dtype != k_cache->dtype)
+      return fail(SAGA_ERR_INVALID, "the caches must share one float dtype");
+    if (src[i]->shape[0] != k_cache->shape[0] || src[i]->shape[2] != k_cache->shape[2] || src[i]->shape[3] != k_cache->shape[3])
+      return fail(SAGA_ERR_INVALID, "caches: shapes must be [B, n_k, Lmax, d] and [B, n_v, Lmax, d]");
+    if (dst[i]->shape[0] != src[i]->shape[0] || dst[i]->shape[1] != src[i]->shape[1] || dst[i]->shape[3] != src[i]->shape[3] ||
+        (out && dst[i]->shape[2] < keep))
+      return fail(SAGA_ERR_INVALID, "results: shapes must be [B, heads, >= keep, d]");
+    const int64_t es = elt_size(k_cache->dtype);
+    p.rows[i].src = static_cast<const char*>(src[i]->data);
+    p.rows[i].s_sb = src[i]->stride[0] * es, p.rows[i].s_sh = src[i]->stride[1] * es, p.rows[i].s_sl = src[i]->stride[2] * es;
+    p.rows[i].dst = static_cast<char*>(dst[i]->data);
+    p.rows[i].d_sb = dst[i]->stride[0] * es, p.rows[i].d_sh = dst[i]->stride[1] * es, p.rows[i].d_sl = dst[i]->stride[2] * es;
+  }
+  const int64_t d = k_cache->shape[3], row = d * elt_size(k_cache->dtype);
+  if (d != 64 && d != 128) return fail(SAGA_ERR_UNSUPPORTED, "head_dim %lld not built (64, 128)", (long long)d);
+  if (k_cache->shape[2] >= kMaxLen || k_cache->shape[1] > 65535 || v_cache->shape[1] > 65535)
+    return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  p.shift = 6;
+  return evict_run(p, weights, kv_len, keep, recent, out, weights_out, k_cache->shape[0], k_cache->shape[1],
+                   v_cache->shape[1], k_cache->shape[2], row, kept, workspace, workspace_bytes, stream);
+}
+
+int saga_evict_kv_fp8(const saga_kv_fp8* cache, const saga_tensor* weights, const int32_t* kv_len, int64_t keep,
+                      int64_t recent, const saga_kv_fp8* cache_out, const saga_tensor* weights_out, int32_t* kept,
+                      void* workspace, size_t workspace_bytes, saga_stream_t stream) {
+  int rc;
+  EvictParams p{};
+  KvFp8 kv, ov;
+  const bool out = cache_out || weights_out;
+  if ((rc = check_kv_fp8(cache, !out, kv)) || (rc = check_kv_fp8(out ? cache_out : cache, true, ov))) return rc;
+  if (out && (ov.B != kv.B || ov.n_k != kv.n_k || ov.n_v != kv.n_v || ov.d != kv.d || ov.shift != kv.shift || ov.Lmax < keep))
+    return fail(SAGA_ERR_INVALID, "cache_out: the cache's heads, head dim and block, and at least keep positions required");
+  EvictRows &k = p.rows[0], &v = p.rows[1];
+  k.src = kv.kc, k.s_sb = kv.kc_sb, k.s_sh = kv.kc_sh, k.s_sl = kv.kc_sl;
+  v.src = kv.vc, v.s_sb = kv.vc_sb, v.s_sh = kv.vc_sh, v.s_sl = kv.vc_sl;
+  k.dst = const_cast<char*>(ov.kc), k.d_sb = ov.kc_sb, k.d_sh = ov.kc_sh, k.d_sl = ov.kc_sl;
+  v.dst = const_cast<char*>(ov.vc), v.d_sb = ov.vc_sb, v.d_sh = ov.vc_sh, v.d_sl = ov.vc_sl;
+  k.ss = kv.ks, k.ss_sb = kv.ks_sb, k.ss_sh = kv.ks_sh;
+  v.ss = kv.vs, v.ss_sb = kv.vs_sb, v.ss_sh = kv.vs_sh;
+  k.ds = const_cast<float*>(ov.ks), k.ds_sb = ov.ks_sb, k.ds_sh = ov.ks_sh;
+  v.ds = const_cast<float*>(ov.vs), v.ds_sb = ov.vs_sb, v.ds_sh = ov.vs_sh;
+  p.fp8 = 1;
+  p.shift = kv.shift;
+  return evict_run(p, weights, kv_len, keep, recent, out, weights_out, kv.B, kv.n_k, kv.n_v, kv.Lmax, kv.d, kept, workspace,
+                   workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -27,6 +27,7 @@
 // 1 x 4096 5.7 + 3.5; every further step per wave 1.0 us (d 64) to 2.3 (d 128, 14 MB a step).
 #include <algorithm>
 
+#include "dense_join.cuh"
 #include "kernels.h"
 #include "q4.cuh"
 
@@ -430,73 +431,6 @@ __global__ void __launch_bounds__(256, 2) dense_q4_kernel(DenseQ4Params p) {
   }
 }
 
-// Joins a head's splits: one block per (batch row, head, JD dims), GR x JD threads; thread
-// (grp, i) sums dim i of the splits grp, grp + GR, ..., the groups add up in a
-// fixed order.  A round's sums are loaded before its references are known, so that a
-// call of at most 8 GR splits waits for memory once.  More than 64 splits (few units, long
-// rows) are read by more blocks, of 32 dims each: 1 x 32768 positions (12 heads, 256 splits)
-// 15.1 -> 12.2 us with the first kernel; at 64 splits (8 x 32768) 21.3 -> 22.4.
-constexpr int kJoinSplits = 1024;
-
-template <int D, int JD, int GR>
-__global__ void __launch_bounds__(GR * JD) dense_q4_join_kernel(DenseQ4Params p) {
-  constexpr int NT = GR * JD;
-  __shared__ float fm[kJoinSplits];
-  __shared__ float red[NT / kWave];
-  __shared__ float og[GR][JD];
-  const int tid = threadIdx.x, grp = tid / JD, i = tid - grp * JD;
-  const int row = blockIdx.x / (D / JD), d0 = (blockIdx.x - row * (D / JD)) * JD;
-  const int bi = row / p.q_h, h = row - bi * p.q_h;
-  const float* base = p.part + static_cast<int64_t>(row) * p.nsplit * D + d0 + i;
-  const float2* ml = reinterpret_cast<const float2*>(p.part + static_cast<int64_t>(p.b) * p.q_h * p.nsplit * D) +
-                     static_cast<int64_t>(row) * p.nsplit;
-  float ov[8];
-  auto load_round = [&](int q0) {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) ov[u] = base[min(q0 + GR * u, p.nsplit - 1) * D];
-  };
-  load_round(grp);
-  float2 v[kJoinSplits / NT];
-  float mloc = kNegInf;
-#pragma unroll
-  for (int k = 0; k < kJoinSplits / NT; ++k) {
-    const int q = tid + k * NT;
-    v[k] = q < p.nsplit ? ml[q] : float2{kNegInf, 0.f};
-    mloc = fmaxf(mloc, v[k].x);
-  }
-  const float M = block_max<NT / kWave>(mloc, red);
-  float lloc = 0.f;
-#pragma unroll
-  for (int k = 0; k < kJoinSplits / NT; ++k) {
-    const float f = v[k].x == kNegInf ? (v[k].y == 0.f ? 0.f : 1.f) : __expf(v[k].x - M);
-    lloc += v[k].y * f;
-    fm[tid + k * NT] = f;
-  }
-  const float l = block_sum<NT / kWave>(lloc, red);  // orders the writes of fm too
-  float a = 0.f;
-  for (int q0 = grp; q0 < p.nsplit; q0 += 8 * GR) {
-    if (q0 != grp) load_round(q0);
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (q0 + GR * u < p.nsplit) a += ov[u] * fm[q0 + GR * u];
-  }
-  og[grp][i] = a;
-  __syncthreads();
-  if (grp == 0) {
-    float t = og[0][i];
-#pragma unroll
-    for (int q = 1; q < GR; ++q) t += og[q][i];
-    store_from_f32(p.out, p.out_dt, bi * p.o_sb + static_cast<int64_t>(h) * p.o_sh + d0 + i, q4_in_range(t / l, p.out_dt));
-  }
-}
-
-template <int D>
-static void launch_dense_q4_join(const DenseQ4Params& p, hipStream_t st) {
-  const unsigned rows = static_cast<unsigned>(p.b * p.q_h);
-  if (p.nsplit > 64) hipLaunchKernelGGL((dense_q4_join_kernel<D, 32, 32>), dim3(rows * (D / 32)), dim3(1024), 0, st, p);
-  else hipLaunchKernelGGL((dense_q4_join_kernel<D, D, 8>), dim3(rows), dim3(8 * D), 0, st, p);
-}
-
 // As many splits as keep every block resident, two per CU (a few blocks more ran after
 // the others: 8 of 520 took 3 us of 26), each of at least a step per wave; up to 512
 // positions in one, without a join (400 positions 6.4 - 9.9 us against 7.4 - 9.5 in a graph, and
@@ -565,11 +499,11 @@ hipError_t launch_dense_decode_q4(DenseQ4Params& p, hipStream_t st) {
   if (p.kv.d == 128) {
     if (p.kv.group == 32) launch_dense_q4_group<128, 32>(p, nv, st);
     else launch_dense_q4_group<128, 64>(p, nv, st);
-    if (ns > 1) launch_dense_q4_join<128>(p, st);
+    if (ns > 1) launch_dense_join<128>(p, st);
   } else {
     if (p.kv.group == 32) launch_dense_q4_group<64, 32>(p, nv, st);
     else launch_dense_q4_group<64, 64>(p, nv, st);
-    if (ns > 1) launch_dense_q4_join<64>(p, st);
+    if (ns > 1) launch_dense_join<64>(p, st);
   }
   return hipGetLastError();
 }

@@ -408,4 +408,120 @@ struct UnpackQ4Params {
 };
 hipError_t launch_unpack_q4(UnpackQ4Params& p, hipStream_t st);
 
+// ---- norms with rotation and append; a cache held in 8 bits (form: include/saga_amd.h) ----
+
+// An 8-bit cache: pointers, byte strides of the codes (batch row, head, position), strides of
+// the scales in floats (batch row, head; a head's blocks are adjacent).
+struct KvFp8 {
+  const char *kc, *vc;
+  const float *ks, *vs;
+  int64_t kc_sb, kc_sh, kc_sl, vc_sb, vc_sh, vc_sl, ks_sb, ks_sh, vs_sb, vs_sh;
+  int32_t B, n_k, n_v, Lmax, d;
+  int32_t shift;  // log2 of the positions of a block
+};
+
+struct NormRopeParams {
+  const void* qkv;
+  int64_t qkv_ld;
+  void* q_out;
+  int64_t q_sn, q_sh;
+  int32_t dt, N, n_q, n_k, n_v, d;
+  int32_t vec;  // 16-byte vectors in every row
+  const float* table;
+  const void *q_norm, *k_norm;  // [d] of type dt, null: no norm
+  float eps;
+  // caches of type dt: a token's row is [batch[n], :, pos[n]]
+  const int32_t *pos, *batch;
+  void *k_cache, *v_cache;
+  int64_t k_sb, k_sh, k_sl, v_sb, v_sh, v_sl;
+  int32_t B, Lmax;
+  // 8-bit cache: row i of `rows` takes tokens offsets[i] .. offsets[i + 1] - 1 (null: N / rows each)
+  // at positions start[i] ..
+  KvFp8 kv;
+  const int32_t *start, *offsets;
+  int32_t rows;
+};
+hipError_t launch_norm_rope_kv_append(const NormRopeParams& p, hipStream_t st);
+hipError_t launch_norm_rope_kv_append_fp8(const NormRopeParams& p, hipStream_t st);
+
+struct KvFp8ReadParams {
+  KvFp8 kv;
+  const int32_t *pos, *batch;
+  void *k, *v;
+  int64_t k_sn, k_sh, v_sn, v_sh;
+  int32_t dt, N, vec;
+};
+hipError_t launch_kv_fp8_read(const KvFp8ReadParams& p, hipStream_t st);
+
+struct DenseFp8Params {
+  KvFp8 kv;
+  const char* q;
+  int64_t q_sb, q_sh;  // elements
+  int32_t q_dt;
+  const void* mask;
+  int32_t mask_dt;
+  int64_t m_sb, m_sh, m_sl;
+  const int32_t* kv_len;
+  int32_t b, q_h, L;
+  int32_t g, g_v;  // query heads per key head and per value head
+  int32_t nseg;    // units of query heads per batch row (set at launch, with the splits)
+  float scale;
+  void* out;
+  int32_t out_dt;
+  int64_t o_sb, o_sh;
+  float* part;  // sums [b * q_h][nsplit][d], then (reference, sum of weights) [b * q_h][nsplit][2]
+  int32_t nsplit, split_len;
+  float* scores;  // [b * q_h][scores_ld] of the positions below kv_len, null: not asked for
+  int64_t scores_ld;
+};
+hipError_t launch_dense_decode_fp8(DenseFp8Params& p, hipStream_t st);
+
+// ---- attention weights per position, eviction ----
+
+// w[b, G, position] (+)= the softmax weights of the row's query heads, from scores and from partial
+// (reference, sum of weights) pairs of their softmax.
+struct WeightsParams {
+  const float* scores;
+  int64_t s_ld;  // a (batch, query head) row
+  const float *pm, *ps;  // [b * q_h][nparts], pstride floats apart
+  int32_t nparts, pstride;
+  const int32_t* kv_len;
+  int32_t b, q_h, G, L;
+  float* w;
+  int64_t w_sb, w_sg;
+  int32_t add;
+};
+hipError_t launch_attention_weights(const WeightsParams& p, hipStream_t st);
+
+// One kind of rows that an eviction moves: 16-byte pieces, byte strides.
+struct EvictRows {
+  const char* src;
+  int64_t s_sb, s_sh, s_sl;
+  char* dst;
+  int64_t d_sb, d_sh, d_sl;
+  const float* ss;  // 8 bits: scales, strides in floats
+  int64_t ss_sb, ss_sh;
+  float* ds;
+  int64_t ds_sb, ds_sh;
+  char* stage;        // in place: rows [B][heads][staged] of the end of what is kept
+  float* stage_s;
+  int32_t heads, pieces;
+};
+struct EvictParams {
+  EvictRows rows[2];  // keys, values
+  const float* w;
+  int64_t w_sb, w_sg;
+  float* w_out;
+  int64_t wo_sb, wo_sg, wo_len;
+  const int32_t* kv_len;
+  int32_t* kept;   // [B][G][keep]
+  int32_t* movers; // [B][G][keep]
+  float* held_w;   // [B][G][keep]
+  int32_t B, G, Lmax, keep, recent;
+  int32_t shift;    // log2 of the positions of a block (6 for rows without scales)
+  int32_t fp8, in_place;
+  int32_t staged0;  // in place: first staged position, a block's first
+};
+hipError_t launch_evict(const EvictParams& p, hipStream_t st);
+
 }  // namespace saga

@@ -50,8 +50,8 @@ __device__ __forceinline__ u32x4 q4_minus_base() { return u32x4{0xc300c300u, 0xc
 __device__ __forceinline__ float q4_lo(uint32_t sz) { return f16_bits_to_f32(sz & 0xffffu); }  // scale
 __device__ __forceinline__ float q4_hi(uint32_t sz) { return f16_bits_to_f32(sz >> 16); }      // offset
 
-// What a result of type dt holds of v.  A group's scale is rounded up, so that its largest value may read a
-// few units past 65504 although what was stored fits f16: finite results end at f16's range.
+// What a result of type dt holds of v.  A group's scale is rounded up (4 bits), or the value itself (e4m3), so that
+// the largest value may read as up to 65536 although what was stored fits f16: finite results end at f16's range.
 __device__ __forceinline__ float q4_in_range(float v, int dt) {
   return dt == SAGA_DTYPE_F16 && fabsf(v) > 65504.f && fabsf(v) < __builtin_inff() ? copysignf(65504.f, v) : v;
 }

@@ -849,3 +849,180 @@ def dense_decode_q4(query, cache: KVQ4, attention_mask=None, scaling=None, kv_le
     _on_device(dev, "dense_decode_q4", lib.saga_dense_decode_q4, _lib.packed(query), _kv_q4(cache), _packed(mask),
                _address(_kv_len(kv_len)), _scale(query, scaling), _lib.packed(out), ws.data_ptr(), ws.numel())
     return out
+
+
+# ------------------------- norms of queries and keys, a cache held in 8 bits, a cache kept short
+
+class KVFP8(NamedTuple):
+    """A layer's key / value cache in 8 bits: codes uint8 [B, heads, Lmax, d], the bytes of e4m3 numbers
+    (.view(torch.float8_e4m3fn)), and scales f32 [B, heads, ceil(Lmax / block)], one per `block` (32, 64 or 128)
+    consecutive positions: value = scale * number (include/saga_amd.h)."""
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+    block: int
+
+    def rows(self, first: int, count: int = 1) -> "KVFP8":
+        """The cache of `count` batch rows from `first` on (views)."""
+        return KVFP8(*(t[first:first + count] for t in self[:4]), self.block)
+
+
+_BLOCK_PACK = struct.Struct("=q").pack
+
+
+def _kv_fp8(cache: KVFP8) -> bytes:
+    kc, ks, vc, vs, block = cache
+    return _lib.packed(kc) + _lib.packed(ks) + _lib.packed(vc) + _lib.packed(vs) + _BLOCK_PACK(block)
+
+
+def _rope_rows(rope_table, n: int, d: int) -> None:
+    if rope_table.dtype is not torch.float32 or rope_table.shape != (n, d // 2, 2) or not rope_table.is_contiguous():
+        raise ValueError("saga_amd: rope_table must be a contiguous float32 [N, d/2, 2] tensor")
+
+
+def norm_rope_kv_append(qkv, n_q, rope_table, pos, k_cache, v_cache, q_norm=None, k_norm=None, eps=1e-6, batch=None,
+                        q_out=None):
+    """New tokens into a cache, RMSNorm of every query and key head (weights q_norm, k_norm [d] of qkv's type; None: no
+    norm), rotation and append in one launch: rows [batch, :, pos] of k_cache and v_cache (batch None: token n is batch
+    row n), each pair (batch, pos) at most once per call.  qkv [N, (n_q+n_k+n_v)*d], d 64 or 128; rope_table:
+    rope_table(positions, d, theta) of these tokens, whose positions need not be the rows'.  Returns q_out [N, n_q, d]."""
+    dev = _need_gpu(qkv, rope_table, pos, k_cache, v_cache, q_norm, k_norm, batch, q_out)
+    n, d = qkv.size(0), k_cache.size(-1)
+    _indices(pos, batch, n)
+    _rope_rows(rope_table, n, d)
+    if q_out is None:
+        q_out = qkv.new_empty(n, n_q, d)
+    _on_device(dev, "norm_rope_kv_append", _lib.load().saga_norm_rope_kv_append, _lib.packed(qkv), n_q,
+               rope_table.data_ptr(), _packed(q_norm), _packed(k_norm), float(eps), pos.data_ptr(), _address(batch),
+               _lib.packed(q_out), _lib.packed(k_cache), _lib.packed(v_cache))
+    return q_out
+
+
+def norm_rope_kv_append_fp8(qkv, n_q, rope_table, start, cache: KVFP8, q_norm=None, k_norm=None, eps=1e-6, offsets=None,
+                            q_out=None):
+    """norm_rope_kv_append into an 8-bit cache: batch row i of the first start.numel() takes tokens
+    offsets[i] .. offsets[i+1] - 1 (int32 [rows + 1]; None: N / rows each) at positions start[i], start[i] + 1, ...
+    (int32 [rows]), in blocks of cache.block that share a scale: a token at a block's first position starts it anew,
+    what a block holds behind a call's last token is lost.  Returns q_out [N, n_q, d]."""
+    dev = _need_gpu(qkv, rope_table, start, q_norm, k_norm, offsets, q_out, *cache[:4])
+    n, d, rows = qkv.size(0), cache.k_codes.size(-1), start.numel()
+    for t, name, m in ((start, "start", rows), (offsets, "offsets", rows + 1)):
+        if t is not None and (t.dtype is not torch.int32 or t.shape != (m,) or not t.is_contiguous()):
+            raise ValueError(f"saga_amd: {name} must be a contiguous int32 [{m}] tensor")
+    _rope_rows(rope_table, n, d)
+    if q_out is None:
+        q_out = qkv.new_empty(n, n_q, d)
+    _on_device(dev, "norm_rope_kv_append_fp8", _lib.load().saga_norm_rope_kv_append_fp8, _lib.packed(qkv), n_q,
+               rope_table.data_ptr(), _packed(q_norm), _packed(k_norm), float(eps), start.data_ptr(), _address(offsets),
+               rows, _lib.packed(q_out), _kv_fp8(cache))
+    return q_out
+
+
+def read_kv_fp8(cache: KVFP8, pos, batch=None, dtype=torch.bfloat16):
+    """What an 8-bit cache holds at [batch, :, pos] (batch None: row n): k [N, n_k, d] and v [N, n_v, d] of `dtype`,
+    NaN where an index is out of range.  Transposed to [1, heads, N, d] they are prefill_attention's operands."""
+    dev = _need_gpu(pos, batch, *cache[:4])
+    n, d = pos.size(0), cache.k_codes.size(-1)
+    _indices(pos, batch, n)
+    k, v = (torch.empty(n, t.size(1), d, dtype=dtype, device=dev) for t in (cache.k_codes, cache.v_codes))
+    _on_device(dev, "read_kv_fp8", _lib.load().saga_kv_fp8_read, _kv_fp8(cache), pos.data_ptr(), _address(batch),
+               _lib.packed(k), _lib.packed(v))
+    return k, v
+
+
+def _row_lengths(kv_len, b: int) -> Optional[torch.Tensor]:
+    if kv_len is not None and kv_len.shape != (b,):
+        raise ValueError("saga_amd: kv_len must be a contiguous int32 tensor [b]")
+    return _kv_len(kv_len)
+
+
+def dense_decode_fp8(query, cache: KVFP8, attention_mask=None, scaling=None, kv_len=None, out=None, out_dtype=None,
+                     workspace=None, weights=None, weights_add=True):
+    """dense_decode over an 8-bit cache (query bf16 or f16 [b, q_h, 1, d]).  weights: f32 [b, G, >= L] that receives
+    the weight of every position as attention_weights writes it (weights_add: added to what is there), G a common
+    divisor of the key and value heads."""
+    dev = _need_gpu(query, attention_mask, kv_len, out, weights, *cache[:4])
+    query = _vec_ready(query)
+    b, q_h, l_q, d = query.shape
+    if l_q != 1:
+        raise NotImplementedError("saga_amd: the HIP decode kernels take l_q == 1")
+    L = cache.k_codes.size(2)
+    mask = _mask_view(attention_mask, L)
+    kv_len = _row_lengths(kv_len, b)
+    if out is None:
+        out = query.new_empty(b, q_h, 1, d, dtype=out_dtype)
+    lib = _lib.load()
+    ws = _take_workspace(workspace, dev, "dense_fp8", lib.saga_dense_fp8_workspace_bytes(b, q_h, L, d, weights is not None))
+    _on_device(dev, "dense_decode_fp8", lib.saga_dense_decode_fp8, _lib.packed(query), _kv_fp8(cache), _packed(mask),
+               _address(kv_len), _scale(query, scaling), _lib.packed(out), _packed(weights), 1 if weights_add else 0,
+               ws.data_ptr(), ws.numel())
+    return out
+
+
+def attention_weights(query, key, weights, attention_mask=None, scaling=None, kv_len=None, add=True, workspace=None):
+    """The softmax weight that every position gets from one decode step (query [b, q_h, 1, d], key [b, k_h, L, d]):
+    weights f32 [b, G, >= L], G a divisor of k_h; weights[i, u, j] is the sum over the query heads of group u (q_h / G
+    consecutive ones).  add: added to what is there at the positions below kv_len; else written, 0 from kv_len to L.
+    A head without a finite softmax adds nothing.  Several queries of one sequence are rows of an expanded key (batch
+    stride 0), each with a kv_len of its own.  Returns weights."""
+    dev = _need_gpu(query, key, weights, attention_mask, kv_len)
+    query, key = _vec_ready(query), _vec_ready(key)
+    b, q_h, l_q, _ = query.shape
+    if l_q != 1:
+        raise NotImplementedError("saga_amd: the HIP decode kernels take l_q == 1")
+    L = key.size(2)
+    mask = _mask_view(attention_mask, L)
+    kv_len = _row_lengths(kv_len, b)
+    lib = _lib.load()
+    ws = _take_workspace(workspace, dev, "attention_weights",
+                         lib.saga_attention_weights_workspace_bytes(b, q_h, key.size(1), L))
+    _on_device(dev, "attention_weights", lib.saga_attention_weights, _lib.packed(query), _lib.packed(key), _packed(mask),
+               _address(kv_len), _scale(query, scaling), _lib.packed(weights), 1 if add else 0, ws.data_ptr(), ws.numel())
+    return weights
+
+
+def _evict(entry, what, dev, tensors, k_like, heads, row_bytes, weights, kv_len, keep, recent, outs, kept, workspace):
+    b, g = k_like.size(0), weights.size(1)
+    if kv_len is None:
+        raise ValueError("saga_amd: an eviction needs kv_len")
+    kv_len = _row_lengths(kv_len, b)
+    keep, recent = int(keep), int(recent)
+    if keep < 1 or not 0 <= recent <= keep:
+        raise ValueError(f"saga_amd: keep >= 1 and 0 <= recent <= keep required, got {keep} and {recent}")
+    if kept is None:
+        kept = torch.empty(b, g, keep, dtype=torch.int32, device=dev)
+    elif kept.dtype is not torch.int32 or kept.shape != (b, g, keep) or not kept.is_contiguous():
+        raise ValueError("saga_amd: kept must be a contiguous int32 [B, G, keep] tensor")
+    ws = _take_workspace(workspace, dev, "evict", _lib.load().saga_evict_workspace_bytes(
+        b, g, keep, recent, heads, row_bytes, not any(outs)))
+    _on_device(dev, what, entry, *tensors, _lib.packed(weights), kv_len.data_ptr(), keep, recent, *outs, kept.data_ptr(),
+               ws.data_ptr(), ws.numel())
+    return kept
+
+
+def evict_kv(k_cache, v_cache, weights, kv_len, keep, recent=0, out=None, kept=None, workspace=None):
+    """Eviction from a cache by gathered attention weight: batch rows of more than `keep` positions (kv_len int32 [B])
+    keep the last `recent` and, of the others, the keep - recent of largest weight (weights f32 [B, G, >= Lmax]; G a
+    common divisor of the key and value heads, each group of heads keeps positions of its own; equal weights: the lower
+    position, NaN above all numbers).  Kept positions below keep - recent stay where they are, the gaps there take the
+    others in their order, the last `recent` follow.  Rows and weights move together.  In place (weights behind
+    min(kv_len, keep) become 0), or into out = (k, v, weights) of at least `keep` positions; kv_len is the caller's to
+    cut to `keep`.  Returns kept int32 [B, G, keep]: the position that each place held before, -1 behind kv_len."""
+    k_out, v_out, w_out = out if out is not None else (None, None, None)
+    dev = _need_gpu(k_cache, v_cache, weights, kv_len, k_out, v_out, w_out, kept)
+    lib = _lib.load()
+    return _evict(lib.saga_evict_kv, "evict_kv", dev, (_lib.packed(k_cache), _lib.packed(v_cache)), k_cache,
+                  k_cache.size(1) + v_cache.size(1), k_cache.size(-1) * k_cache.element_size(), weights, kv_len, keep,
+                  recent, (_packed(k_out), _packed(v_out), _packed(w_out)), kept, workspace)
+
+
+def evict_kv_fp8(cache: KVFP8, weights, kv_len, keep, recent=0, out=None, kept=None, workspace=None):
+    """evict_kv over an 8-bit cache; out = (KVFP8 of the same block, weights).  A block of the result takes the largest
+    of its rows' scales."""
+    c_out, w_out = out if out is not None else (None, None)
+    dev = _need_gpu(weights, kv_len, w_out, kept, *cache[:4], *(c_out[:4] if c_out is not None else ()))
+    lib = _lib.load()
+    return _evict(lib.saga_evict_kv_fp8, "evict_kv_fp8", dev, (_kv_fp8(cache),), cache.k_codes,
+                  cache.k_codes.size(1) + cache.v_codes.size(1), cache.k_codes.size(-1), weights, kv_len, keep, recent,
+                  (None if c_out is None else _kv_fp8(c_out), _packed(w_out)), kept, workspace)
