@@ -10,80 +10,73 @@ namespace saga {
 
 // ---- weights per position ----
 
-// Weights of CH positions of one (batch row, group of query heads): w (+)= sum_h exp(x_h - M_h) / l_h,
-// where M_h and l_h come from the softmax's partial (reference, sum) pairs.  A head without a
-// finite sum (no position, a NaN score) adds nothing.  The heads of a position are added by one
-// thread in their order.  Reads the scores (4 bytes a head and position) and writes 4 bytes a
-// group and position; every block joins its heads' partials itself (a launch less).
-constexpr int kWeightHeads = 64;  // heads whose (M, 1 / l) are held at a time
+// w (+)= sum_h exp(x_h - M_h) / l_h of one (batch row, group of query heads), where M_h and l_h come from
+// the softmax's partial (reference, sum) pairs.  A head without a finite sum (no position, a NaN
+// score) adds nothing.  A thread adds the heads of its position in their order.  Every block
+// joins its heads' partials itself (a launch less), under the loads of its first scores.
+// Bound by the scores (4 bytes a head and position read, 4 bytes a group and position written).
+constexpr int kWeightHeads = 16;  // heads whose scores are in flight at a time
 
-template <int PER>
 __global__ void __launch_bounds__(256) attention_weights_kernel(WeightsParams p) {
   __shared__ float fm[kWeightHeads], fr[kWeightHeads];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int nchunk = (p.L + 256 * PER - 1) / (256 * PER);
-  const int row = blockIdx.x / nchunk, chunk = blockIdx.x - row * nchunk;
+  const int nchunk = (p.L + 255) / 256;
+  const int row = blockIdx.x / nchunk, pos = (blockIdx.x - row * nchunk) * 256 + tid;
   const int bi = row / p.G, gi = row - bi * p.G, gq = p.q_h / p.G;
   int Leff = p.L;
   if (p.kv_len) Leff = min(Leff, max(p.kv_len[bi], 0));
-  const int pos0 = chunk * 256 * PER;
-  float* w = p.w + bi * p.w_sb + gi * p.w_sg;
-  if (pos0 >= Leff) {
-    if (!p.add) {
-#pragma unroll
-      for (int k = 0; k < PER; ++k)
-        if (pos0 + k * 256 + tid < p.L) w[pos0 + k * 256 + tid] = 0.f;
-    }
+  float* w = p.w + bi * p.w_sb + gi * p.w_sg + pos;
+  if (pos - tid >= Leff) {
+    if (!p.add && pos < p.L) *w = 0.f;
     return;
   }
-  float acc[PER];
-#pragma unroll
-  for (int k = 0; k < PER; ++k) acc[k] = 0.f;
+  const int64_t r0 = static_cast<int64_t>(bi) * p.q_h + gi * gq;
+  const float* x0 = p.scores + r0 * p.s_ld + min(pos, Leff - 1);
+  float acc = 0.f;
   for (int hb = 0; hb < gq; hb += kWeightHeads) {
     const int n = min(gq - hb, kWeightHeads);
-    const int64_t r0 = static_cast<int64_t>(bi) * p.q_h + gi * gq + hb;
+    float x[kWeightHeads];
+#pragma unroll
+    for (int i = 0; i < kWeightHeads; ++i) x[i] = x0[min(hb + i, gq - 1) * p.s_ld];
     if (hb) __syncthreads();
     for (int i = wave; i < n; i += 4) {
-      const int64_t base = (r0 + i) * p.nparts;
-      float m = kNegInf;
-      for (int q = lane; q < p.nparts; q += 64) m = fmaxf(m, p.pm[(base + q) * p.pstride]);
-      m = wave_max(m);
-      float l = 0.f;
-      for (int q = lane; q < p.nparts; q += 64) {
-        const float pm = p.pm[(base + q) * p.pstride], ps = p.ps[(base + q) * p.pstride];
-        l += pm == kNegInf ? ps : ps * __expf(pm - m);  // (an empty part holds (-inf, 0), one of NaN scores a NaN sum)
+      const int64_t base = (r0 + hb + i) * p.nparts;
+      float m = kNegInf, l = 0.f;  // (an empty part holds (-inf, 0), one of NaN scores a NaN sum)
+      for (int q0 = lane; q0 < p.nparts; q0 += 256) {
+        float pm[4], ps[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int64_t at = (base + min(q0 + 64 * u, p.nparts - 1)) * p.pstride;
+          pm[u] = q0 + 64 * u < p.nparts ? p.pm[at] : kNegInf;
+          ps[u] = q0 + 64 * u < p.nparts ? p.ps[at] : 0.f;
+        }
+        const float mn = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
+        l = m == kNegInf ? l : l * __expf(m - mn);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) l += pm[u] == kNegInf ? ps[u] : ps[u] * __expf(pm[u] - mn);
+        m = mn;
       }
-      l = wave_sum(l);
+      const float M = wave_max(m);
+      l = wave_sum(m == kNegInf ? l : l * __expf(m - M));
       if (lane == 0) {
         const bool some = l > 0.f && l < __builtin_inff();
-        fm[i] = some ? m : 0.f;
+        fm[i] = some ? M : __builtin_inff();
         fr[i] = some ? 1.f / l : 0.f;
       }
     }
     __syncthreads();
-    const float* x = p.scores + r0 * p.s_ld + pos0 + tid;
-    for (int i = 0; i < n; ++i) {
-      const float m = fm[i], r = fr[i];
 #pragma unroll
-      for (int k = 0; k < PER; ++k)
-        if (r > 0.f && pos0 + k * 256 + tid < Leff) acc[k] += __expf(x[i * p.s_ld + k * 256] - m) * r;
-    }
+    for (int i = 0; i < kWeightHeads; ++i)
+      if (i < n && fr[i] > 0.f) acc += __expf(x[i] - fm[i]) * fr[i];
   }
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int pos = pos0 + k * 256 + tid;
-    if (pos < Leff) w[pos] = p.add ? w[pos] + acc[k] : acc[k];
-    else if (pos < p.L && !p.add) w[pos] = 0.f;
-  }
+  if (pos < Leff) *w = p.add ? *w + acc : acc;
+  else if (pos < p.L && !p.add) *w = 0.f;
 }
 
 hipError_t launch_attention_weights(const WeightsParams& p, hipStream_t st) {
-  const int64_t rows = static_cast<int64_t>(p.b) * p.G;
-  const int per = rows * ((p.L + 1023) / 1024) >= 256 ? 4 : 1;
-  const int64_t blocks = rows * ((p.L + 256LL * per - 1) / (256 * per));
+  const int64_t blocks = static_cast<int64_t>(p.b) * p.G * ((p.L + 255LL) / 256);
   if (blocks >= (1LL << 24)) return hipErrorInvalidValue;  // a launch holds less than 2^32 threads
-  if (per == 4) hipLaunchKernelGGL(attention_weights_kernel<4>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(attention_weights_kernel<1>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(attention_weights_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 
@@ -98,31 +91,51 @@ hipError_t launch_attention_weights(const WeightsParams& p, hipStream_t st) {
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 
+template <int SEG>
 struct SelShared {
+  uint32_t key[SEG];  // ranking keys; then, of a row of one segment, the positions that move
   int hist[2048];
   int cnt[kSelWaves];
   int sel_bin, sel_above, sel_cnt;
-  int eq[kSelWaves], mov[kSelWaves], gap[kSelWaves];
+  int sums[3][kSelWaves];
+  unsigned long long a[SEG / kWave], b[SEG / kWave];  // per chunk: masks of keys above T and equal to it, then of
+  int a0[SEG / kWave], b0[SEG / kWave];               // those that move and of the gaps, and their first ones' ranks
 };
 
-// A weight as what it is ranked by: any NaN above all numbers, -0 as 0.
-__device__ __forceinline__ float rank_value(float w) { return w == w ? w + 0.f : __uint_as_float(0x7fffffffu); }
+// A weight as what it is ranked by: any NaN above all numbers, -0 as 0; never 0, which stands for no position.
+__device__ __forceinline__ uint32_t rank_key(float w) { return f32_to_key(w == w ? w + 0.f : __uint_as_float(0x7fffffffu)); }
 
-// One block per (batch row, group): wave v holds positions [v S, (v + 1) S), lane by lane, S a
-// multiple of 64, so that a position's rank in a class is a count of its wave's ballots. The
-// H-th largest by radix (11, 11, 10 bits), equal ones by position.  R: passes of 64 a wave
-// holds in registers, 0: reads them again (rows longer than 16 x 64 x 64).
-template <int R>
+// The lowest `count` set bits of m.
+__device__ __forceinline__ unsigned long long low_bits(unsigned long long m, int count) {
+  if (count == 0) return 0ull;
+  const int drop = __popcll(m) - count;
+  for (int i = 0; i < drop; ++i) m &= ~(1ull << (63 - __clzll(static_cast<long long>(m))));
+  return m;
+}
+
+// Bits of positions below `end` of a chunk of 64 that starts at p0.
+__device__ __forceinline__ unsigned long long bits_below(int end, int p0) {
+  const int n = min(max(end - p0, 0), 64);
+  return n == 0 ? 0ull : ~0ull >> (64 - n);
+}
+
+// One block per (batch row, group), a segment of SEG positions' ranking keys in LDS (a row of one
+// segment is read once, longer ones for every pass).  The H-th largest key by radix (11, 11, 10
+// bits), equal ones by position.  What is large of a chunk of 64 positions is then one 64-bit
+// mask, and thread c counts chunk c: every prefix of the selection is one scan of the block, and a
+// wave places its chunks' positions with one count each.
+template <int SEG>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p) {
-  __shared__ SelShared sh;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ SelShared<SEG> sh;
+  constexpr int CH = SEG / kWave;
+  static_assert(CH <= kSelThreads && SEG % kSelThreads == 0, "a thread per chunk");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bi = blockIdx.x / p.G, gi = blockIdx.x - bi * p.G;
   const int n = min(max(p.kv_len[bi], 0), p.Lmax);
   const float* w = p.w + bi * p.w_sb + gi * p.w_sg;
   float* wo = p.w_out + bi * p.wo_sb + gi * p.wo_sg;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * p.keep;
   int32_t *kept = p.kept + row, *movers = p.movers + row;
-  float* held = p.held_w + row;
   const int wlen = static_cast<int>(p.wo_len);
   if (n <= p.keep) {
     for (int j = tid; j < p.keep; j += kSelThreads) {
@@ -133,115 +146,161 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
     return;
   }
   const int H = p.keep - p.recent, nc = n - p.recent;  // candidates: [0, nc), nc > H
-  const int span = (nc + kSelThreads - 1) / kSelThreads * kWave, base = wave * span;
-  float reg[R > 0 ? R : 1];
-  if constexpr (R > 0) {
+  const int nseg = (nc + SEG - 1) / SEG;
+  constexpr int U = 4;
+  auto load = [&](int seg) {  // (a thread's own keys: no barrier is needed to count them)
+    for (int j0 = tid; j0 < min(SEG, nc - seg * SEG); j0 += 2 * U * kSelThreads) {
+      float v[2 * U];
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int pos = base + k * kWave + lane;
-      reg[k] = k * kWave < span && pos < nc ? rank_value(w[pos]) : 0.f;
-    }
-  }
-  // f(k, pos, value) of this lane's candidates; whole waves
-  auto each = [&](auto f) {
-    if constexpr (R > 0) {
+      for (int u = 0; u < 2 * U; ++u) v[u] = w[min(seg * SEG + j0 + u * kSelThreads, nc - 1)];
 #pragma unroll
-      for (int k = 0; k < R; ++k) {
-        if (k * kWave >= span) break;
-        f(base + k * kWave + lane, reg[k]);
-      }
-    } else {
-      for (int k = 0; k * kWave < span; ++k) {
-        const int pos = base + k * kWave + lane;
-        f(pos, pos < nc ? rank_value(w[pos]) : 0.f);
-      }
+      for (int u = 0; u < 2 * U; ++u)
+        if (j0 + u * kSelThreads < SEG) sh.key[j0 + u * kSelThreads] = seg * SEG + j0 + u * kSelThreads < nc ? rank_key(v[u]) : 0u;
     }
   };
+  // f(chunk, key) of the segment's chunks, wave by wave; keys are 0 behind nc
+  auto chunks = [&](int seg, auto f) {
+    const int nch = (min(SEG, nc - seg * SEG) + kWave - 1) / kWave;
+    for (int c0 = wave; c0 < nch; c0 += U * kSelWaves) {
+      uint32_t key[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) key[u] = c0 + u * kSelWaves < nch ? sh.key[(c0 + u * kSelWaves) * kWave + lane] : 0u;
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(c0 + u * kSelWaves, key[u]);
+    }
+  };
+  load(0);
   uint32_t T = 0xffffffffu;  // the H-th largest key
   int need = 0;              // of those equal to it, the first `need` stay
   if (H > 0) {
+    constexpr uint32_t kZero = 0x80000000u;
     need = H;
-    // (positions past nc take no part: filtered by position)
     uint32_t prefix = 0;
-    const int shifts[3] = {21, 10, 0}, nbits[3] = {11, 11, 10};
-#pragma unroll
+#pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
-      const int nb = 1 << nbits[pass];
-      const uint32_t hmask = pass == 0 ? 0u : (0xffffffffu << (shifts[pass] + nbits[pass]));
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, nb = pass == 2 ? 1024 : 2048;
+      const uint32_t hmask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
       for (int i = tid; i < 2048; i += kSelThreads) sh.hist[i] = 0;
       lds_sync();
-      each([&](int pos, float v) {
-        const uint32_t key = f32_to_key(v);
-        const bool in = pos < nc && (key & hmask) == prefix;
-        // what never gathered anything is often many: one count for a wave
-        const bool zero = in && key == 0x80000000u;
-        const unsigned long long zeros = __ballot(zero);
-        if (in && !zero) atomicAdd(&sh.hist[(key >> shifts[pass]) & (nb - 1)], 1);
-        if (zeros && lane == 0) atomicAdd(&sh.hist[(0x80000000u >> shifts[pass]) & (nb - 1)], __popcll(zeros));
-      });
+      int zeros = 0;  // weights of 0 may be many: counted by the wave (what is no position counts in the lowest bin)
+      for (int seg = 0; seg < nseg; ++seg) {
+        if (seg || (pass && nseg > 1)) load(seg);
+        chunks(seg, [&](int c, uint32_t key) {
+          const bool zero = key == kZero;
+          zeros += __popcll(__ballot(zero));
+          if ((((key ^ prefix) & hmask) | (zero ? 1u : 0u)) == 0u) atomicAdd(&sh.hist[(key >> shift) & (nb - 1)], 1);
+        });
+      }
+      if (((kZero ^ prefix) & hmask) == 0 && lane == 0 && zeros) atomicAdd(&sh.hist[(kZero >> shift) & (nb - 1)], zeros);
       lds_sync();
       int bin, above, count;
       hist_pick<kSelThreads>(sh, nb, need, bin, above, count);
-      prefix |= static_cast<uint32_t>(bin) << shifts[pass];
+      prefix |= static_cast<uint32_t>(bin) << shift;
       need -= above;
     }
     T = prefix;
   }
-  // equal ones of the waves before
-  int eq = 0;
-  each([&](int pos, float v) { eq += __popcll(__ballot(pos < nc && H > 0 && f32_to_key(v) == T)); });
-  if (lane == 0) sh.eq[wave] = eq;
-  lds_sync();
-  int eq0 = 0;
-  for (int i = 0; i < wave; ++i) eq0 += sh.eq[i];
-  // the large ones: f(pos, value, large) in order
-  const unsigned long long below = lanes_below(lane);
-  auto large = [&](auto f) {
-    int before = eq0;
-    each([&](int pos, float v) {
-      const bool in = pos < nc && H > 0;
-      const uint32_t key = f32_to_key(v);
-      const unsigned long long same = __ballot(in && key == T);
-      const int rank = before + __popcll(same & below);
-      before += __popcll(same);
-      f(pos, in && (key > T || (key == T && rank < need)));
+  int eq_base = 0, mov_base = 0, gap_base = 0;  // of the segments before
+  // The masks and ranks of a segment's chunks
+  auto masks = [&](int seg) {
+    chunks(seg, [&](int c, uint32_t key) {
+      const unsigned long long g = __ballot(key > T), e = __ballot(key == T);
+      if (lane == 0 && c < CH) sh.a[c] = g, sh.b[c] = e;
     });
+    lds_sync();
+    const int p0 = (seg * CH + tid) * kWave;
+    const bool mine = tid < CH && p0 < nc;
+    const unsigned long long gt = mine ? sh.a[tid] : 0ull, eq = mine ? sh.b[tid] : 0ull;
+    auto scan = [&](int v, int which, int& all) {  // v of the threads before, and of all
+      const int incl = wave_incl_scan(v, lane);
+      if (lane == kWave - 1) sh.sums[which][wave] = incl;
+      lds_sync();
+      int before = incl - v;
+      all = 0;
+#pragma unroll
+      for (int i = 0; i < kSelWaves; ++i) {
+        const int s = sh.sums[which][i];
+        before += i < wave ? s : 0;
+        all += s;
+      }
+      return before;
+    };
+    int all;
+    const int ne = __popcll(eq), before = eq_base + scan(ne, 0, all);
+    eq_base += all;
+    const unsigned long long large = gt | low_bits(eq, min(max(need - before, 0), ne)), low = bits_below(H, p0);
+    const unsigned long long mov = large & ~low, gap = mine ? ~large & low : 0ull;
+    const int mov_at = mov_base + scan(__popcll(mov), 1, all);
+    mov_base += all;
+    const int gap_at = gap_base + scan(__popcll(gap), 2, all);
+    gap_base += all;
+    if (mine) sh.a[tid] = mov, sh.b[tid] = gap, sh.a0[tid] = mov_at, sh.b0[tid] = gap_at;
+    lds_sync();
   };
-  int mov = 0, gap = 0;
-  large([&](int pos, bool is) {
-    mov += __popcll(__ballot(is && pos >= H));
-    gap += __popcll(__ballot(!is && pos < H));
-  });
-  if (lane == 0) sh.mov[wave] = mov, sh.gap[wave] = gap;
-  lds_sync();
-  int mov0 = 0, gap0 = 0;
-  for (int i = 0; i < wave; ++i) mov0 += sh.mov[i], gap0 += sh.gap[i];
-  int at = mov0;
-  large([&](int pos, bool is) {
-    const unsigned long long m = __ballot(is && pos >= H);
-    if (is && pos >= H) movers[at + __popcll(m & below)] = pos;
-    at += __popcll(m);
-  });
-  __threadfence_block();
-  __syncthreads();
-  at = gap0;
-  large([&](int pos, bool is) {
-    const bool open = !is && pos < H;
-    const unsigned long long m = __ballot(open);
-    if (pos < H) {
-      const int from = open ? movers[at + __popcll(m & below)] : pos;
-      kept[pos] = from;
-      held[pos] = w[from];
+  const unsigned long long below = lanes_below(lane);
+  for (int seg = 0; seg < nseg; ++seg) {
+    if (nseg > 1) {
+      __syncthreads();  // (the segment before has been read)
+      load(seg);
+      lds_sync();
     }
-    at += __popcll(m);
-  });
+    masks(seg);
+    const int nch = (min(SEG, nc - seg * SEG) + kWave - 1) / kWave, c0 = max(H - seg * SEG, 0) / kWave;  // (none wholly below H)
+    for (int c = c0 + wave; c < nch; c += kSelWaves) {
+      const unsigned long long m = sh.a[c];
+      const int at = sh.a0[c] + __popcll(m & below);
+      if ((m >> lane) & 1) (nseg > 1 ? reinterpret_cast<uint32_t*>(movers) : sh.key)[at] = seg * SEG + c * kWave + lane;
+    }
+  }
+  __syncthreads();
+  // Places below H.  Positions read there are at or past H or stay, so in place nothing is
+  // overwritten before it is read
+  eq_base = mov_base = gap_base = 0;
+  for (int seg = 0; seg * SEG < H; ++seg) {
+    if (nseg > 1) {
+      __syncthreads();
+      load(seg);
+      lds_sync();
+      masks(seg);
+    }
+    const int nch = (min(SEG, H - seg * SEG) + kWave - 1) / kWave;
+    for (int c0 = wave; c0 < nch; c0 += U * kSelWaves) {
+      int from[U];
+      float v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = min(c0 + u * kSelWaves, nch - 1);
+        const unsigned long long g = sh.b[c];
+        from[u] = seg * SEG + c * kWave + lane;
+        if ((g >> lane) & 1) {
+          const int at = sh.b0[c] + __popcll(g & below);
+          from[u] = nseg > 1 ? movers[at] : static_cast<int>(sh.key[at]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = w[min(from[u], nc - 1)];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + u * kSelWaves, pos = seg * SEG + c * kWave + lane;
+        if (c < nch && pos < H) {
+          kept[pos] = from[u];
+          if (!p.in_place || from[u] != pos) wo[pos] = v[u];
+        }
+      }
+    }
+  }
+  // the last `recent`; in place through the workspace, for they may overlap their places
+  float* held = p.held_w + row;
   for (int j = tid; j < p.recent; j += kSelThreads) {
     kept[H + j] = nc + j;
-    held[H + j] = w[nc + j];
+    (p.in_place ? held : wo + H)[j] = w[nc + j];
   }
-  __threadfence_block();
-  __syncthreads();
-  for (int j = tid; j < wlen; j += kSelThreads) wo[j] = j < p.keep ? held[j] : 0.f;
+  if (p.in_place) {
+    __threadfence_block();
+    __syncthreads();
+    for (int j = tid; j < p.recent; j += kSelThreads) wo[H + j] = held[j];
+  }
+  for (int j = p.keep + tid; j < wlen; j += kSelThreads) wo[j] = 0.f;
 }
 
 // Rows to their places: a block of threads per (batch row, head, S positions of the result, S a block of
@@ -326,11 +385,8 @@ static void launch_evict_moves(const EvictParams& p, hipStream_t st) {
 
 hipError_t launch_evict(const EvictParams& p, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.B * p.G)), block(kSelThreads);
-  const int passes = (p.Lmax + kSelThreads - 1) / kSelThreads;
-  if (passes <= 8) hipLaunchKernelGGL(evict_select_kernel<8>, grid, block, 0, st, p);
-  else if (passes <= 32) hipLaunchKernelGGL(evict_select_kernel<32>, grid, block, 0, st, p);
-  else if (passes <= 64) hipLaunchKernelGGL(evict_select_kernel<64>, grid, block, 0, st, p);
-  else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, st, p);
+  if (p.Lmax <= 4096) hipLaunchKernelGGL(evict_select_kernel<4096>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(evict_select_kernel<32768>, grid, block, 0, st, p);
   if (p.fp8) launch_evict_moves<true>(p, st);
   else launch_evict_moves<false>(p, st);
   return hipGetLastError();
