@@ -149,7 +149,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
   const int nseg = (nc + SEG - 1) / SEG;
   constexpr int U = 4;
   auto load = [&](int seg) {  // (a thread's own keys: no barrier is needed to count them)
-    for (int j0 = tid; j0 < min(SEG, nc - seg * SEG); j0 += 2 * U * kSelThreads) {
+    const int whole = (min(SEG, nc - seg * SEG) + kWave - 1) / kWave * kWave;  // the last chunk's end too
+    for (int j0 = tid; j0 < whole; j0 += 2 * U * kSelThreads) {
       float v[2 * U];
 #pragma unroll
       for (int u = 0; u < 2 * U; ++u) v[u] = w[min(seg * SEG + j0 + u * kSelThreads, nc - 1)];
