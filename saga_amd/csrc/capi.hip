@@ -1745,7 +1745,7 @@ int saga_kv_fp8_read(const saga_kv_fp8* cache, const int32_t* pos, const int32_t
     return fail(SAGA_ERR_INVALID, "k and v: shapes must be [N, n_k, d] and [N, n_v, d]");
   if (k->stride[2] != 1 || v->stride[2] != 1) return fail(SAGA_ERR_INVALID, "innermost strides must be 1");
   if (!batch && N > p.kv.B) return fail(SAGA_ERR_INVALID, "without batch indices N must be <= B");
-  if (N * (p.kv.n_k + p.kv.n_v) * (d / 8) >= (1LL << 32) - 256) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  if (N * (p.kv.n_k + p.kv.n_v) * (d / 16) >= (1LL << 32) - 256) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
   p.pos = pos;
   p.batch = batch;
   p.k = k->data;

@@ -73,9 +73,10 @@ __device__ __forceinline__ float fp8_size(float x) { return fabsf(x) < __builtin
 __device__ __forceinline__ float odd_float(double v) {
   const float f = static_cast<float>(v);
   const double d = static_cast<double>(f);
-  const uint32_t u = __float_as_uint(f);
-  if (d == v || (u & 1u) || !(fabs(v) < 3e38)) return f;
-  return __uint_as_float(fabs(d) > fabs(v) ? u - 1 : u + 1);
+  uint32_t u = __float_as_uint(f);
+  u -= fabs(d) > fabs(v) ? 1u : 0u;  // towards zero
+  u |= d != v ? 1u : 0u;
+  return __uint_as_float(u);
 }
 
 }  // namespace saga
