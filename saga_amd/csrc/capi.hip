@@ -1603,7 +1603,7 @@ WeightsParams make_weights(const saga_tensor* w, int32_t add, const int32_t* kv_
 
 // Byte offsets of an eviction's workspace.
 struct EvictLayout {
-  int64_t movers, held, stage, stage_s, total;
+  int64_t gap, gap_at, movers, stage, stage_s, stage_w, total;
 };
 EvictLayout evict_layout(int64_t B, int64_t G, int64_t keep, int64_t recent, int64_t heads, int64_t row_bytes, bool in_place) {
   EvictLayout o{};
@@ -1613,11 +1613,13 @@ EvictLayout evict_layout(int64_t B, int64_t G, int64_t keep, int64_t recent, int
     off = align256(off + bytes);
     return at;
   };
+  const int64_t chunks = (keep + 63) / 64, staged = in_place ? std::min(keep, recent + 127) : 0;
+  o.gap = take(B * G * chunks * 8);
+  o.gap_at = take(B * G * chunks * 4);
   o.movers = take(B * G * keep * 4);
-  o.held = take(B * G * keep * 4);
-  const int64_t staged = in_place ? B * heads * std::min(keep, recent + 127) : 0;
-  o.stage = take(staged * row_bytes);
-  o.stage_s = take(staged * 4);
+  o.stage = take(B * heads * staged * row_bytes);
+  o.stage_s = take(B * heads * staged * 4);
+  o.stage_w = take(B * G * staged * 4);
   o.total = off;
   return o;
 }
@@ -1636,7 +1638,7 @@ int evict_run(EvictParams& p, const saga_tensor* weights, const int32_t* kv_len,
   if (out && weights_out->shape[1] != G) return fail(SAGA_ERR_INVALID, "weights_out: groups differ from weights");
   const int64_t S = 1LL << p.shift, nblk = (keep + S - 1) / S;
   // (a launch holds less than 2^32 threads)
-  if (B > (1LL << 22) / G - 1 || B * heads > ((1LL << 24) - 1) / nblk || B * G * keep > (1LL << 40))
+  if (B > (1LL << 22) / G - 1 || B * (heads + G) > ((1LL << 24) - 1) / (nblk + 1) || B * G * keep > (1LL << 40))
     return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
   const EvictLayout lay = evict_layout(B, G, keep, recent, heads, row_bytes, !out);
   if (!workspace || workspace_bytes < static_cast<size_t>(lay.total))
@@ -1650,8 +1652,10 @@ int evict_run(EvictParams& p, const saga_tensor* weights, const int32_t* kv_len,
   p.wo_sb = wo->stride[0], p.wo_sg = wo->stride[1], p.wo_len = wo->shape[2];
   p.kv_len = kv_len;
   p.kept = kept;
+  p.gap = reinterpret_cast<uint64_t*>(ws + lay.gap);
+  p.gap_at = reinterpret_cast<int32_t*>(ws + lay.gap_at);
   p.movers = reinterpret_cast<int32_t*>(ws + lay.movers);
-  p.held_w = reinterpret_cast<float*>(ws + lay.held);
+  p.stage_w = reinterpret_cast<float*>(ws + lay.stage_w);
   p.B = static_cast<int32_t>(B);
   p.G = static_cast<int32_t>(G);
   p.Lmax = static_cast<int32_t>(L);

@@ -118,13 +118,13 @@ constexpr int kSelWaves = kSelThreads / kWave;
 
 template <int SEG>
 struct SelShared {
-  uint32_t key[SEG];  // ranking keys; then, of a row of one segment, the positions that move
+  uint32_t key[SEG];  // ranking keys
   int hist[2048];
   int cnt[kSelWaves];
   int sel_bin, sel_above, sel_cnt;
-  int sums[3][kSelWaves];
-  unsigned long long a[SEG / kWave], b[SEG / kWave];  // per chunk: masks of keys above T and equal to it, then of
-  int a0[SEG / kWave], b0[SEG / kWave];               // those that move and of the gaps, and their first ones' ranks
+  int sums[4][kSelWaves];
+  uint32_t near[SEG / 16];                                // keys of the H-th largest's bin
+  unsigned long long a[SEG / kWave], b[SEG / kWave];      // per chunk: masks of larger and of equal keys
 };
 
 // A weight as what it is ranked by: any NaN above all numbers, -0 as 0; never 0, which stands for no position.
@@ -146,46 +146,49 @@ __device__ __forceinline__ unsigned long long bits_below(int end, int p0) {
 
 // One block per (batch row, group), a segment of SEG positions' ranking keys in LDS (a row of one
 // segment is read once, longer ones for every pass).  The H-th largest key by radix (11, 11, 10
-// bits), equal ones by position.  What is large of a chunk of 64 positions is then one 64-bit
-// mask, and thread c counts chunk c: every prefix of the selection is one scan of the block, and a
-// wave places its chunks' positions with one count each.
+// bits), equal ones by position: the first digits are counted as the row is read; the other two
+// over the few keys that share the H-th's, if they are few and the row is one segment, else
+// over all.  What is large of a chunk of 64 positions is one 64-bit mask, and thread c counts
+// chunk c: every prefix of the selection is one scan of the block.  The result is, per chunk of
+// places below H, the mask of its gaps and the first one's rank, and the positions that move there
+// in order; what to do with them is the moving blocks' work, of which there are many.
+// One CU's work, about 4 cycles an instruction and wave: 8 x 32769 positions 82 us with keys in
+// registers and code unrolled over them, 36 with three digits over all keys.
 template <int SEG>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p) {
   __shared__ SelShared<SEG> sh;
-  constexpr int CH = SEG / kWave;
+  constexpr int CH = SEG / kWave, NEAR = SEG / 16;
   static_assert(CH <= kSelThreads && SEG % kSelThreads == 0, "a thread per chunk");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bi = blockIdx.x / p.G, gi = blockIdx.x - bi * p.G;
   const int n = min(max(p.kv_len[bi], 0), p.Lmax);
+  if (n <= p.keep) return;
   const float* w = p.w + bi * p.w_sb + gi * p.w_sg;
-  float* wo = p.w_out + bi * p.wo_sb + gi * p.wo_sg;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * p.keep;
-  int32_t *kept = p.kept + row, *movers = p.movers + row;
-  const int wlen = static_cast<int>(p.wo_len);
-  if (n <= p.keep) {
-    for (int j = tid; j < p.keep; j += kSelThreads) {
-      kept[j] = j < n ? j : -1;
-      if (!p.in_place) wo[j] = j < n ? w[j] : 0.f;
-    }
-    for (int j = (p.in_place ? n : p.keep) + tid; j < wlen; j += kSelThreads) wo[j] = 0.f;
-    return;
-  }
+  const int64_t row = blockIdx.x;
   const int H = p.keep - p.recent, nc = n - p.recent;  // candidates: [0, nc), nc > H
   const int nseg = (nc + SEG - 1) / SEG;
-  constexpr int U = 4;
-  auto load = [&](int seg) {  // (a thread's own keys: no barrier is needed to count them)
-    const int whole = (min(SEG, nc - seg * SEG) + kWave - 1) / kWave * kWave;  // the last chunk's end too
-    for (int j0 = tid; j0 < whole; j0 += 2 * U * kSelThreads) {
-      float v[2 * U];
+  constexpr uint32_t kZero = 0x80000000u;
+  // f(key) of this thread's positions of a segment as they are read into LDS (a wave's chunks are its own:
+  // it reads them without a barrier); 0 behind nc, to the last chunk's end
+  auto load = [&](int seg, auto f) {
+    constexpr int U = 8;
+    const int whole = (min(SEG, nc - seg * SEG) + kWave - 1) / kWave * kWave;
+    for (int j0 = tid; j0 < whole; j0 += U * kSelThreads) {
+      float v[U];
 #pragma unroll
-      for (int u = 0; u < 2 * U; ++u) v[u] = w[min(seg * SEG + j0 + u * kSelThreads, nc - 1)];
+      for (int u = 0; u < U; ++u) v[u] = w[min(seg * SEG + j0 + u * kSelThreads, nc - 1)];
 #pragma unroll
-      for (int u = 0; u < 2 * U; ++u)
-        if (j0 + u * kSelThreads < SEG) sh.key[j0 + u * kSelThreads] = seg * SEG + j0 + u * kSelThreads < nc ? rank_key(v[u]) : 0u;
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * kSelThreads;
+        const uint32_t key = seg * SEG + j < nc ? rank_key(v[u]) : 0u;
+        if (j < SEG) sh.key[j] = key;
+        f(key);
+      }
     }
   };
-  // f(chunk, key) of the segment's chunks, wave by wave; keys are 0 behind nc
+  // f(chunk, key) of the segment's chunks, wave by wave
   auto chunks = [&](int seg, auto f) {
+    constexpr int U = 4;
     const int nch = (min(SEG, nc - seg * SEG) + kWave - 1) / kWave;
     for (int c0 = wave; c0 < nch; c0 += U * kSelWaves) {
       uint32_t key[U];
@@ -195,200 +198,224 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
       for (int u = 0; u < U; ++u) f(c0 + u * kSelWaves, key[u]);
     }
   };
-  load(0);
+  // The masks of keys above `top` and of keys in [from, top] of a segment's chunks: chunk c's in thread c
+  unsigned long long gt = 0, eq = 0;
+  auto masks = [&](int seg, uint32_t from, uint32_t top) {
+    int k = 0;
+    unsigned long long ga = 0, ea = 0;  // lane k: chunk k of the wave
+    chunks(seg, [&](int c, uint32_t key) {
+      const unsigned long long g = __ballot(key > top), e = __ballot(key >= from) & ~g;
+      ga = lane == k ? g : ga;
+      ea = lane == k ? e : ea;
+      ++k;
+    });
+    const int c = lane * kSelWaves + wave;
+    if (lane < CH / kSelWaves) sh.a[c] = ga, sh.b[c] = ea;
+    lds_sync();
+    gt = tid < CH ? sh.a[tid] : 0ull;
+    eq = tid < CH ? sh.b[tid] : 0ull;
+  };
+  auto wave_part = [&](int v, int which) {  // v of the wave's threads before
+    const int incl = wave_incl_scan(v, lane);
+    if (lane == kWave - 1) sh.sums[which][wave] = incl;
+    return incl - v;
+  };
+  auto block_part = [&](int which, int& all) {  // of the waves before, and of all
+    int before = 0;
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < kSelWaves; ++i) {
+      const int s = sh.sums[which][i];
+      before += i < wave ? s : 0;
+      all += s;
+    }
+    return before;
+  };
+
   uint32_t T = 0xffffffffu;  // the H-th largest key
   int need = 0;              // of those equal to it, the first `need` stay
+  bool few = false;          // gt and eq hold the row's masks already
+  for (int i = tid; i < 2048; i += kSelThreads) sh.hist[i] = 0;
+  lds_sync();
+  {
+    int zeros = 0;  // weights of 0 may be many: counted by the wave
+    for (int seg = 0; seg < nseg; ++seg) {
+      load(seg, [&](uint32_t key) {
+        zeros += __popcll(__ballot(key == kZero));
+        if (key << 1) atomicAdd(&sh.hist[key >> 21], 1);
+      });
+    }
+    if (zeros && lane == 0) atomicAdd(&sh.hist[kZero >> 21], zeros);
+  }
   if (H > 0) {
-    constexpr uint32_t kZero = 0x80000000u;
     need = H;
-    uint32_t prefix = 0;
+    lds_sync();
+    int bin, above, count;
+    hist_pick<kSelThreads>(sh, 2048, need, bin, above, count);
+    uint32_t prefix = static_cast<uint32_t>(bin) << 21;
+    need -= above;
+    few = nseg == 1 && count <= NEAR;
+    int listed = 0;
+    if (few) {
+      masks(0, prefix, prefix | 0x1fffffu);
+      const int at = wave_part(__popcll(eq), 0);
+      lds_sync();
+      int k = at + block_part(0, listed);
+      for (unsigned long long m = eq; m; m &= m - 1) sh.near[k++] = sh.key[tid * kWave + __builtin_ctzll(m)];
+    }
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, nb = pass == 2 ? 1024 : 2048;
-      const uint32_t hmask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
+    for (int pass = 1; pass < 3; ++pass) {
+      const int shift = pass == 1 ? 10 : 0, nb = pass == 1 ? 2048 : 1024;
+      const uint32_t hmask = pass == 1 ? 0xffe00000u : 0xfffffc00u;
       for (int i = tid; i < 2048; i += kSelThreads) sh.hist[i] = 0;
       lds_sync();
-      int zeros = 0;  // weights of 0 may be many: counted by the wave (what is no position counts in the lowest bin)
-      for (int seg = 0; seg < nseg; ++seg) {
-        if (seg || (pass && nseg > 1)) load(seg);
-        chunks(seg, [&](int c, uint32_t key) {
-          const bool zero = key == kZero;
-          zeros += __popcll(__ballot(zero));
-          if ((((key ^ prefix) & hmask) | (zero ? 1u : 0u)) == 0u) atomicAdd(&sh.hist[(key >> shift) & (nb - 1)], 1);
-        });
+      if (few) {
+        for (int i = tid; i < listed; i += kSelThreads) {
+          const uint32_t key = sh.near[i];
+          if (((key ^ prefix) & hmask) == 0u) atomicAdd(&sh.hist[(key >> shift) & (nb - 1)], 1);
+        }
+      } else {
+        int zeros = 0;
+        for (int seg = 0; seg < nseg; ++seg) {
+          if (nseg > 1) load(seg, [](uint32_t) {});
+          chunks(seg, [&](int c, uint32_t key) {
+            const bool zero = key == kZero;
+            zeros += __popcll(__ballot(zero));
+            if ((((key ^ prefix) & hmask) | (zero ? 1u : 0u)) == 0u) atomicAdd(&sh.hist[(key >> shift) & (nb - 1)], 1);
+          });
+        }
+        if (((kZero ^ prefix) & hmask) == 0 && lane == 0 && zeros) atomicAdd(&sh.hist[(kZero >> shift) & (nb - 1)], zeros);
       }
-      if (((kZero ^ prefix) & hmask) == 0 && lane == 0 && zeros) atomicAdd(&sh.hist[(kZero >> shift) & (nb - 1)], zeros);
       lds_sync();
-      int bin, above, count;
       hist_pick<kSelThreads>(sh, nb, need, bin, above, count);
       prefix |= static_cast<uint32_t>(bin) << shift;
       need -= above;
     }
     T = prefix;
-  }
-  int eq_base = 0, mov_base = 0, gap_base = 0;  // of the segments before
-  // The masks and ranks of a segment's chunks
-  auto masks = [&](int seg) {
-    chunks(seg, [&](int c, uint32_t key) {
-      const unsigned long long g = __ballot(key > T), e = __ballot(key == T);
-      if (lane == 0 && c < CH) sh.a[c] = g, sh.b[c] = e;
-    });
-    lds_sync();
-    const int p0 = (seg * CH + tid) * kWave;
-    const bool mine = tid < CH && p0 < nc;
-    const unsigned long long gt = mine ? sh.a[tid] : 0ull, eq = mine ? sh.b[tid] : 0ull;
-    auto scan = [&](int v, int which, int& all) {  // v of the threads before, and of all
-      const int incl = wave_incl_scan(v, lane);
-      if (lane == kWave - 1) sh.sums[which][wave] = incl;
-      lds_sync();
-      int before = incl - v;
-      all = 0;
-#pragma unroll
-      for (int i = 0; i < kSelWaves; ++i) {
-        const int s = sh.sums[which][i];
-        before += i < wave ? s : 0;
-        all += s;
+    if (few) {  // of the H-th's bin: above T, and T
+      unsigned long long same = 0;
+      for (unsigned long long m = eq; m; m &= m - 1) {
+        const uint32_t key = sh.key[tid * kWave + __builtin_ctzll(m)];
+        if (key > T) gt |= m & -m;
+        if (key == T) same |= m & -m;
       }
-      return before;
-    };
-    int all;
-    const int ne = __popcll(eq), before = eq_base + scan(ne, 0, all);
-    eq_base += all;
-    const unsigned long long large = gt | low_bits(eq, min(max(need - before, 0), ne)), low = bits_below(H, p0);
-    const unsigned long long mov = large & ~low, gap = mine ? ~large & low : 0ull;
-    const int mov_at = mov_base + scan(__popcll(mov), 1, all);
-    mov_base += all;
-    const int gap_at = gap_base + scan(__popcll(gap), 2, all);
-    gap_base += all;
-    if (mine) sh.a[tid] = mov, sh.b[tid] = gap, sh.a0[tid] = mov_at, sh.b0[tid] = gap_at;
-    lds_sync();
-  };
-  const unsigned long long below = lanes_below(lane);
+      eq = same;
+    }
+  }
+  const int nplace = (p.keep + kWave - 1) / kWave;
+  int32_t* movers = p.movers + row * p.keep;
+  int eq_base = 0, moved = 0, opened = 0;  // of the segments before
   for (int seg = 0; seg < nseg; ++seg) {
     if (nseg > 1) {
       __syncthreads();  // (the segment before has been read)
-      load(seg);
-      lds_sync();
+      load(seg, [](uint32_t) {});
     }
-    masks(seg);
-    const int nch = (min(SEG, nc - seg * SEG) + kWave - 1) / kWave, c0 = max(H - seg * SEG, 0) / kWave;  // (none wholly below H)
-    for (int c = c0 + wave; c < nch; c += kSelWaves) {
-      const unsigned long long m = sh.a[c];
-      const int at = sh.a0[c] + __popcll(m & below);
-      if ((m >> lane) & 1) (nseg > 1 ? reinterpret_cast<uint32_t*>(movers) : sh.key)[at] = seg * SEG + c * kWave + lane;
-    }
-  }
-  __syncthreads();
-  // Places below H.  Positions read there are at or past H or stay, so in place nothing is
-  // overwritten before it is read
-  eq_base = mov_base = gap_base = 0;
-  for (int seg = 0; seg * SEG < H; ++seg) {
-    if (nseg > 1) {
-      __syncthreads();
-      load(seg);
-      lds_sync();
-      masks(seg);
-    }
-    const int nch = (min(SEG, H - seg * SEG) + kWave - 1) / kWave;
-    for (int c0 = wave; c0 < nch; c0 += U * kSelWaves) {
-      int from[U];
-      float v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = min(c0 + u * kSelWaves, nch - 1);
-        const unsigned long long g = sh.b[c];
-        from[u] = seg * SEG + c * kWave + lane;
-        if ((g >> lane) & 1) {
-          const int at = sh.b0[c] + __popcll(g & below);
-          from[u] = nseg > 1 ? movers[at] : static_cast<int>(sh.key[at]);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = w[min(from[u], nc - 1)];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = c0 + u * kSelWaves, pos = seg * SEG + c * kWave + lane;
-        if (c < nch && pos < H) {
-          kept[pos] = from[u];
-          if (!p.in_place || from[u] != pos) wo[pos] = v[u];
-        }
-      }
+    if (!few) masks(seg, T, T);
+    const int chunk = seg * CH + tid, p0 = chunk * kWave, ne = __popcll(eq), eq_at = wave_part(ne, 1);
+    lds_sync();
+    int all;
+    const int before = eq_base + eq_at + block_part(1, all);
+    eq_base += all;
+    const unsigned long long large = gt | low_bits(eq, min(max(need - before, 0), ne)), low = bits_below(H, p0);
+    const unsigned long long mov = large & ~low, gap = tid < CH ? ~large & low : 0ull;
+    const int mov_at = wave_part(__popcll(mov), 2), gap_at = wave_part(__popcll(gap), 3);
+    lds_sync();
+    int k = moved + mov_at + block_part(2, all);
+    moved += all;
+    for (unsigned long long m = mov; m; m &= m - 1) movers[k++] = p0 + __builtin_ctzll(m);
+    k = opened + gap_at + block_part(3, all);
+    opened += all;
+    if (tid < CH && chunk < nplace) {
+      p.gap[row * nplace + chunk] = gap;
+      p.gap_at[row * nplace + chunk] = k;
     }
   }
-  // the last `recent`; in place through the workspace, for they may overlap their places
-  float* held = p.held_w + row;
-  for (int j = tid; j < p.recent; j += kSelThreads) {
-    kept[H + j] = nc + j;
-    (p.in_place ? held : wo + H)[j] = w[nc + j];
-  }
-  if (p.in_place) {
-    __threadfence_block();
-    __syncthreads();
-    for (int j = tid; j < p.recent; j += kSelThreads) wo[H + j] = held[j];
-  }
-  for (int j = p.keep + tid; j < wlen; j += kSelThreads) wo[j] = 0.f;
 }
 
 // Rows to their places: a block of threads per (batch row, head, S positions of the result, S a block of
-// the cache's scales).  FP8: the block's scale is the largest of its rows' and a row from
-// under a smaller one is rounded to it.  PHASE 0: into other tensors.  In place, two launches: 1: the blocks
-// below staged0, whose rows come from at or above it or stay, and the rows of the end into the
-// stage; 2: from the stage to the end.
+// the cache's scales); the heads behind keys and values are the groups' weights, whose blocks write
+// `kept` too.  FP8: the block's scale is the largest of its rows' and a row from under a smaller
+// one is rounded to it.  PHASE 0: into other tensors.  In place, two launches: 1: the blocks below
+// staged0, whose rows come from at or above it or stay, and the rows of the end into the stage;
+// 2: from the stage to the end, and zeros for the weights behind.
 template <int PHASE, bool FP8>
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictParams p) {
   __shared__ int from_sh[128];
   __shared__ float scale_sh[128], red[4];
   const int tid = threadIdx.x, S = 1 << p.shift;
   const int nblk = (p.keep + S - 1) >> p.shift, staged_blk = p.staged0 >> p.shift;
-  const int blocks = PHASE == 2 ? nblk - staged_blk : nblk;
-  const int heads = p.rows[0].heads + p.rows[1].heads;
+  const int blocks = nblk + (PHASE == 1 ? 0 : 1) - (PHASE == 2 ? staged_blk : 0);  // (a last one for the weights behind)
+  const int kv_heads = p.rows[0].heads + p.rows[1].heads, heads = kv_heads + p.G;
   int64_t id = blockIdx.x;
   const int blk = static_cast<int>(id % blocks) + (PHASE == 2 ? staged_blk : 0);
   id /= blocks;
   const int hh = static_cast<int>(id % heads), bi = static_cast<int>(id / heads);
-  const bool is_v = hh >= p.rows[0].heads;
+  const bool is_v = hh >= p.rows[0].heads, is_w = hh >= kv_heads;
   const EvictRows& r = p.rows[is_v ? 1 : 0];
-  const int h = hh - (is_v ? p.rows[0].heads : 0), gi = h / (r.heads / p.G);
-  const int32_t* kept = p.kept + (static_cast<int64_t>(bi) * p.G + gi) * p.keep;
+  const int h = is_w ? hh - kv_heads : hh - (is_v ? p.rows[0].heads : 0), gi = is_w ? h : h / (r.heads / p.G);
+  const int64_t group = static_cast<int64_t>(bi) * p.G + gi;
+  const int n = min(max(p.kv_len[bi], 0), p.Lmax), H = p.keep - p.recent;
   const int j0 = blk << p.shift, count = min(S, p.keep - j0);
+  if (blk == nblk) {  // (weights only)
+    float* wo = p.w_out + bi * p.wo_sb + gi * p.wo_sg;
+    if (is_w)
+      for (int64_t j = p.keep + tid; j < p.wo_len; j += 256) wo[j] = 0.f;
+    return;
+  }
   const bool stage = PHASE == 1 && blk >= staged_blk;
-  const int64_t nstage = p.keep - p.staged0, srow = (static_cast<int64_t>(bi) * r.heads + h) * nstage - p.staged0;  // + j
+  int from = -1;
+  if (tid < count) {
+    const int j = j0 + tid;
+    if (n <= p.keep) from = j < n ? j : -1;
+    else if (j >= H) from = n - p.keep + j;
+    else {
+      const int64_t at = group * ((p.keep + kWave - 1) / kWave) + j / kWave;
+      const unsigned long long gap = p.gap[at];
+      const int rank = p.gap_at[at] + __popcll(gap & lanes_below(j & 63));
+      from = (gap >> (j & 63)) & 1 ? p.movers[group * p.keep + rank] : j;
+    }
+    from_sh[tid] = from;
+  }
+  const int64_t nstage = p.keep - p.staged0;
+  if (is_w) {
+    if (tid >= count) return;
+    const int j = j0 + tid;
+    float* held = p.stage_w + group * nstage - p.staged0;
+    if (PHASE != 2) p.kept[group * p.keep + j] = from;
+    const float v = from < 0 ? 0.f : PHASE == 2 ? held[j] : p.w[bi * p.w_sb + gi * p.w_sg + from];
+    if (stage) held[j] = v;
+    else if (j < p.wo_len && (PHASE != 1 || from != j)) p.w_out[bi * p.wo_sb + gi * p.wo_sg + j] = v;
+    return;
+  }
+  const int64_t srow = (static_cast<int64_t>(bi) * r.heads + h) * nstage - p.staged0;  // + j
   const char* src = r.src + bi * r.s_sb + h * r.s_sh;
   char* dst = r.dst + bi * r.d_sb + h * r.d_sh;
   const float* ss = FP8 ? r.ss + bi * r.ss_sb + h * r.ss_sh : nullptr;
   float* ds = FP8 ? r.ds + bi * r.ds_sb + h * r.ds_sh : nullptr;
-
   float mine = 0.f;
-  int any = 0;
-  if (tid < count) {
-    const int from = kept[j0 + tid];
-    from_sh[tid] = from;
-    any = from >= 0;
-    if (FP8 && from >= 0) {
-      mine = PHASE == 2 ? r.stage_s[srow + j0 + tid] : ss[from >> p.shift];
-      scale_sh[tid] = mine;
-    }
+  if (FP8 && from >= 0) {
+    mine = PHASE == 2 ? r.stage_s[srow + j0 + tid] : ss[from >> p.shift];
+    scale_sh[tid] = mine;
   }
   float top = 0.f, own = 0.f;
   if constexpr (FP8) {
     if (PHASE == 1 && !stage) own = ss[blk];  // (before the store below: the barrier orders them)
     top = block_max<4>(mine, red);
   }
-  const bool live = __syncthreads_or(any);
-  if (!live) return;
+  if (!__syncthreads_or(from >= 0)) return;
   const float inv = FP8 ? fp8_inverse(top) : 0.f;
   const int pieces = r.pieces;
   for (int e = tid; e < count * pieces; e += 256) {
-    const int j = e / pieces, c = e - j * pieces, from = from_sh[j];
-    if (from < 0) continue;
+    const int j = e / pieces, c = e - j * pieces, at = from_sh[j];
+    if (at < 0) continue;
     if (stage) {
-      *reinterpret_cast<u32x4*>(r.stage + ((srow + j0 + j) * pieces + c) * 16) = ld16(src + from * r.s_sl + 16 * c);
+      *reinterpret_cast<u32x4*>(r.stage + ((srow + j0 + j) * pieces + c) * 16) = ld16(src + at * r.s_sl + 16 * c);
       if (FP8 && c == 0) r.stage_s[srow + j0 + j] = scale_sh[j];
       continue;
     }
     const float s = FP8 ? scale_sh[j] : 0.f;
-    if (PHASE == 1 && from == j0 + j && (!FP8 || s == top)) continue;
-    u32x4 v = ld16(PHASE == 2 ? r.stage + ((srow + j0 + j) * pieces + c) * 16 : src + from * r.s_sl + 16 * c);
+    if (PHASE == 1 && at == j0 + j && (!FP8 || s == top)) continue;
+    u32x4 v = ld16(PHASE == 2 ? r.stage + ((srow + j0 + j) * pieces + c) * 16 : src + at * r.s_sl + 16 * c);
     if (FP8 && s != top) v = fp8_rescaled(v, s * inv);
     *reinterpret_cast<u32x4*>(dst + (j0 + j) * r.d_sl + 16 * c) = v;
   }
@@ -398,15 +425,14 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictParams p) {
 template <bool FP8>
 static void launch_evict_moves(const EvictParams& p, hipStream_t st) {
   const int64_t S = 1LL << p.shift, nblk = (p.keep + S - 1) / S;
-  const int64_t rows = static_cast<int64_t>(p.B) * (p.rows[0].heads + p.rows[1].heads);
-  const dim3 grid(static_cast<unsigned>(rows * nblk));
+  const int64_t rows = static_cast<int64_t>(p.B) * (p.rows[0].heads + p.rows[1].heads + p.G);
   if (!p.in_place) {
-    hipLaunchKernelGGL((evict_move_kernel<0, FP8>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((evict_move_kernel<0, FP8>), dim3(static_cast<unsigned>(rows * (nblk + 1))), dim3(256), 0, st, p);
     return;
   }
-  hipLaunchKernelGGL((evict_move_kernel<1, FP8>), grid, dim3(256), 0, st, p);
-  const int64_t rest = nblk - (p.staged0 >> p.shift);
-  if (rest) hipLaunchKernelGGL((evict_move_kernel<2, FP8>), dim3(static_cast<unsigned>(rows * rest)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((evict_move_kernel<1, FP8>), dim3(static_cast<unsigned>(rows * nblk)), dim3(256), 0, st, p);
+  const int64_t rest = nblk + 1 - (p.staged0 >> p.shift);
+  hipLaunchKernelGGL((evict_move_kernel<2, FP8>), dim3(static_cast<unsigned>(rows * rest)), dim3(256), 0, st, p);
 }
 
 hipError_t launch_evict(const EvictParams& p, hipStream_t st) {
