@@ -1636,7 +1636,7 @@ int evict_run(EvictParams& p, const saga_tensor* weights, const int32_t* kv_len,
   const int64_t G = weights->shape[1], heads = k_h + v_h;
   if (out && (rc = check_weights(weights_out, "weights_out", B, k_h, v_h, keep, true))) return rc;
   if (out && weights_out->shape[1] != G) return fail(SAGA_ERR_INVALID, "weights_out: groups differ from weights");
-  const int64_t S = 1LL << p.shift, nblk = (keep + S - 1) / S;
+  const int64_t S = 1LL << p.shift, nblk = (keep + 127) / 128;
   // (a launch holds less than 2^32 threads)
   if (B > (1LL << 22) / G - 1 || B * (heads + G) > ((1LL << 24) - 1) / (nblk + 1) || B * G * keep > (1LL << 40))
     return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");

@@ -332,115 +332,142 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
   }
 }
 
-// Rows to their places: a block of threads per (batch row, head, S positions of the result, S a block of
-// the cache's scales); the heads behind keys and values are the groups' weights, whose blocks write
-// `kept` too.  FP8: the block's scale is the largest of its rows' and a row from under a smaller
-// one is rounded to it.  PHASE 0: into other tensors.  In place, two launches: 1: the blocks below
-// staged0, whose rows come from at or above it or stay, and the rows of the end into the stage;
-// 2: from the stage to the end, and zeros for the weights behind.
-template <int PHASE, bool FP8>
+// Rows to their places: a block of threads per (batch row, head, 128 places); the heads behind keys and
+// values are the groups' weights, whose blocks write `kept` too.  FP8: a block of S places takes
+// the largest of its rows' scales and a row from under a smaller one is rounded to it.  PHASE 0:
+// into other tensors.  In place, two launches: 1: the places below staged0 (a multiple of S), whose
+// rows come from at or above it or stay, and the rows of the end into the stage; 2: from the stage to
+// the end, and zeros for the weights behind.  PIECES: 16 bytes each of a row; a thread's are all in
+// flight while the scales are compared.
+// Bound by the rows, read once and written once: 8 x 16384 rows of 3 heads of 256 bytes (201 MB)
+// 42 us, 4.8 TB/s.
+constexpr int kMoveRows = 128;
+
+template <int PHASE, bool FP8, int PIECES>
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictParams p) {
-  __shared__ int from_sh[128];
-  __shared__ float scale_sh[128], red[4];
-  const int tid = threadIdx.x, S = 1 << p.shift;
-  const int nblk = (p.keep + S - 1) >> p.shift, staged_blk = p.staged0 >> p.shift;
-  const int blocks = nblk + (PHASE == 1 ? 0 : 1) - (PHASE == 2 ? staged_blk : 0);  // (a last one for the weights behind)
+  constexpr int PT = kMoveRows * PIECES / 256, ROWS = 256 / PIECES;  // pieces of a thread, rows side by side
+  __shared__ int from_sh[kMoveRows];
+  __shared__ float scale_sh[kMoveRows], top_sh[kMoveRows], wave_top[2];
+  const int tid = threadIdx.x;
+  const int nblk = (p.keep + kMoveRows - 1) / kMoveRows, first = PHASE == 2 ? p.staged0 / kMoveRows : 0;
+  const int blocks = nblk - first + (PHASE == 1 ? 0 : 1);  // (a last one for the weights behind)
   const int kv_heads = p.rows[0].heads + p.rows[1].heads, heads = kv_heads + p.G;
-  int64_t id = blockIdx.x;
-  const int blk = static_cast<int>(id % blocks) + (PHASE == 2 ? staged_blk : 0);
+  int id = blockIdx.x;
+  const int blk = id % blocks + first;
   id /= blocks;
-  const int hh = static_cast<int>(id % heads), bi = static_cast<int>(id / heads);
+  const int hh = id % heads, bi = id / heads;
   const bool is_v = hh >= p.rows[0].heads, is_w = hh >= kv_heads;
   const EvictRows& r = p.rows[is_v ? 1 : 0];
   const int h = is_w ? hh - kv_heads : hh - (is_v ? p.rows[0].heads : 0), gi = is_w ? h : h / (r.heads / p.G);
   const int64_t group = static_cast<int64_t>(bi) * p.G + gi;
-  const int n = min(max(p.kv_len[bi], 0), p.Lmax), H = p.keep - p.recent;
-  const int j0 = blk << p.shift, count = min(S, p.keep - j0);
+  const int j0 = blk * kMoveRows, H = p.keep - p.recent;
   if (blk == nblk) {  // (weights only)
     float* wo = p.w_out + bi * p.wo_sb + gi * p.wo_sg;
     if (is_w)
       for (int64_t j = p.keep + tid; j < p.wo_len; j += 256) wo[j] = 0.f;
     return;
   }
-  const bool stage = PHASE == 1 && blk >= staged_blk;
+  const int64_t nstage = p.keep - p.staged0;
+  const int64_t srow = (static_cast<int64_t>(bi) * r.heads + h) * nstage - p.staged0;  // + place
+  const int mine = j0 + tid;  // the place that this thread looks up
   int from = -1;
-  if (tid < count) {
-    const int j = j0 + tid;
-    if (n <= p.keep) from = j < n ? j : -1;
-    else if (j >= H) from = n - p.keep + j;
-    else {
-      const int64_t at = group * ((p.keep + kWave - 1) / kWave) + j / kWave;
-      const unsigned long long gap = p.gap[at];
-      const int rank = p.gap_at[at] + __popcll(gap & lanes_below(j & 63));
-      from = (gap >> (j & 63)) & 1 ? p.movers[group * p.keep + rank] : j;
+  float scale = 0.f;
+  if (tid < kMoveRows) {
+    const int64_t at = group * ((p.keep + kWave - 1) / kWave) + min(mine, p.keep - 1) / kWave;
+    const int kv = p.kv_len[bi];
+    const unsigned long long gap = p.gap[at];  // (nothing is there where nothing is evicted)
+    const int rank = p.gap_at[at] + __popcll(gap & lanes_below(mine & 63));
+    const int n = min(max(kv, 0), p.Lmax);
+    if (mine < p.keep && (PHASE != 2 || mine >= p.staged0)) {
+      if (n <= p.keep) from = mine < n ? mine : -1;
+      else if (mine >= H) from = n - p.keep + mine;
+      else from = (gap >> (mine & 63)) & 1 ? p.movers[group * p.keep + rank] : mine;
     }
     from_sh[tid] = from;
+    if (FP8 && from >= 0 && !is_w) {
+      const float* ss = r.ss + bi * r.ss_sb + h * r.ss_sh;
+      scale = PHASE == 2 ? r.stage_s[srow + mine] : ss[from >> p.shift];
+    }
   }
-  const int64_t nstage = p.keep - p.staged0;
   if (is_w) {
-    if (tid >= count) return;
-    const int j = j0 + tid;
+    if (tid >= kMoveRows || mine >= p.keep || (PHASE == 2 && mine < p.staged0)) return;
     float* held = p.stage_w + group * nstage - p.staged0;
-    if (PHASE != 2) p.kept[group * p.keep + j] = from;
-    const float v = from < 0 ? 0.f : PHASE == 2 ? held[j] : p.w[bi * p.w_sb + gi * p.w_sg + from];
-    if (stage) held[j] = v;
-    else if (j < p.wo_len && (PHASE != 1 || from != j)) p.w_out[bi * p.wo_sb + gi * p.wo_sg + j] = v;
+    if (PHASE != 2) p.kept[group * p.keep + mine] = from;
+    const float v = from < 0 ? 0.f : PHASE == 2 ? held[mine] : p.w[bi * p.w_sb + gi * p.w_sg + from];
+    if (PHASE == 1 && mine >= p.staged0) held[mine] = v;
+    else if (mine < p.wo_len && (PHASE != 1 || from != mine)) p.w_out[bi * p.wo_sb + gi * p.wo_sg + mine] = v;
     return;
   }
-  const int64_t srow = (static_cast<int64_t>(bi) * r.heads + h) * nstage - p.staged0;  // + j
+  __syncthreads();
   const char* src = r.src + bi * r.s_sb + h * r.s_sh;
   char* dst = r.dst + bi * r.d_sb + h * r.d_sh;
-  const float* ss = FP8 ? r.ss + bi * r.ss_sb + h * r.ss_sh : nullptr;
   float* ds = FP8 ? r.ds + bi * r.ds_sb + h * r.ds_sh : nullptr;
-  float mine = 0.f;
-  if (FP8 && from >= 0) {
-    mine = PHASE == 2 ? r.stage_s[srow + j0 + tid] : ss[from >> p.shift];
-    scale_sh[tid] = mine;
+  const int c = tid % PIECES, row0 = tid / PIECES;
+  u32x4 v[PT];
+#pragma unroll
+  for (int i = 0; i < PT; ++i) {  // (no branch: it would be waited for; what has no place is read from its head's first row)
+    const int row = row0 + i * ROWS, at = from_sh[row];
+    const char* a = PHASE == 2 ? (at < 0 ? src : r.stage + (srow + j0 + row) * PIECES * 16) : src + max(at, 0) * r.s_sl;
+    v[i] = ld16(a + 16 * c);
   }
-  float top = 0.f, own = 0.f;
   if constexpr (FP8) {
-    if (PHASE == 1 && !stage) own = ss[blk];  // (before the store below: the barrier orders them)
-    top = block_max<4>(mine, red);
+    const int S = 1 << p.shift;
+    float top = scale;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+    if (S > 32) top = fmaxf(top, __shfl_xor(top, 32));
+    if (tid < kMoveRows && (tid & 63) == 0) wave_top[tid >> 6] = top;
+    if (tid < kMoveRows) scale_sh[tid] = scale;
+    lds_sync();
+    if (S > 64) top = fmaxf(wave_top[0], wave_top[1]);
+    if (tid < kMoveRows) top_sh[tid] = top;
+    lds_sync();
+    // a block's scale, by its first row's thread, where any of its rows is there (rows of a block are there
+    // from its first one on); in place it is read above by this block alone
+    if (tid < kMoveRows && (mine & (S - 1)) == 0 && from >= 0 && (PHASE != 1 || mine < p.staged0)) ds[mine >> p.shift] = top;
   }
-  if (!__syncthreads_or(from >= 0)) return;
-  const float inv = FP8 ? fp8_inverse(top) : 0.f;
-  const int pieces = r.pieces;
-  for (int e = tid; e < count * pieces; e += 256) {
-    const int j = e / pieces, c = e - j * pieces, at = from_sh[j];
+#pragma unroll
+  for (int i = 0; i < PT; ++i) {
+    const int row = row0 + i * ROWS, at = from_sh[row], place = j0 + row;
     if (at < 0) continue;
-    if (stage) {
-      *reinterpret_cast<u32x4*>(r.stage + ((srow + j0 + j) * pieces + c) * 16) = ld16(src + at * r.s_sl + 16 * c);
-      if (FP8 && c == 0) r.stage_s[srow + j0 + j] = scale_sh[j];
+    if (PHASE == 1 && place >= p.staged0) {
+      *reinterpret_cast<u32x4*>(r.stage + ((srow + place) * PIECES + c) * 16) = v[i];
+      if (FP8 && c == 0) r.stage_s[srow + place] = scale_sh[row];
       continue;
     }
-    const float s = FP8 ? scale_sh[j] : 0.f;
-    if (PHASE == 1 && at == j0 + j && (!FP8 || s == top)) continue;
-    u32x4 v = ld16(PHASE == 2 ? r.stage + ((srow + j0 + j) * pieces + c) * 16 : src + at * r.s_sl + 16 * c);
-    if (FP8 && s != top) v = fp8_rescaled(v, s * inv);
-    *reinterpret_cast<u32x4*>(dst + (j0 + j) * r.d_sl + 16 * c) = v;
+    const float s = FP8 ? scale_sh[row] : 0.f, top = FP8 ? top_sh[row] : 0.f;
+    if (PHASE == 1 && at == place && s == top) continue;
+    if (FP8 && s != top) v[i] = fp8_rescaled(v[i], s * fp8_inverse(top));
+    *reinterpret_cast<u32x4*>(dst + place * r.d_sl + 16 * c) = v[i];
   }
-  if (FP8 && tid == 0 && !stage && (PHASE != 1 || top != own)) ds[blk] = top;
 }
 
-template <bool FP8>
+template <bool FP8, int PIECES>
 static void launch_evict_moves(const EvictParams& p, hipStream_t st) {
-  const int64_t S = 1LL << p.shift, nblk = (p.keep + S - 1) / S;
+  const int64_t nblk = (p.keep + kMoveRows - 1) / kMoveRows;
   const int64_t rows = static_cast<int64_t>(p.B) * (p.rows[0].heads + p.rows[1].heads + p.G);
   if (!p.in_place) {
-    hipLaunchKernelGGL((evict_move_kernel<0, FP8>), dim3(static_cast<unsigned>(rows * (nblk + 1))), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((evict_move_kernel<0, FP8, PIECES>), dim3(static_cast<unsigned>(rows * (nblk + 1))), dim3(256), 0, st, p);
     return;
   }
-  hipLaunchKernelGGL((evict_move_kernel<1, FP8>), dim3(static_cast<unsigned>(rows * nblk)), dim3(256), 0, st, p);
-  const int64_t rest = nblk + 1 - (p.staged0 >> p.shift);
-  hipLaunchKernelGGL((evict_move_kernel<2, FP8>), dim3(static_cast<unsigned>(rows * rest)), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((evict_move_kernel<1, FP8, PIECES>), dim3(static_cast<unsigned>(rows * nblk)), dim3(256), 0, st, p);
+  const int64_t rest = nblk + 1 - p.staged0 / kMoveRows;
+  hipLaunchKernelGGL((evict_move_kernel<2, FP8, PIECES>), dim3(static_cast<unsigned>(rows * rest)), dim3(256), 0, st, p);
 }
 
 hipError_t launch_evict(const EvictParams& p, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.B * p.G)), block(kSelThreads);
   if (p.Lmax <= 4096) hipLaunchKernelGGL(evict_select_kernel<4096>, grid, block, 0, st, p);
   else hipLaunchKernelGGL(evict_select_kernel<32768>, grid, block, 0, st, p);
-  if (p.fp8) launch_evict_moves<true>(p, st);
-  else launch_evict_moves<false>(p, st);
+  const int pieces = p.rows[0].pieces;  // of a row: 64 or 128 dims of 1, 2 or 4 bytes
+  if (p.fp8) {
+    if (pieces == 4) launch_evict_moves<true, 4>(p, st);
+    else launch_evict_moves<true, 8>(p, st);
+  } else {
+    if (pieces == 8) launch_evict_moves<false, 8>(p, st);
+    else if (pieces == 16) launch_evict_moves<false, 16>(p, st);
+    else launch_evict_moves<false, 32>(p, st);
+  }
   return hipGetLastError();
 }
 
