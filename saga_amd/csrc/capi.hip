@@ -1829,17 +1829,11 @@ int saga_dense_decode_fp8(const saga_tensor* query, const saga_kv_fp8* cache, co
     p.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + part);
     p.scores_ld = ld;
   }
-  if ((rc = hip_status(launch_dense_decode_fp8(p, static_cast<hipStream_t>(stream)), "dense_decode_fp8 launch"))) return rc;
-  if (weights) {
-    WeightsParams w = make_weights(weights, weights_add, kv_len, s.b, s.q_h, s.L);
-    w.scores = p.scores;
-    w.s_ld = ld;
-    w.pm = p.part + s.b * s.q_h * p.nsplit * s.d;
-    w.ps = w.pm + 1;
-    w.pstride = 2;
-    w.nparts = p.nsplit;
-    if ((rc = hip_status(launch_attention_weights(w, static_cast<hipStream_t>(stream)), "attention_weights launch"))) return rc;
-  }
+  WeightsParams w{};
+  if (weights) w = make_weights(weights, weights_add, kv_len, s.b, s.q_h, s.L);
+  if ((rc = hip_status(launch_dense_decode_fp8(p, weights ? &w : nullptr, static_cast<hipStream_t>(stream)),
+                       "dense_decode_fp8 launch")))
+    return rc;
   return ok();
 }
 

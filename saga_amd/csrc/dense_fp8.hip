@@ -15,13 +15,14 @@
 //     an MFMA each.  Lane (m, s) loads dims [m d / 16, + d / 16) of positions 8 s .. 8 s + 7 and
 //     pairs neighbouring positions with byte permutes, so that values pass through no LDS;
 //     MFMA e has dim m d / 16 + e in row m.
-// With scores asked for, a step's go to memory for the weights per position (evict.hip).
-// Kernel 2 joins the splits.
+// Kernel 2 joins the splits.  With weights per position asked for, a step's scores go to memory, and
+// kernel 2 has blocks that turn them into weights beside those that join.
 #include <algorithm>
 
 #include "dense_join.cuh"
 #include "fp8.cuh"
 #include "kernels.h"
+#include "weights.cuh"
 
 namespace saga {
 
@@ -309,6 +310,35 @@ __global__ void __launch_bounds__(256, 2) dense_fp8_kernel(DenseFp8Params p) {
   }
 }
 
+template <int D>
+__global__ void __launch_bounds__(256) dense_fp8_finish_kernel(DenseFp8Params p, WeightsParams w, int joins) {
+  if (static_cast<int>(blockIdx.x) < joins) dense_join<DenseFp8Params, D, 32, 8>(p, blockIdx.x);
+  else attention_weights(w, blockIdx.x - joins);
+}
+
+template <int D>
+static hipError_t launch_dense_fp8_finish(const DenseFp8Params& p, WeightsParams* w, hipStream_t st) {
+  if (!w) {
+    if (p.nsplit > 1) launch_dense_join<D>(p, st);
+    return hipSuccess;
+  }
+  w->scores = p.scores;
+  w->s_ld = p.scores_ld;
+  w->pm = p.part + static_cast<int64_t>(p.b) * p.q_h * p.nsplit * D;
+  w->ps = w->pm + 1;
+  w->pstride = 2;
+  w->nparts = p.nsplit;
+  // (to 64 splits a join in blocks of 32 dims adds in the order of one block of D: the same bits as without
+  // weights; more are joined by 32 groups)
+  if (p.nsplit > 64) launch_dense_join<D>(p, st);
+  const int64_t joins = p.nsplit > 1 && p.nsplit <= 64 ? static_cast<int64_t>(p.b) * p.q_h * (D / 32) : 0;
+  const int64_t blocks = joins + attention_weights_blocks(*w);
+  if (blocks >= (1LL << 24)) return hipErrorInvalidValue;  // a launch holds less than 2^32 threads
+  hipLaunchKernelGGL(dense_fp8_finish_kernel<D>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, p, *w,
+                     static_cast<int>(joins));
+  return hipSuccess;
+}
+
 template <int DT, int D, int NV>
 static void launch_dense_fp8_typed(const DenseFp8Params& p, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.b * p.nseg * p.nsplit));
@@ -330,7 +360,7 @@ static void launch_dense_fp8_units(const DenseFp8Params& p, int nv, hipStream_t 
   launch_dense_fp8_typed<DT, D, 1>(p, st);
 }
 
-hipError_t launch_dense_decode_fp8(DenseFp8Params& p, hipStream_t st) {
+hipError_t launch_dense_decode_fp8(DenseFp8Params& p, WeightsParams* w, hipStream_t st) {
   // Units of several whole value heads read and score their keys once for all of them: 5 (d 64) or 2
   // where a key head's count divides by that and 16 columns hold their query heads
   int nv = 1;
@@ -354,11 +384,13 @@ hipError_t launch_dense_decode_fp8(DenseFp8Params& p, hipStream_t st) {
   if (p.kv.d == 128) {
     if (bf) launch_dense_fp8_units<SAGA_DTYPE_BF16, 128>(p, nv, st);
     else launch_dense_fp8_units<SAGA_DTYPE_F16, 128>(p, nv, st);
-    if (ns > 1) launch_dense_join<128>(p, st);
+    const hipError_t e = launch_dense_fp8_finish<128>(p, w, st);
+    if (e != hipSuccess) return e;
   } else {
     if (bf) launch_dense_fp8_units<SAGA_DTYPE_BF16, 64>(p, nv, st);
     else launch_dense_fp8_units<SAGA_DTYPE_F16, 64>(p, nv, st);
-    if (ns > 1) launch_dense_join<64>(p, st);
+    const hipError_t e = launch_dense_fp8_finish<64>(p, w, st);
+    if (e != hipSuccess) return e;
   }
   return hipGetLastError();
 }

@@ -17,13 +17,13 @@ namespace saga {
 constexpr int kJoinSplits = 1024;
 
 template <class P, int D, int JD, int GR>
-__global__ void __launch_bounds__(GR * JD) dense_join_kernel(P p) {
+__device__ __forceinline__ void dense_join(const P& p, int block) {
   constexpr int NT = GR * JD;
   __shared__ float fm[kJoinSplits];
   __shared__ float red[NT / kWave];
   __shared__ float og[GR][JD];
   const int tid = threadIdx.x, grp = tid / JD, i = tid - grp * JD;
-  const int row = blockIdx.x / (D / JD), d0 = (blockIdx.x - row * (D / JD)) * JD;
+  const int row = block / (D / JD), d0 = (block - row * (D / JD)) * JD;
   const int bi = row / p.q_h, h = row - bi * p.q_h;
   const float* base = p.part + static_cast<int64_t>(row) * p.nsplit * D + d0 + i;
   const float2* ml = reinterpret_cast<const float2*>(p.part + static_cast<int64_t>(p.b) * p.q_h * p.nsplit * D) +
@@ -66,6 +66,11 @@ __global__ void __launch_bounds__(GR * JD) dense_join_kernel(P p) {
     for (int q = 1; q < GR; ++q) t += og[q][i];
     store_from_f32(p.out, p.out_dt, bi * p.o_sb + static_cast<int64_t>(h) * p.o_sh + d0 + i, q4_in_range(t / l, p.out_dt));
   }
+}
+
+template <class P, int D, int JD, int GR>
+__global__ void __launch_bounds__(GR * JD) dense_join_kernel(P p) {
+  dense_join<P, D, JD, GR>(p, blockIdx.x);
 }
 
 template <int D, class P>

@@ -474,7 +474,6 @@ struct DenseFp8Params {
   float* scores;  // [b * q_h][scores_ld] of the positions below kv_len, null: not asked for
   int64_t scores_ld;
 };
-hipError_t launch_dense_decode_fp8(DenseFp8Params& p, hipStream_t st);
 
 // ---- attention weights per position, eviction ----
 
@@ -492,6 +491,8 @@ struct WeightsParams {
   int32_t add;
 };
 hipError_t launch_attention_weights(const WeightsParams& p, hipStream_t st);
+// w: weights per position asked for (its scores and partials are p's), or null.
+hipError_t launch_dense_decode_fp8(DenseFp8Params& p, WeightsParams* w, hipStream_t st);
 
 // One kind of rows that an eviction moves: 16-byte pieces, byte strides.
 struct EvictRows {
