@@ -25,6 +25,8 @@ Decoder layout (SagaDecoder._WEIGHT_SHAPES): q, k, v rows concatenated in
 w_qkv [(n_q + n_k + n_v) * d, hidden] (zero bias when the model has none),
 gate and up rows in w_gu [2 * intermediate, hidden], RMSNorm weights ln1 /
 ln2 per layer and ln_f, the embedding, and lm_head (None when tied).
+Checkpoints with norms of queries and keys per head (q_norm / k_norm weights
+[head_dim]) give a shape with qk_norm and both weights per layer.
 Models with o_proj / MLP biases or a RoPE scaling rule other than the
 default are refused, not silently mis-run.
 """
@@ -33,6 +35,7 @@ from __future__ import annotations
 import glob
 import json
 import os
+from dataclasses import replace
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -147,6 +150,8 @@ def load_checkpoint(path: str, num_key_heads: Optional[int] = None,
             raise NotImplementedError(f"checkpoint has {extra}: o_proj / MLP biases are not supported")
     stored = shape_from_config(cfg, qkv_bias)  # the heads the tensors hold
     shape = stored if num_key_heads is None else shape_from_config(cfg, qkv_bias, num_key_heads)
+    qk_norm = pre.format(0) + "self_attn.q_norm.weight" in T
+    shape = replace(shape, qk_norm=qk_norm)
     s, d = shape, shape.head_dim
     src_n_k = stored.n_k
 
@@ -159,6 +164,8 @@ def load_checkpoint(path: str, num_key_heads: Optional[int] = None,
         return t
 
     w = {"ln1": [], "ln2": [], "w_qkv": [], "b_qkv": [], "w_o": [], "w_gu": [], "w_d": []}
+    if qk_norm:
+        w["q_norm"], w["k_norm"] = [], []
     for l in range(s.layers):
         p = pre.format(l)
         a = p + "self_attn."
@@ -176,6 +183,9 @@ def load_checkpoint(path: str, num_key_heads: Optional[int] = None,
             w["b_qkv"].append(cast(torch.cat([qb, kb, vb], 0)))
         else:
             w["b_qkv"].append(torch.zeros(s.qkv_width, dtype=dtype))
+        if qk_norm:
+            for n in ("q_norm", "k_norm"):
+                w[n].append(cast(expect(T.get(a + n + ".weight"), (d,), a + n + ".weight")))
         w["w_o"].append(cast(T.get(a + "o_proj.weight")))
         m = p + "mlp."
         w["w_gu"].append(cast(torch.cat([T.get(m + "gate_proj.weight"), T.get(m + "up_proj.weight")], 0)))

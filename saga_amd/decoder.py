@@ -21,6 +21,11 @@ captured graph serves every step.
 kv_bits=4 holds the caches in 4 bits (dense attention over them; RoPE and the
 quantising append are a launch of their own) and weight_bits=4 the decode
 projections and the LM head (opened layer by layer for a prompt's GEMMs).
+kv_fp8_block holds the caches in 8 bits, a scale per head and block of
+positions.  Models with norms of queries and keys (DecoderShape.qk_norm) take
+them with the rotation and the append in one launch.  kv_budget bounds a
+cache: whenever it is full, the positions that gathered the least attention
+weight leave it.
 """
 from __future__ import annotations
 
@@ -32,7 +37,7 @@ import torch
 
 from . import ops
 from .attention.attention import sdpa_attention_forward
-from .kv_cache import (KVCache, check_q4_decoder, kv_cache_bytes, projection_shapes,  # noqa: F401  (kv_cache_bytes re-exported)
+from .kv_cache import (KVCache, check_fp8_decoder, check_q4_decoder, kv_cache_bytes, projection_shapes,  # noqa: F401  (kv_cache_bytes re-exported)
                        skinny_gemm_supported)
 
 
@@ -50,6 +55,7 @@ class DecoderShape:
     rope_theta: float
     eps: float
     qkv_bias: bool = True
+    qk_norm: bool = False  # RMSNorm of every query and key head before the rotation
 
     @property
     def qkv_width(self) -> int:
@@ -99,19 +105,38 @@ class SagaDecoder:
     prompt attends over what its cache holds.  weight_bits 4 (bf16, batch at
     most 32): the projections and the LM head in 4 bits, groups of
     weight_group columns, in prompts too; the embedding stays as it is.
+    kv_fp8_block 32, 64 or 128 (mode "dense", bf16 or f16): caches in 8 bits,
+    a scale per head and so many positions; a prompt attends over what its
+    cache holds.
+    kv_budget > 0 (mode "dense", 16- or 8-bit caches): a cache of max_len places
+    that generation may run past.  When a step finds it full, every layer and
+    group of heads keeps kv_budget positions: the last kv_recent and the ones
+    that gathered the most attention weight, summed over the steps and over
+    a prompt's last 32 queries.  Rotations go on with the tokens' own positions.
+    What is evicted is gone: reset() then needs a prompt again.
     """
+
+    PROMPT_QUERIES = 32  # a prompt's last queries, whose attention weights a bounded cache starts with
 
     def __init__(self, shape: DecoderShape, batch: int, max_len: int, mode: str = "atopn", top_n: int = 512,
                  exempt_layers=(), device="cuda", dtype=torch.bfloat16, seed: int = 0, fuse_rope: bool = True,
                  pack_weights: bool = True, weights: Optional[dict] = None, keep_source_weights: bool = False,
                  k2_variant: int = 0, kv_bits: int = 16, kv_group: int = 64, weight_bits: int = 16,
-                 weight_group: int = 64):
+                 weight_group: int = 64, kv_fp8_block: int = 0, kv_budget: int = 0, kv_recent: int = 0):
         if mode not in ("atopn", "dense", "vanilla"):
             raise ValueError(f"mode must be 'atopn', 'dense' or 'vanilla', got {mode!r}")
         if kv_bits == 4 and mode != "dense":
             raise ValueError("kv_bits=4 needs mode 'dense'")
         check_q4_decoder(shape, batch, dtype, kv_bits, kv_group, weight_bits, weight_group)
+        check_fp8_decoder(shape, dtype, kv_fp8_block, kv_bits)
+        if kv_fp8_block and mode != "dense":
+            raise ValueError("kv_fp8_block needs mode 'dense'")
+        if kv_budget and (mode != "dense" or kv_bits != 16 or shape.head_dim not in (64, 128)):
+            raise ValueError("kv_budget needs mode 'dense', 16- or 8-bit caches and a head dim of 64 or 128")
+        if (kv_budget or kv_recent) and not (0 < kv_budget < max_len and 0 <= kv_recent <= kv_budget):
+            raise ValueError("kv_budget must lie between 1 and max_len - 1, kv_recent between 0 and kv_budget")
         self.kv_bits, self.weight_bits, self.weight_group = kv_bits, weight_bits, weight_group
+        self.kv_fp8_block, self.kv_budget, self.kv_recent = kv_fp8_block, kv_budget, kv_recent
         self.shape, self.batch, self.max_len, self.mode, self.top_n = shape, batch, max_len, mode, top_n
         self.exempt = set(exempt_layers)
         self.device, self.dtype = torch.device(device), dtype
@@ -135,8 +160,13 @@ class SagaDecoder:
             self.w_gu = [w(2 * s.intermediate, s.hidden) for _ in range(s.layers)]
             self.w_d = [w(s.hidden, s.intermediate) for _ in range(s.layers)]
             self.ln_f = torch.ones(s.hidden, device=self.device, dtype=dtype)
+            if s.qk_norm:
+                self.q_norm, self.k_norm = ([torch.ones(d, device=self.device, dtype=dtype) for _ in range(s.layers)]
+                                            for _ in range(2))
+        if not s.qk_norm:
+            self.q_norm = self.k_norm = [None] * s.layers
         # separate key-head and value-head caches [layer][batch, heads, max_len, d]
-        self.kv = KVCache(s, batch, max_len, self.device, dtype, bits=kv_bits, group=kv_group)
+        self.kv = KVCache(s, batch, max_len, self.device, dtype, bits=kv_bits, group=kv_group, fp8_block=kv_fp8_block)
         self.k_cache, self.v_cache = self.kv.k, self.kv.v
         # Atop-N threshold table, rows = batch * n_q (attention/attention.py:92-99)
         self.table = torch.zeros(max(s.layers, 1), batch * s.n_q, device=self.device, dtype=torch.float32)
@@ -144,6 +174,12 @@ class SagaDecoder:
         self.tokens = torch.zeros(batch, dtype=torch.int64, device=self.device)
         self.pos = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self.kv_len = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        # the place of a step's tokens in the cache: their position, but in a bounded cache
+        self.slot = torch.zeros_like(self.pos) if kv_budget else self.pos
+        self._used, self._evicted = 0, False  # places taken (every row's), on the host; whether a prompt's are gone
+        if kv_budget:
+            self.kv_weights = torch.zeros(s.layers, batch, math.gcd(s.n_k, s.n_v), max_len, device=self.device)
+            self._prompt_weights = torch.zeros_like(self.kv_weights)
         self._positions = torch.arange(max_len, dtype=torch.int32, device=self.device)  # vanilla mode's mask
         self._x = torch.empty(batch, s.hidden, device=self.device, dtype=dtype)
         self._h = torch.empty(batch, s.hidden, device=self.device, dtype=dtype)
@@ -157,7 +193,9 @@ class SagaDecoder:
         # decode projections: the skinny-GEMM kernel for up to 32 token rows
         self.use_gemv = skinny_gemm_supported(s, batch, dtype)
         # q/k/v projection, RoPE and cache append in one launch (pair-ordered rows)
-        self.fuse_rope = fuse_rope and self.use_gemv and d % 16 == 0 and kv_bits == 16 and weight_bits == 16
+        self.norm_append = bool(s.qk_norm or kv_budget or kv_fp8_block)  # the append with norms and rotations of its own
+        self.fuse_rope = (fuse_rope and self.use_gemv and d % 16 == 0 and kv_bits == 16 and weight_bits == 16
+                          and not self.norm_append)
         self.pack_weights = pack_weights
         self.keep_source_weights = keep_source_weights
         self.k2_variant = k2_variant
@@ -179,18 +217,21 @@ class SagaDecoder:
         "w_o": lambda s: (s.hidden, s.n_q * s.head_dim),
         "w_gu": lambda s: (2 * s.intermediate, s.hidden),
         "w_d": lambda s: (s.hidden, s.intermediate),
+        "q_norm": lambda s: (s.head_dim,),
+        "k_norm": lambda s: (s.head_dim,),
     }
-    _PER_LAYER = ("ln1", "ln2", "w_qkv", "b_qkv", "w_o", "w_gu", "w_d")
+    _PER_LAYER = ("ln1", "ln2", "w_qkv", "b_qkv", "w_o", "w_gu", "w_d", "q_norm", "k_norm")
 
     def _take_weights(self, weights: dict) -> None:
         """Weights given as tensors in the decoder's layout (one per name of
-        _WEIGHT_SHAPES; per-layer names hold a list; lm_head None = tied),
+        _WEIGHT_SHAPES; per-layer names hold a list; lm_head None = tied;
+        q_norm and k_norm where the shape has them),
         moved to the decoder's device and dtype, shapes checked."""
         s = self.shape
         for name, shape_of in self._WEIGHT_SHAPES.items():
             want = tuple(shape_of(s))
             val = weights.get(name)
-            if name == "lm_head" and val is None:
+            if name == "lm_head" and val is None or name in ("q_norm", "k_norm") and not s.qk_norm:
                 continue
             if val is None:
                 raise KeyError(f"weights: missing {name!r}")
@@ -295,8 +336,16 @@ class SagaDecoder:
         def buf(n):
             return torch.empty(max(int(n), 256), dtype=torch.uint8, device=self.device)
 
+        if self.kv_budget:
+            row = d if self.kv_fp8_block else d * torch.tensor([], dtype=self.dtype).element_size()
+            self.ws["evict"] = buf(lib.saga_evict_workspace_bytes(B, self.kv_weights.shape[2], self.kv_budget, self.kv_recent,
+                                                                  s.n_k + s.n_v, row, 1))
+            if not self.kv_fp8_block:
+                self.ws["weights"] = buf(lib.saga_attention_weights_workspace_bytes(B, s.n_q, s.n_k, L))
         if self.kv_bits == 4:
             self.ws["dense_q4"] = buf(lib.saga_dense_q4_workspace_bytes(B, s.n_q, L, d))
+        elif self.kv_fp8_block:
+            self.ws["dense_fp8"] = buf(lib.saga_dense_fp8_workspace_bytes(B, s.n_q, L, d, 1 if self.kv_budget else 0))
         else:
             self.ws["atopn"] = buf(max(ops.atopn_workspace_bytes(B, s.n_q, s.n_k, L, d, self.top_n, cal)
                                        for cal in (True, False)))
@@ -342,7 +391,7 @@ class SagaDecoder:
         x = self.embed.index_select(0, prompt.to(self.device).reshape(-1))
         pos = torch.arange(T, device=self.device, dtype=torch.int32)
         zeros = torch.zeros(T, device=self.device, dtype=torch.int32)
-        table = ops.rope_table(pos, d, s.rope_theta) if self.kv_bits == 4 else None
+        table = ops.rope_table(pos, d, s.rope_theta) if self.kv_bits == 4 or self.norm_append else None
         mod = _HeadGroups()
         for l in range(s.layers):
             n1, w_qkv, w_o, n2, w_gu, w_d = self._prefill_layer(l)
@@ -352,11 +401,21 @@ class SagaDecoder:
                 cache = self.kv.layer(l)
                 q = ops.rope_kv_append_q4(qkv, s.n_q, table, pos, cache, batch=zeros)
                 k, v = (t.transpose(0, 1).unsqueeze(0) for t in ops.read_kv_q4(cache, pos, zeros, dtype=self.dtype))
+            elif self.kv_fp8_block:
+                cache = self.kv.layer(l).rows(0)
+                q = ops.norm_rope_kv_append_fp8(qkv, s.n_q, table, zeros[:1], cache, self.q_norm[l], self.k_norm[l], s.eps)
+                k, v = (t.transpose(0, 1).unsqueeze(0) for t in ops.read_kv_fp8(cache, pos, zeros, dtype=self.dtype))
+            elif self.norm_append:
+                q = ops.norm_rope_kv_append(qkv, s.n_q, table, pos, self.k_cache[l], self.v_cache[l], self.q_norm[l],
+                                            self.k_norm[l], s.eps, batch=zeros)
+                k, v = self.k_cache[l, 0:1, :, :T], self.v_cache[l, 0:1, :, :T]
             else:
                 q = ops.rope_kv_append(qkv, s.n_q, s.n_k, s.n_v, s.rope_theta, pos, self.k_cache[l], self.v_cache[l],
                                        batch=zeros)
                 k = self.k_cache[l, 0:1, :, :T]
                 v = self.v_cache[l, 0:1, :, :T]
+            if self.kv_budget:
+                self._prompt_attention_weights(l, q, k)
             # the HIP prefill kernel when ops.prefill_supported holds for these
             # operands, else torch SDPA (attention/attention.py:13-53)
             o, _ = sdpa_attention_forward(mod, q.transpose(0, 1).unsqueeze(0), k, v, None, is_causal=True)
@@ -383,26 +442,39 @@ class SagaDecoder:
             first = ops.gemv(x[-1:], self.kw_lm, rms_eps=s.eps, workspace=self.ws.get("gemv")).argmax(dim=-1)
         for c in self.kv.tensors:
             c[:, 1:, :, :T] = c[:, 0:1, :, :T]
+        self._evicted = False
         self.prompt_len = T
         self.reset()
         self._first_token = first
         self.tokens.fill_(0)
         self.tokens.copy_(first.expand(self.batch))
 
+    def _prompt_attention_weights(self, l: int, q: torch.Tensor, k: torch.Tensor) -> None:
+        """What the prompt's positions gather from its last queries: rows of an expanded key, each as far as it sees."""
+        T, n = q.shape[0], min(self.PROMPT_QUERIES, q.shape[0])
+        seen = torch.arange(T - n + 1, T + 1, device=self.device, dtype=torch.int32)
+        w = torch.empty(n, self.kv_weights.shape[2], T, device=self.device)
+        ops.attention_weights(q[T - n:].unsqueeze(2), k.expand(n, -1, -1, -1), w, kv_len=seen, add=False)
+        self._prompt_weights[l] = 0.0
+        self._prompt_weights[l, :, :, :T] = w.sum(0)
+
     def fill_synthetic(self, prompt_len: int, seed: int = 1) -> None:
         """Fill the cache with N(0,1) keys/values of prompt_len positions
         instead of a prefill (tests and kernel-level runs)."""
         g = torch.Generator(device=self.device).manual_seed(seed)
-        if self.kv_bits == 4:
-            self._fill_synthetic_q4(prompt_len, g)
-        for c in (self.k_cache, self.v_cache) if self.kv_bits == 16 else ():
+        if self.kv_bits == 4 or self.kv_fp8_block:
+            self._fill_synthetic_held(prompt_len, g)
+        for c in (self.k_cache, self.v_cache) if self.k_cache is not None else ():
             c[..., :prompt_len, :] = torch.randn(c[..., :prompt_len, :].shape, generator=g, device=self.device,
                                                  dtype=torch.float32).to(self.dtype)
+        if self.kv_budget:
+            self._prompt_weights.zero_()
+        self._evicted = False
         self.prompt_len = prompt_len
         self._first_token = torch.zeros(1, dtype=torch.int64, device=self.device)
         self.reset()
 
-    def _fill_synthetic_q4(self, prompt_len: int, g: torch.Generator) -> None:
+    def _fill_synthetic_held(self, prompt_len: int, g: torch.Generator) -> None:
         s, d, B = self.shape, self.shape.head_dim, self.batch
         for l in range(s.layers):
             for p0 in range(0, prompt_len, 4096):
@@ -411,10 +483,19 @@ class SagaDecoder:
                 rows = torch.arange(B, device=self.device, dtype=torch.int32).repeat_interleave(n)
                 x = torch.randn(B * n, (1 + s.n_k + s.n_v) * d, generator=g, device=self.device).to(self.dtype)
                 unrotated = torch.tensor([1.0, 0.0], device=self.device).expand(B * n, d // 2, 2).contiguous()
-                ops.rope_kv_append_q4(x, 1, unrotated, pos, self.kv.layer(l), batch=rows)
+                if self.kv_fp8_block:  # (row by row, so are the tokens)
+                    ops.norm_rope_kv_append_fp8(x, 1, unrotated, pos[::n].contiguous(), self.kv.layer(l))
+                else:
+                    ops.rope_kv_append_q4(x, 1, unrotated, pos, self.kv.layer(l), batch=rows)
 
     def reset(self) -> None:
         """Rewind the decode state to just after the prompt."""
+        if self._evicted:
+            raise RuntimeError("reset: positions of the prompt were evicted from the bounded cache (prefill again)")
+        self._used = self.prompt_len
+        if self.kv_budget:
+            self.slot.fill_(self.prompt_len)
+            self.kv_weights.copy_(self._prompt_weights)
         self.pos.fill_(self.prompt_len)
         self.kv_len.fill_(self.prompt_len + 1)
         if hasattr(self, "_first_token"):
@@ -423,13 +504,38 @@ class SagaDecoder:
     # ------------------------------------------------------------------- decode
     @torch.no_grad()
     def step(self, calibrate: bool) -> None:
-        """One decode step for every batch row (static buffers only)."""
+        """One decode step for every batch row."""
+        self._make_room()
+        self._step(calibrate)
+
+    @torch.no_grad()
+    def _make_room(self) -> None:
+        """A place for the step's tokens: where a bounded cache is full, every layer is cut to kv_budget positions."""
+        if not self.kv_budget:
+            return
+        if self._used == self.max_len:
+            held = self.kv_len - 1  # (kv_len counts the step's token)
+            for l in range(self.shape.layers):
+                if self.kv_fp8_block:
+                    ops.evict_kv_fp8(self.kv.layer(l), self.kv_weights[l], held, self.kv_budget, self.kv_recent,
+                                     workspace=self.ws["evict"])
+                else:
+                    ops.evict_kv(self.k_cache[l], self.v_cache[l], self.kv_weights[l], held, self.kv_budget, self.kv_recent,
+                                 workspace=self.ws["evict"])
+            self.slot.fill_(self.kv_budget)
+            self.kv_len.fill_(self.kv_budget + 1)
+            self._used, self._evicted = self.kv_budget, True
+        self._used += 1
+
+    @torch.no_grad()
+    def _step(self, calibrate: bool) -> None:
+        """The kernels of a step (static buffers only)."""
         s, d, B = self.shape, self.shape.head_dim, self.batch
         ws = self.ws
         x = self._x
         # the token rows' embeddings and their rotations (once for all layers)
         ops.embed_rope(self.tokens, self.embed, x, self.pos, d, s.rope_theta,
-                       rope_table=self._rope if self.fuse_rope or self.kv_bits == 4 else None)
+                       rope_table=self._rope if self.fuse_rope or self.kv_bits == 4 or self.norm_append else None)
         gemv = ops.gemv_q4 if self.weight_bits == 4 else ops.gemv
         q4 = self._q.view(B, s.n_q, 1, d)
         for l in range(s.layers):
@@ -445,11 +551,20 @@ class SagaDecoder:
                     torch.addmm(self.b_qkv[l], self._h, self.w_qkv[l].t(), out=self._qkv)
                 if self.kv_bits == 4:
                     ops.rope_kv_append_q4(self._qkv, s.n_q, self._rope, self.pos, self.kv.layer(l), q_out=self._q)
+                elif self.kv_fp8_block:
+                    ops.norm_rope_kv_append_fp8(self._qkv, s.n_q, self._rope, self.slot, self.kv.layer(l), self.q_norm[l],
+                                                self.k_norm[l], s.eps, q_out=self._q)
+                elif self.norm_append:
+                    ops.norm_rope_kv_append(self._qkv, s.n_q, self._rope, self.slot, self.k_cache[l], self.v_cache[l],
+                                            self.q_norm[l], self.k_norm[l], s.eps, q_out=self._q)
                 else:
                     ops.rope_kv_append(self._qkv, s.n_q, s.n_k, s.n_v, s.rope_theta, self.pos, self.k_cache[l],
                                        self.v_cache[l], q_out=self._q)
             if self.kv_bits == 4:
                 ops.dense_decode_q4(q4, self.kv.layer(l), kv_len=self.kv_len, out=self._attn, workspace=ws["dense_q4"])
+            elif self.kv_fp8_block:
+                ops.dense_decode_fp8(q4, self.kv.layer(l), kv_len=self.kv_len, out=self._attn, workspace=ws["dense_fp8"],
+                                     weights=self.kv_weights[l] if self.kv_budget else None)
             else:
                 self._attention(l, q4, calibrate)
             if self.use_gemv:
@@ -470,6 +585,8 @@ class SagaDecoder:
             torch.mm(self._h, self.lm_head.t(), out=self._logits)
             torch.argmax(self._logits, dim=-1, out=self.tokens)
         ops.advance_positions(self.pos, self.kv_len)
+        if self.kv_budget:
+            ops.advance_positions(self.slot)
 
     def _attention(self, l: int, q4: torch.Tensor, calibrate: bool) -> None:
         """Layer l's attention over its 16-bit caches."""
@@ -478,6 +595,8 @@ class SagaDecoder:
             self._vanilla_attention(q4, K, V)
         elif self.mode == "dense" or l in self.exempt:
             ops.dense_decode(q4, K, V, kv_len=self.kv_len, out=self._attn, workspace=ws["dense"])
+            if self.kv_budget:
+                ops.attention_weights(q4, K, self.kv_weights[l], kv_len=self.kv_len, workspace=ws["weights"])
         elif calibrate:
             ops.atopn_calibrate(q4, K, V, self.top_n, self.table[l], kv_len=self.kv_len, out=self._attn,
                                 workspace=ws["atopn"])
@@ -502,7 +621,7 @@ class SagaDecoder:
         with torch.cuda.stream(side):
             for cal in (True, False):
                 self.reset()
-                self.step(cal)
+                self._step(cal)
         torch.cuda.current_stream(self.device).wait_stream(side)
         torch.cuda.synchronize(self.device)
         self.reset()
@@ -510,13 +629,14 @@ class SagaDecoder:
         for cal in (True, False):
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
-                self.step(cal)
+                self._step(cal)
             graphs.append(g)
         self.graph_cal, self.graph_fast = graphs
         torch.cuda.synchronize(self.device)
 
     def replay(self, i: int) -> None:
         """Step i of a generation: the calibration graph first (Atop-N), then fast steps."""
+        self._make_room()
         if self.mode == "atopn" and i == 0:
             self.graph_cal.replay()
         else:
@@ -533,7 +653,7 @@ class SagaDecoder:
         run the steps eagerly (same kernels, same results)."""
         if max_new_tokens < 1:
             return torch.empty(self.batch, 0, dtype=torch.int64, device=self.device)
-        if int(prompt.numel()) + max_new_tokens > self.max_len:
+        if not self.kv_budget and int(prompt.numel()) + max_new_tokens > self.max_len:
             raise ValueError("prompt + max_new_tokens does not fit the cache (max_len)")
         self.prefill(prompt)
         if graphs and self.graph_fast is None:

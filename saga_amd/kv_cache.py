@@ -13,7 +13,8 @@ kind: K [layers, B, k_h, Lmax, d] and V [layers, B, v_h, Lmax, d].
 
 With bits=4 a cache holds 4-bit codes with an f16 scale and offset per group
 of 32 or 64 dims (ops.KVQ4 per layer): 4.5 or 5 bits a value, so 3.2 to 3.6
-times the positions.
+times the positions.  With fp8_block it holds e4m3 numbers with a scale per
+head and block of that many positions (ops.KVFP8 per layer): twice the positions.
 
 plan_capacity() answers how long a context, or how large a batch, fits on one
 GPU next to the decode weights and workspaces: an MI355X has 288 GB of HBM3E.
@@ -40,6 +41,23 @@ def _check_bits(name: str, bits: int) -> None:
 def _check_q4_rows(d: int, group: int) -> None:
     if d not in (64, 128) or group not in (32, 64):
         raise ValueError(f"a 4-bit cache needs a head dim of 64 or 128 and groups of 32 or 64, got {d} and {group}")
+
+
+def check_fp8_decoder(shape, dtype, kv_fp8_block: int, kv_bits: int = 16) -> None:
+    """ValueError for 8-bit caches, or norms of queries and keys, that SagaDecoder does not take."""
+    if kv_fp8_block:
+        _check_fp8_rows(shape.head_dim, kv_fp8_block)
+        if kv_bits != 16:
+            raise ValueError("kv_fp8_block and kv_bits=4 exclude each other")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("kv_fp8_block needs bf16 or f16")
+    if shape.qk_norm and (shape.head_dim not in (64, 128) or kv_bits != 16):
+        raise ValueError("norms of queries and keys need a head dim of 64 or 128 and 16- or 8-bit caches")
+
+
+def _check_fp8_rows(d: int, block: int) -> None:
+    if d not in (64, 128) or block not in (32, 64, 128):
+        raise ValueError(f"an 8-bit cache needs a head dim of 64 or 128 and blocks of 32, 64 or 128 positions, got {d} and {block}")
 
 
 def projection_shapes(shape):
@@ -70,12 +88,17 @@ def check_q4_decoder(shape, batch: int, dtype, kv_bits: int, kv_group: int, weig
             raise ValueError("weight_bits=4 needs bf16, a batch of at most 32 and widths that are multiples of weight_group")
 
 
-def kv_cache_bytes(shape, batch: int, max_len: int, dtype=torch.bfloat16, bits: int = 16, group: int = 64) -> int:
-    """Bytes of the K and V caches of every layer; bits 4: codes and the scales of groups of `group` dims."""
+def kv_cache_bytes(shape, batch: int, max_len: int, dtype=torch.bfloat16, bits: int = 16, group: int = 64,
+                   fp8_block: int = 0) -> int:
+    """Bytes of the K and V caches of every layer; bits 4: codes and the scales of groups of `group` dims; fp8_block:
+    e4m3 numbers and the scales of blocks of so many positions."""
     _check_bits("bits", bits)
     d = shape.head_dim
     if bits == 4:
         _check_q4_rows(d, group)
+    if fp8_block:
+        _check_fp8_rows(d, fp8_block)
+        return shape.layers * batch * (shape.n_k + shape.n_v) * (max_len * d + -(-max_len // fp8_block) * 4)
     row = d * _es(dtype) if bits == 16 else d // 2 + 4 * (d // group)
     return shape.layers * batch * (shape.n_k + shape.n_v) * max_len * row
 
@@ -107,15 +130,17 @@ def decode_weight_bytes(shape, dtype=torch.bfloat16, decode_copies: bool = True,
 
 
 def decode_workspace_bytes(shape, batch: int, max_len: int, top_n: int, kv_bits: int = 16,
-                           weight_bits: int = 16) -> int:
+                           weight_bits: int = 16, kv_fp8_block: int = 0) -> int:
     """Atop-N and dense decode workspaces of one layer call (shared by all
-    layers; a 4-bit cache: its dense workspace), the projections' (of 16- or
-    4-bit weights), plus the per-step activations and the threshold table."""
+    layers; a 4- or 8-bit cache: its dense workspace), the projections' (of 16-
+    or 4-bit weights), plus the per-step activations and the threshold table."""
     from . import _lib
     lib = _lib.load()
     s = shape
     if kv_bits == 4:
         ws = lib.saga_dense_q4_workspace_bytes(batch, s.n_q, max_len, s.head_dim)
+    elif kv_fp8_block:
+        ws = lib.saga_dense_fp8_workspace_bytes(batch, s.n_q, max_len, s.head_dim, 0)
     else:
         ws = lib.saga_atopn_workspace_bytes(batch, s.n_q, s.n_k, max_len, s.head_dim, min(2 * top_n, max_len))
         ws += lib.saga_dense_workspace_bytes(batch, s.n_q, max_len, s.head_dim)
@@ -151,19 +176,22 @@ class CapacityPlan:
 def plan_capacity(shape, batch: Optional[int] = None, max_len: Optional[int] = None, budget_bytes: Optional[int] = None,
                   reserve_fraction: float = 0.05, top_n: int = 512, dtype=torch.bfloat16,
                   align: int = 256, kv_bits: int = 16, weight_bits: int = 16, group: int = 64,
-                  kv_group: Optional[int] = None, weight_group: Optional[int] = None) -> CapacityPlan:
+                  kv_group: Optional[int] = None, weight_group: Optional[int] = None,
+                  kv_fp8_block: int = 0) -> CapacityPlan:
     """The largest max_len for a given batch, or the largest batch for a given
     max_len (give exactly one), that fits budget_bytes (default: the current
     device's total memory, else 288 GB) minus reserve_fraction, next to the
     decode weights (with their decode copies) and workspaces.  max_len is
     rounded down to a multiple of `align` positions.  kv_bits, weight_bits:
     caches and decode copies in 4 bits, in groups of kv_group and weight_group
-    (`group` where not given); what SagaDecoder refuses is refused, and a
-    batch searched for ends at the 32 rows that 4-bit weights take."""
+    (`group` where not given); kv_fp8_block: caches in 8 bits, in blocks of so
+    many positions; what SagaDecoder refuses is refused, and a batch searched
+    for ends at the 32 rows that 4-bit weights take."""
     if (batch is None) == (max_len is None):
         raise ValueError("give exactly one of batch and max_len")
     kv_group, weight_group = kv_group or group, weight_group or group
     check_q4_decoder(shape, batch or 1, dtype, kv_bits, kv_group, weight_bits, weight_group)
+    check_fp8_decoder(shape, dtype, kv_fp8_block, kv_bits)
     if budget_bytes is None:
         budget_bytes = (torch.cuda.get_device_properties(0).total_memory if torch.cuda.is_available()
                         else HBM_BYTES_MI355X)
@@ -173,8 +201,8 @@ def plan_capacity(shape, batch: Optional[int] = None, max_len: Optional[int] = N
     def fits(b: int, L: int) -> Optional[CapacityPlan]:
         if weight_bits == 4 and b > 32:
             return None
-        kv = kv_cache_bytes(shape, b, L, dtype, kv_bits, kv_group)
-        ws = decode_workspace_bytes(shape, b, L, top_n, kv_bits, weight_bits)
+        kv = kv_cache_bytes(shape, b, L, dtype, kv_bits, kv_group, kv_fp8_block)
+        ws = decode_workspace_bytes(shape, b, L, top_n, kv_bits, weight_bits, kv_fp8_block)
         if kv + wbytes + ws > avail:
             return None
         return CapacityPlan(b, L, kv, wbytes, ws, budget_bytes)
@@ -211,36 +239,47 @@ class KVCache:
     """K [layers, B, k_h, Lmax, d] and V [layers, B, v_h, Lmax, d], zero-filled;
     layer(l) returns the reference-layout views (k [B, k_h, Lmax, d],
     v [B, v_h, Lmax, d]).  bits=4: 4-bit codes and scales (zeros) of groups of
-    `group` dims; layer(l) returns ops.KVQ4 and k, v are None."""
+    `group` dims; layer(l) returns ops.KVQ4 and k, v are None.  fp8_block: e4m3
+    numbers and scales (zeros) of blocks of so many positions; layer(l) returns
+    ops.KVFP8 and k, v are None."""
 
     def __init__(self, shape, batch: int, max_len: int, device="cuda", dtype=torch.bfloat16,
-                 check_free: bool = True, bits: int = 16, group: int = 64):
+                 check_free: bool = True, bits: int = 16, group: int = 64, fp8_block: int = 0):
         dev = torch.device(device)
         d = shape.head_dim
         _check_bits("bits", bits)
-        need = kv_cache_bytes(shape, batch, max_len, dtype, bits, group)
+        if fp8_block and bits != 16:
+            raise ValueError("fp8_block and bits=4 exclude each other")
+        need = kv_cache_bytes(shape, batch, max_len, dtype, bits, group, fp8_block)
         if check_free and dev.type == "cuda":
             free, _ = torch.cuda.mem_get_info(dev)
             if need > 0.8 * free:
                 raise MemoryError(f"KV cache of {need / 2**30:.1f} GiB does not fit in {free / 2**30:.1f} GiB free "
                                   f"HBM (plan_capacity() gives the largest batch / context)")
-        if bits == 4:
+        self.k = self.v = self.q4 = self.fp8 = None
+        if fp8_block:
+            from .ops import KVFP8
+            blocks = -(-max_len // fp8_block)
+            parts = [torch.zeros(shape.layers, batch, h, *row, device=dev, dtype=dt) for h in (shape.n_k, shape.n_v)
+                     for row, dt in (((max_len, d), torch.uint8), ((blocks,), torch.float32))]
+            self.fp8 = KVFP8(*parts, fp8_block)
+        elif bits == 4:
             from .ops import KVQ4
 
             def zeros(heads, row, dt):
                 return torch.zeros(shape.layers, batch, heads, max_len, row, device=dev, dtype=dt)
 
-            self.k = self.v = None
             self.q4 = KVQ4(*(zeros(h, row, dt) for h in (shape.n_k, shape.n_v)
                              for row, dt in ((d // 2, torch.uint8), (2 * d // group, torch.float16))))
         else:
             self.k = torch.zeros(shape.layers, batch, shape.n_k, max_len, d, device=dev, dtype=dtype)
             self.v = torch.zeros(shape.layers, batch, shape.n_v, max_len, d, device=dev, dtype=dtype)
-            self.q4 = None
         self.batch, self.max_len, self.bits = batch, max_len, bits
 
     @property
     def tensors(self):
+        if self.fp8 is not None:
+            return self.fp8[:4]
         return self.q4 if self.bits == 4 else (self.k, self.v)
 
     @property
@@ -248,4 +287,6 @@ class KVCache:
         return sum(t.numel() * t.element_size() for t in self.tensors)
 
     def layer(self, l: int):
+        if self.fp8 is not None:
+            return type(self.fp8)(*(t[l] for t in self.fp8[:4]), self.fp8.block)
         return type(self.q4)(*(t[l] for t in self.q4)) if self.bits == 4 else (self.k[l], self.v[l])

@@ -44,7 +44,9 @@ What it mirrors (speedup.py:447-700):
                         (speedup.py:640-661).
 
 Beyond the reference: --kv_bits 4 decodes `full` over 4-bit caches and
---weight_bits 4 with 4-bit projections and LM head (SagaDecoder's options).
+--weight_bits 4 with 4-bit projections and LM head, --kv_fp8_block 64 decodes
+`full` over 8-bit caches with a scale per head and 64 positions (SagaDecoder's
+options).
 
 Models: `--model_path` is a local checkpoint directory (config.json +
 safetensors, loaded by saga_amd.checkpoint; merge mode averages its key heads
@@ -85,8 +87,11 @@ def _label(mode: str, param: Optional[int]) -> str:
 
 
 def _bits(args) -> str:
-    """What of a configuration is held in 4 bits: "", "kv4", "w4" or "kv4-w4"."""
+    """What of a configuration is held in few bits: "", "kv4", "w4", "kv4-w4", or with "kv8b64" in the place of "kv4"
+    (8 bits, blocks of 64)."""
     names = [n for n, flag in (("kv4", "kv_bits"), ("w4", "weight_bits")) if getattr(args, flag, 16) == 4]
+    if getattr(args, "kv_fp8_block", 0):
+        names.insert(0, f"kv8b{args.kv_fp8_block}")
     return "-".join(names)
 
 
@@ -126,7 +131,8 @@ def run_config(args, mode: str, param: Optional[int], batch: int, seq_len: int, 
     exempt = tuple(int(x) for x in args.exempt_layers.split(",") if x.strip())
     n_new = args.num_new_tokens
     m = build_decoder(args.model_path, merge, args.new_heads, batch, seq_len + n_new, mode, param or 512, exempt,
-                      dtype, kv_bits=getattr(args, "kv_bits", 16), weight_bits=getattr(args, "weight_bits", 16))
+                      dtype, kv_bits=getattr(args, "kv_bits", 16), weight_bits=getattr(args, "weight_bits", 16),
+                      kv_fp8_block=getattr(args, "kv_fp8_block", 0))
     torch.manual_seed(0)
     m.prefill(torch.randint(0, m.shape.vocab, (seq_len,), dtype=torch.int64))
     graphs = bool(getattr(args, "cuda_graph", True))
@@ -178,6 +184,8 @@ def _sub_cmd(args, mode, param, batch, seq_len, merge_mode) -> List[str]:
     for flag in ("kv_bits", "weight_bits"):
         if getattr(args, flag, 16) != 16:
             cmd += ["--" + flag, str(getattr(args, flag))]
+    if getattr(args, "kv_fp8_block", 0):
+        cmd += ["--kv_fp8_block", str(args.kv_fp8_block)]
     if args.exempt_layers:
         cmd += ["--exempt_layers", args.exempt_layers]
     if getattr(args, "cuda_graph", False):
@@ -194,8 +202,11 @@ def describe_flags(args) -> str:
              f"{', --no_compile' if args.no_compile else ''} accepted)",
              "CUDA graph: " + ("enabled (HIP graphs: calibration step, fast step)" if args.cuda_graph
                                else "disabled (kernels launched eagerly per step)")]
-    if _bits(args):
-        lines.append(f"Held in 4 bits: {_bits(args)} (kv4: caches; w4: projections and LM head)")
+    if getattr(args, "kv_fp8_block", 0):
+        lines.append(f"Caches in 8 bits: a scale per head and {args.kv_fp8_block} positions")
+    four = "-".join(n for n in _bits(args).split("-") if n.endswith("4") and not n.startswith("kv8"))
+    if four:
+        lines.append(f"Held in 4 bits: {four} (kv4: caches; w4: projections and LM head)")
     if args.calibrate_during_measurement:
         lines.append("Calibration during measurement: on (every measured generation starts with it)")
     if args.profile_decode:
@@ -226,6 +237,8 @@ def build_parser() -> argparse.ArgumentParser:
                     help="bits of a cached key / value element (4: full attention only)")
     ap.add_argument("--weight_bits", type=int, default=16, choices=[16, 4],
                     help="bits of a projection weight in the decode step (4: bfloat16, batch at most 32)")
+    ap.add_argument("--kv_fp8_block", type=int, default=0, choices=[0, 32, 64, 128],
+                    help="caches in 8 bits with a scale per head and so many positions (full attention only; 0: no)")
     ap.add_argument("--no_compile", action="store_true",
                     help="accepted (no-op): the decode step is hand-written HIP kernels, not torch.compile output")
     ap.add_argument("--compile_mode", default="default", choices=["default", "reduce-overhead", "max-autotune"],
@@ -255,6 +268,8 @@ def main(argv=None) -> int:
     modes = parse_attention(args.attention)
     if args.kv_bits == 4 and any(m != "full" for m, _ in modes):
         raise ValueError("--kv_bits 4 decodes with --attention full")
+    if args.kv_fp8_block and (args.kv_bits == 4 or any(m != "full" for m, _ in modes)):
+        raise ValueError("--kv_fp8_block decodes with --attention full and without --kv_bits 4")
 
     if args._subprocess_json:  # one configuration, JSON on stdout
         (mode, param), = modes

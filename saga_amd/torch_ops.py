@@ -16,6 +16,8 @@ Operators (namespace "saga"):
     -> out [b, q_h, 1, d]                         (attention/attention.py:64-85)
   * dense_decode_q4(query, k_codes, k_scales, v_codes, v_scales, attention_mask,
     scaling, kv_len) -> out [b, q_h, 1, d]        (the same over the parts of an ops.KVQ4)
+  * dense_decode_fp8(query, k_codes, k_scales, v_codes, v_scales, block,
+    attention_mask, scaling, kv_len) -> out [b, q_h, 1, d]  (... of an ops.KVFP8)
   * prefill_attention(query, key, value, attention_mask, scaling, is_causal)
     -> out [b, l_q, q_h, d]                       (attention/attention.py:13-53)
 """
@@ -79,6 +81,20 @@ def dense_decode_q4(query: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.
 
 @dense_decode_q4.register_fake
 def _dense_decode_q4_fake(query, k_codes, k_scales, v_codes, v_scales, attention_mask=None, scaling=None, kv_len=None):
+    return _out_like(query)
+
+
+@torch.library.custom_op("saga::dense_decode_fp8", mutates_args=())
+def dense_decode_fp8(query: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+                     v_scales: torch.Tensor, block: int, attention_mask: Optional[torch.Tensor] = None,
+                     scaling: Optional[float] = None, kv_len: Optional[torch.Tensor] = None) -> torch.Tensor:
+    return ops.dense_decode_fp8(query, ops.KVFP8(k_codes, k_scales, v_codes, v_scales, block), attention_mask, scaling,
+                                kv_len=kv_len)
+
+
+@dense_decode_fp8.register_fake
+def _dense_decode_fp8_fake(query, k_codes, k_scales, v_codes, v_scales, block, attention_mask=None, scaling=None,
+                           kv_len=None):
     return _out_like(query)
 
 
