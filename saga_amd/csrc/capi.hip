@@ -1613,8 +1613,8 @@ EvictLayout evict_layout(int64_t B, int64_t G, int64_t keep, int64_t recent, int
     off = align256(off + bytes);
     return at;
   };
-  const int64_t chunks = (keep + 63) / 64, staged = in_place ? std::min(keep, recent + 127) : 0;
-  o.gap = take(B * G * chunks * 8);
+  const int64_t chunks = (keep + 31) / 32, staged = in_place ? std::min(keep, recent + 127) : 0;
+  o.gap = take(B * G * chunks * 4);
   o.gap_at = take(B * G * chunks * 4);
   o.movers = take(B * G * keep * 4);
   o.stage = take(B * heads * staged * row_bytes);
@@ -1652,7 +1652,7 @@ int evict_run(EvictParams& p, const saga_tensor* weights, const int32_t* kv_len,
   p.wo_sb = wo->stride[0], p.wo_sg = wo->stride[1], p.wo_len = wo->shape[2];
   p.kv_len = kv_len;
   p.kept = kept;
-  p.gap = reinterpret_cast<uint64_t*>(ws + lay.gap);
+  p.gap = reinterpret_cast<uint32_t*>(ws + lay.gap);
   p.gap_at = reinterpret_cast<int32_t*>(ws + lay.gap_at);
   p.movers = reinterpret_cast<int32_t*>(ws + lay.movers);
   p.stage_w = reinterpret_cast<float*>(ws + lay.stage_w);

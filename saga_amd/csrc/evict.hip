@@ -30,50 +30,51 @@ hipError_t launch_attention_weights(const WeightsParams& p, hipStream_t st) {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
+constexpr int kSelNear = 2048;
 
 template <int SEG>
 struct SelShared {
-  uint32_t key[SEG];  // ranking keys
+  alignas(16) uint32_t key[SEG];  // ranking keys, four positions' together, of each 32 positions in an order of their own
   int hist[2048];
   int cnt[kSelWaves];
   int sel_bin, sel_above, sel_cnt;
   int sums[4][kSelWaves];
-  uint32_t near[SEG / 16];                                // keys of the H-th largest's bin
-  unsigned long long a[SEG / kWave], b[SEG / kWave];      // per chunk: masks of larger and of equal keys
+  uint32_t near[kSelNear];  // keys of the H-th largest's bin
 };
 
 // A weight as what it is ranked by: any NaN above all numbers, -0 as 0; never 0, which stands for no position.
 __device__ __forceinline__ uint32_t rank_key(float w) { return f32_to_key(w == w ? w + 0.f : __uint_as_float(0x7fffffffu)); }
 
 // The lowest `count` set bits of m.
-__device__ __forceinline__ unsigned long long low_bits(unsigned long long m, int count) {
-  if (count == 0) return 0ull;
-  const int drop = __popcll(m) - count;
-  for (int i = 0; i < drop; ++i) m &= ~(1ull << (63 - __clzll(static_cast<long long>(m))));
+__device__ __forceinline__ uint32_t low_bits(uint32_t m, int count) {
+  if (count == 0) return 0u;
+  const int drop = __popc(m) - count;
+  for (int i = 0; i < drop; ++i) m &= ~(1u << (31 - __clz(static_cast<int>(m))));
   return m;
 }
 
-// Bits of positions below `end` of a chunk of 64 that starts at p0.
-__device__ __forceinline__ unsigned long long bits_below(int end, int p0) {
-  const int n = min(max(end - p0, 0), 64);
-  return n == 0 ? 0ull : ~0ull >> (64 - n);
+// Bits of positions below `end` of 32 that start at p0.
+__device__ __forceinline__ uint32_t bits_below(int end, int p0) {
+  const int n = min(max(end - p0, 0), 32);
+  return n == 0 ? 0u : ~0u >> (32 - n);
 }
 
 // One block per (batch row, group), a segment of SEG positions' ranking keys in LDS (a row of one
 // segment is read once, longer ones for every pass).  The H-th largest key by radix (11, 11, 10
 // bits), equal ones by position: the first digits are counted as the row is read; the other two
 // over the few keys that share the H-th's, if they are few and the row is one segment, else
-// over all.  What is large of a chunk of 64 positions is one 64-bit mask, and thread c counts
-// chunk c: every prefix of the selection is one scan of the block.  The result is, per chunk of
-// places below H, the mask of its gaps and the first one's rank, and the positions that move there
-// in order; what to do with them is the moving blocks' work, of which there are many.
-// One CU's work, about 4 cycles an instruction and wave: 8 x 32769 positions 82 us with keys in
-// registers and code unrolled over them, 36 with three digits over all keys.
+// over all.  What is large of 32 positions is one mask, a thread's: every prefix of the selection
+// is one scan of the block.  The result is, per 32 places below H, the mask of their gaps and
+// the first one's rank, and the positions that move there in order; what to do with them is the
+// moving blocks' work, of which there are many.
+// One CU's work: 8 x 32769 positions 18.8 us, of which the row's 128 KB take 5 (what one CU gets from
+// memory; 16 or 32 loads in flight for 8, or 16 bytes each, no less), 20 rows of 8195 15.5.  Measured
+// before: 82 us with keys in registers and code unrolled over them, 36 with three digits over all
+// keys, 22 with masks by ballots over 64 positions a wave.
 template <int SEG>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p) {
   __shared__ SelShared<SEG> sh;
-  constexpr int CH = SEG / kWave, NEAR = SEG / 16;
-  static_assert(CH <= kSelThreads && SEG % kSelThreads == 0, "a thread per chunk");
+  static_assert(SEG <= 32 * kSelThreads && SEG % (4 * kSelThreads) == 0, "32 positions a thread");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bi = blockIdx.x / p.G, gi = blockIdx.x - bi * p.G;
   const int n = min(max(p.kv_len[bi], 0), p.Lmax);
@@ -83,52 +84,58 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
   const int H = p.keep - p.recent, nc = n - p.recent;  // candidates: [0, nc), nc > H
   const int nseg = (nc + SEG - 1) / SEG;
   constexpr uint32_t kZero = 0x80000000u;
-  // f(key) of this thread's positions of a segment as they are read into LDS (a wave's chunks are its own:
-  // it reads them without a barrier); 0 behind nc, to the last chunk's end
+  // f(key) of this thread's positions of a segment as they are read into LDS, 0 behind nc to the end of
+  // a round.  Units of four positions are permuted within their 32, so that threads that each read
+  // their 32 meet other banks.
+  constexpr int U = SEG < 8 * kSelThreads ? SEG / kSelThreads : 8, ROUND = U * kSelThreads;
+  const int own = (tid & ~31) | ((((tid >> 2) ^ (tid >> 5)) & 7) << 2) | (tid & 3);
   auto load = [&](int seg, auto f) {
-    constexpr int U = 8;
-    const int whole = (min(SEG, nc - seg * SEG) + kWave - 1) / kWave * kWave;
-    for (int j0 = tid; j0 < whole; j0 += U * kSelThreads) {
+    const int end = nc - seg * SEG, whole = min(SEG, end);
+    float next[U];
+    auto fetch = [&](int j0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u] = w[seg * SEG + min(j0 + u * kSelThreads + tid, end - 1)];
+    };
+    fetch(0);
+    for (int j0 = 0; j0 < whole; j0 += ROUND) {
       float v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = w[min(seg * SEG + j0 + u * kSelThreads, nc - 1)];
+      for (int u = 0; u < U; ++u) v[u] = next[u];
+      if (j0 + ROUND < whole) fetch(j0 + ROUND);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = j0 + u * kSelThreads;
-        const uint32_t key = seg * SEG + j < nc ? rank_key(v[u]) : 0u;
-        if (j < SEG) sh.key[j] = key;
+        const uint32_t key = j0 + u * kSelThreads + tid < end ? rank_key(v[u]) : 0u;
+        sh.key[j0 + u * kSelThreads + own] = key;
         f(key);
       }
     }
   };
-  // f(chunk, key) of the segment's chunks, wave by wave
-  auto chunks = [&](int seg, auto f) {
-    constexpr int U = 4;
-    const int nch = (min(SEG, nc - seg * SEG) + kWave - 1) / kWave;
-    for (int c0 = wave; c0 < nch; c0 += U * kSelWaves) {
-      uint32_t key[U];
+  // f(key) of the segment's positions, a wave's those that it has read
+  auto each = [&](int seg, auto f) {
+    for (int j0 = 0; j0 < min(SEG, nc - seg * SEG); j0 += 4 * kSelThreads) {
+      uint32_t key[4];
 #pragma unroll
-      for (int u = 0; u < U; ++u) key[u] = c0 + u * kSelWaves < nch ? sh.key[(c0 + u * kSelWaves) * kWave + lane] : 0u;
+      for (int u = 0; u < 4; ++u) key[u] = sh.key[j0 + u * kSelThreads + tid];
 #pragma unroll
-      for (int u = 0; u < U; ++u) f(c0 + u * kSelWaves, key[u]);
+      for (int u = 0; u < 4; ++u) f(key[u]);
     }
   };
-  // The masks of keys above `top` and of keys in [from, top] of a segment's chunks: chunk c's in thread c
-  unsigned long long gt = 0, eq = 0;
+  auto key_of = [&](int i) { return sh.key[tid * 32 + ((((i >> 2) ^ tid) & 7) << 2) + (i & 3)]; };
+  // The masks of keys above `top` and of keys in [from, top] of this thread's positions of a segment
+  uint32_t gt = 0, eq = 0;
   auto masks = [&](int seg, uint32_t from, uint32_t top) {
-    int k = 0;
-    unsigned long long ga = 0, ea = 0;  // lane k: chunk k of the wave
-    chunks(seg, [&](int c, uint32_t key) {
-      const unsigned long long g = __ballot(key > top), e = __ballot(key >= from) & ~g;
-      ga = lane == k ? g : ga;
-      ea = lane == k ? e : ea;
-      ++k;
-    });
-    const int c = lane * kSelWaves + wave;
-    if (lane < CH / kSelWaves) sh.a[c] = ga, sh.b[c] = ea;
-    lds_sync();
-    gt = tid < CH ? sh.a[tid] : 0ull;
-    eq = tid < CH ? sh.b[tid] : 0ull;
+    gt = eq = 0;
+    if (tid * 32 >= min(SEG, nc - seg * SEG)) return;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(&sh.key[tid * 32 + (((i ^ tid) & 7) << 2)]);
+#pragma unroll
+      for (int e = 3; e >= 0; --e) {
+        gt = 2 * gt + (k[e] > top ? 1u : 0u);
+        eq = 2 * eq + (k[e] >= from ? 1u : 0u);
+      }
+    }
+    eq &= ~gt;
   };
   auto wave_part = [&](int v, int which) {  // v of the wave's threads before
     const int incl = wave_incl_scan(v, lane);
@@ -162,21 +169,21 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
     }
     if (zeros && lane == 0) atomicAdd(&sh.hist[kZero >> 21], zeros);
   }
+  lds_sync();
   if (H > 0) {
     need = H;
-    lds_sync();
     int bin, above, count;
     hist_pick<kSelThreads>(sh, 2048, need, bin, above, count);
     uint32_t prefix = static_cast<uint32_t>(bin) << 21;
     need -= above;
-    few = nseg == 1 && count <= NEAR;
+    few = nseg == 1 && count <= kSelNear;
     int listed = 0;
     if (few) {
       masks(0, prefix, prefix | 0x1fffffu);
-      const int at = wave_part(__popcll(eq), 0);
+      const int at = wave_part(__popc(eq), 0);
       lds_sync();
       int k = at + block_part(0, listed);
-      for (unsigned long long m = eq; m; m &= m - 1) sh.near[k++] = sh.key[tid * kWave + __builtin_ctzll(m)];
+      for (uint32_t m = eq; m; m &= m - 1) sh.near[k++] = key_of(__builtin_ctz(m));
     }
 #pragma unroll 1
     for (int pass = 1; pass < 3; ++pass) {
@@ -193,7 +200,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
         int zeros = 0;
         for (int seg = 0; seg < nseg; ++seg) {
           if (nseg > 1) load(seg, [](uint32_t) {});
-          chunks(seg, [&](int c, uint32_t key) {
+          each(seg, [&](uint32_t key) {
             const bool zero = key == kZero;
             zeros += __popcll(__ballot(zero));
             if ((((key ^ prefix) & hmask) | (zero ? 1u : 0u)) == 0u) atomicAdd(&sh.hist[(key >> shift) & (nb - 1)], 1);
@@ -208,41 +215,42 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
     }
     T = prefix;
     if (few) {  // of the H-th's bin: above T, and T
-      unsigned long long same = 0;
-      for (unsigned long long m = eq; m; m &= m - 1) {
-        const uint32_t key = sh.key[tid * kWave + __builtin_ctzll(m)];
+      uint32_t same = 0;
+      for (uint32_t m = eq; m; m &= m - 1) {
+        const uint32_t key = key_of(__builtin_ctz(m));
         if (key > T) gt |= m & -m;
         if (key == T) same |= m & -m;
       }
       eq = same;
     }
   }
-  const int nplace = (p.keep + kWave - 1) / kWave;
+  const int nplace = (p.keep + 31) / 32;
   int32_t* movers = p.movers + row * p.keep;
   int eq_base = 0, moved = 0, opened = 0;  // of the segments before
   for (int seg = 0; seg < nseg; ++seg) {
     if (nseg > 1) {
       __syncthreads();  // (the segment before has been read)
       load(seg, [](uint32_t) {});
+      lds_sync();
     }
     if (!few) masks(seg, T, T);
-    const int chunk = seg * CH + tid, p0 = chunk * kWave, ne = __popcll(eq), eq_at = wave_part(ne, 1);
+    const int p0 = seg * SEG + tid * 32, ne = __popc(eq), eq_at = wave_part(ne, 1);
     lds_sync();
     int all;
     const int before = eq_base + eq_at + block_part(1, all);
     eq_base += all;
-    const unsigned long long large = gt | low_bits(eq, min(max(need - before, 0), ne)), low = bits_below(H, p0);
-    const unsigned long long mov = large & ~low, gap = tid < CH ? ~large & low : 0ull;
-    const int mov_at = wave_part(__popcll(mov), 2), gap_at = wave_part(__popcll(gap), 3);
+    const uint32_t large = gt | low_bits(eq, min(max(need - before, 0), ne)), low = bits_below(H, p0);
+    const uint32_t mov = large & ~low, gap = tid * 32 < SEG ? ~large & low : 0u;
+    const int mov_at = wave_part(__popc(mov), 2), gap_at = wave_part(__popc(gap), 3);
     lds_sync();
     int k = moved + mov_at + block_part(2, all);
     moved += all;
-    for (unsigned long long m = mov; m; m &= m - 1) movers[k++] = p0 + __builtin_ctzll(m);
+    for (uint32_t m = mov; m; m &= m - 1) movers[k++] = p0 + __builtin_ctz(m);
     k = opened + gap_at + block_part(3, all);
     opened += all;
-    if (tid < CH && chunk < nplace) {
-      p.gap[row * nplace + chunk] = gap;
-      p.gap_at[row * nplace + chunk] = k;
+    if (tid * 32 < SEG && p0 < p.keep) {
+      p.gap[row * nplace + p0 / 32] = gap;
+      p.gap_at[row * nplace + p0 / 32] = k;
     }
   }
 }
@@ -288,15 +296,15 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictParams p) {
   int from = -1;
   float scale = 0.f;
   if (tid < kMoveRows) {
-    const int64_t at = group * ((p.keep + kWave - 1) / kWave) + min(mine, p.keep - 1) / kWave;
+    const int64_t at = group * ((p.keep + 31) / 32) + min(mine, p.keep - 1) / 32;
     const int kv = p.kv_len[bi];
-    const unsigned long long gap = p.gap[at];  // (nothing is there where nothing is evicted)
-    const int rank = p.gap_at[at] + __popcll(gap & lanes_below(mine & 63));
+    const uint32_t gap = p.gap[at];  // (nothing is there where nothing is evicted)
+    const int rank = p.gap_at[at] + __popc(gap & ((1u << (mine & 31)) - 1));
     const int n = min(max(kv, 0), p.Lmax);
     if (mine < p.keep && (PHASE != 2 || mine >= p.staged0)) {
       if (n <= p.keep) from = mine < n ? mine : -1;
       else if (mine >= H) from = n - p.keep + mine;
-      else from = (gap >> (mine & 63)) & 1 ? p.movers[group * p.keep + rank] : mine;
+      else from = (gap >> (mine & 31)) & 1 ? p.movers[group * p.keep + rank] : mine;
     }
     from_sh[tid] = from;
     if (FP8 && from >= 0 && !is_w) {

@@ -516,8 +516,8 @@ struct EvictParams {
   int64_t wo_sb, wo_sg, wo_len;
   const int32_t* kv_len;
   int32_t* kept;     // [B][G][keep]
-  uint64_t* gap;     // [B][G][keep / 64, rounded up] places below keep - recent whose position goes
-  int32_t* gap_at;   // rank of a chunk's first gap among all
+  uint32_t* gap;     // [B][G][keep / 32, rounded up] places below keep - recent whose position goes
+  int32_t* gap_at;   // rank of the first gap of 32 among all
   int32_t* movers;   // [B][G][keep] what comes to the gaps, by rank
   float* stage_w;    // in place: weights of the staged places
   int32_t B, G, Lmax, keep, recent;
