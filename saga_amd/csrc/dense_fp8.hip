@@ -9,7 +9,7 @@
 //   * x[h, j] = (scale s_k) q_h . c_j: key rows straight from memory as the A operand, in the
 //     query's type;
 //   * softmax with a running reference and sum in fp32: the reference moves only when a score
-//     exceeds it by kSlack nats, so most steps exchange and rescale nothing;
+//     exceeds it by kFp8Slack nats, so most steps exchange and rescale nothing;
 //   * o[h, i] += sum_j (p_hj s_v) c_ji: p s_v of the head's own value head is split into two bf16 terms
 //     (16 bits: one would cost 2^-9 of each weight, as much as a bf16 output's own rounding),
 //     an MFMA each.  Lane (m, s) loads dims [m d / 16, + d / 16) of positions 8 s .. 8 s + 7 and
@@ -17,6 +17,11 @@
 //     MFMA e has dim m d / 16 + e in row m.
 // Kernel 2 joins the splits.  With weights per position asked for, a step's scores go to memory, and
 // kernel 2 has blocks that turn them into weights beside those that join.
+// Bound by the cache's bytes: 12 / 1 / 2 heads of 128, 32 x 65541 positions (806 MB) 146 us with its
+// join, 5.5 TB/s, 8 x 32769 (101 MB) 22.8 + 3.9 (one of 17 steps over four waves, two launches).  With
+// weights 192 + 24 at 32 x 65541: 100 MB of scores written between the reads (906 MB at 4.7 TB/s, where a
+// copy gets 5.1) and read; whole lines a store, stores past the caches and waits that leave the
+// stores out were the same 192.  Two blocks a CU: three or four spill.
 #include <algorithm>
 
 #include "dense_join.cuh"
