@@ -1644,6 +1644,10 @@ int evict_run(EvictParams& p, const saga_tensor* weights, const int32_t* kv_len,
   if (!workspace || workspace_bytes < static_cast<size_t>(lay.total))
     return fail(SAGA_ERR_WORKSPACE, "workspace of %zu bytes, need %lld", workspace_bytes, (long long)lay.total);
   if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(SAGA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  // (views that interleave without meeting are allowed, so that only the same tensors are told)
+  bool same = out && weights_out->data == weights->data;
+  for (const EvictRows& r : p.rows) same = same || (out && (r.src == r.dst || (p.fp8 && r.ss == r.ds)));
+  if (same) return fail(SAGA_ERR_INVALID, "results must not overlap the cache and its weights (null: in place)");
   char* ws = static_cast<char*>(workspace);
   const saga_tensor* wo = out ? weights_out : weights;
   p.w = static_cast<const float*>(weights->data);
@@ -1725,7 +1729,8 @@ int saga_norm_rope_kv_append_fp8(const saga_tensor* qkv, int64_t n_q, const floa
   if (!start) return fail(SAGA_ERR_INVALID, "start: null");
   if (rows < 1 || rows > kv.B) return fail(SAGA_ERR_INVALID, "rows: 1 to B required");
   if (!offsets && p.N % rows) return fail(SAGA_ERR_INVALID, "without offsets N must be a multiple of rows");
-  if ((p.N >> kv.shift) + 2 * rows >= (1LL << 24)) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
+  const int64_t threads = std::max<int64_t>(256, (1LL << kv.shift) * (kv.d / 16));  // of a block per positions that share a scale
+  if (((p.N >> kv.shift) + 2 * rows) * threads >= (1LL << 32)) return fail(SAGA_ERR_UNSUPPORTED, "sizes too large");
   p.kv = kv;
   p.start = start;
   p.offsets = offsets;

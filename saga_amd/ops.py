@@ -1021,7 +1021,7 @@ def evict_kv(k_cache, v_cache, weights, kv_len, keep, recent=0, out=None, kept=N
     common divisor of the key and value heads, each group of heads keeps positions of its own; equal weights: the lower
     position, NaN above all numbers).  Kept positions below keep - recent stay where they are, the gaps there take the
     others in their order, the last `recent` follow.  Rows and weights move together.  In place (weights behind
-    min(kv_len, keep) become 0), or into out = (k, v, weights) of at least `keep` positions; kv_len is the caller's to
+    min(kv_len, keep) become 0), or into other tensors, out = (k, v, weights) of at least `keep` positions; kv_len is the caller's to
     cut to `keep`.  Returns kept int32 [B, G, keep]: the position that each place held before, -1 behind kv_len."""
     k_out, v_out, w_out = out if out is not None else (None, None, None)
     dev = _need_gpu(k_cache, v_cache, weights, kv_len, k_out, v_out, w_out, kept)

@@ -152,15 +152,21 @@ int main(int argc, char** argv) {
         const int64_t Lo = keep > 0 && keep < 100000 ? keep + static_cast<int64_t>(next() % 3) : 5;
         saga_tensor wt = spoil(contig(SAGA_DTYPE_F32, {B, G, Lw})), wo = spoil(contig(SAGA_DTYPE_F32, {B, G, Lo}));
         const bool out = next() % 2, odd = next() % 16 == 0;
+        const auto away = [](saga_tensor& t) {  // results lie elsewhere, mostly
+          if (t.data && next() % 16) t.data = reinterpret_cast<void*>(reinterpret_cast<uintptr_t>(t.data) + (1u << 24));
+        };
+        away(wo);
         const int32_t* len = next() % 8 ? idx : nullptr;
         int32_t* kept = next() % 8 ? idx : nullptr;
         if (which == 5) {
           saga_tensor k = spoil(contig(dt, {B, n_k, L, d})), v = spoil(contig(dt, {B, n_v, L, d}));
           saga_tensor ko = spoil(contig(dt, {B, n_k, Lo, d})), vo = spoil(contig(dt, {B, n_v, Lo, d}));
+          away(ko), away(vo);
           rc = saga_evict_kv(&k, &v, &wt, len, keep, recent, out ? &ko : nullptr, out != odd ? &vo : nullptr,
                              out ? &wo : nullptr, kept, w, ws_bytes, nullptr);
         } else {
-          const saga_kv_fp8 co = cache(B, n_k, n_v, Lo, d, block);
+          saga_kv_fp8 co = cache(B, n_k, n_v, Lo, d, block);
+          for (saga_tensor* t : {&co.k_codes, &co.k_scales, &co.v_codes, &co.v_scales}) away(*t);
           rc = saga_evict_kv_fp8(cp, &wt, len, keep, recent, out ? &co : nullptr, out != odd ? &wo : nullptr, kept, w, ws_bytes,
                                  nullptr);
         }

@@ -206,6 +206,37 @@ def test_evict_result_refusals():
     assert call8(_cache(L=10), None) == -1 and "null" in _err()
 
 
+def test_evictions_into_their_own_tensors_are_refused():
+    """Rows would be overwritten before they are read: in place is the null results' form."""
+    lib = _lib.load()
+    at = iter(range(1 << 24, 1 << 30, 1 << 24))
+    new = lambda shape, dt=_lib.DTYPE_BF16: _t(shape, dt, data=next(at))
+    F32, U8 = _lib.DTYPE_F32, _lib.DTYPE_U8
+    w, wo, k, v = new((2, 1, 48), F32), new((2, 1, 48), F32), new((2, 1, 48, 128)), new((2, 2, 48, 128))
+    ko, vo = new((2, 1, 48, 128)), new((2, 2, 48, 128))
+    for kk, vv, ww in ((k, vo, wo), (ko, v, wo), (ko, vo, w), (k, v, w)):
+        assert lib.saga_evict_kv(_r(k), _r(v), _r(w), 0x300000, 10, 2, _r(kk), _r(vv), _r(ww), 0x300000, 0x200000, 1 << 30, None) == -1
+        assert "must not overlap" in _err()
+    parts = lambda: dict(k_codes=new((2, 1, 48, 128), U8), k_scales=new((2, 1, 2), F32), v_codes=new((2, 2, 48, 128), U8),
+                         v_scales=new((2, 2, 2), F32))
+    src, dst = parts(), parts()
+    for name in (*src, None):
+        co = _cache(**{**dst, **({name: src[name]} if name else {})})
+        rc = lib.saga_evict_kv_fp8(_r(_cache(**src)), _r(w), 0x300000, 10, 2, _r(co), _r(wo if name else w), 0x300000, 0x200000,
+                                   1 << 30, None)
+        assert rc == -1 and "must not overlap" in _err(), name
+
+
+def test_appends_refuse_more_rows_than_a_launch_holds():
+    """Less than 2^32 threads: blocks of 1024 where 128 positions of 128 dims share a scale."""
+    lib = _lib.load()
+    for rows, block in (((1 << 21) - 1, 128), ((1 << 23) - 1, 32)):
+        qkv, q = _t((rows, 4 * 64 if block == 32 else 4 * 128), strides=(0, 1)), _t((rows, 1, 64 if block == 32 else 128))
+        c = _cache(B=rows, L=256, d=64 if block == 32 else 128, block=block)
+        assert lib.saga_norm_rope_kv_append_fp8(_r(qkv), 1, 0x300000, None, None, 1e-6, 0x300000, 0x300000, rows, _r(q), _r(c),
+                                                None) == -2 and "sizes too large" in _err()
+
+
 def test_attention_weights_refusals():
     lib = _lib.load()
     q, k, w = _t((2, 12, 1, 128)), _t((2, 2, 48, 128)), _t((2, 2, 48), _lib.DTYPE_F32)
