@@ -30,7 +30,6 @@ hipError_t launch_attention_weights(const WeightsParams& p, hipStream_t st) {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
-constexpr int kSelNear = 2048;
 
 template <int SEG>
 struct SelShared {
@@ -39,7 +38,6 @@ struct SelShared {
   int cnt[kSelWaves];
   int sel_bin, sel_above, sel_cnt;
   int sums[4][kSelWaves];
-  uint32_t near[kSelNear];  // keys of the H-th largest's bin
 };
 
 // A weight as what it is ranked by: any NaN above all numbers, -0 as 0; never 0, which stands for no position.
@@ -61,12 +59,11 @@ __device__ __forceinline__ uint32_t bits_below(int end, int p0) {
 
 // One block per (batch row, group), a segment of SEG positions' ranking keys in LDS (a row of one
 // segment is read once, longer ones for every pass).  The H-th largest key by radix (11, 11, 10
-// bits), equal ones by position: the first digits are counted as the row is read; the other two
-// over the few keys that share the H-th's, if they are few and the row is one segment, else
-// over all.  What is large of 32 positions is one mask, a thread's: every prefix of the selection
-// is one scan of the block.  The result is, per 32 places below H, the mask of their gaps and
-// the first one's rank, and the positions that move there in order; what to do with them is the
-// moving blocks' work, of which there are many.
+// bits), equal ones by position: the first digits are counted as the row is read; the other two, of a
+// row of one segment, over the keys that share the H-th's.  What is large of 32 positions is one
+// mask, a thread's: every prefix of the selection is one scan of the block.  The result is, per 32
+// places below H, the mask of their gaps and the first one's rank, and the positions that move there
+// in order; what to do with them is the moving blocks' work, of which there are many.
 // One CU's work: 8 x 32769 positions 18.8 us, of which the row's 128 KB take 5 (what one CU gets from
 // memory; 16 or 32 loads in flight for 8, or 16 bytes each, no less), 20 rows of 8195 15.5.  Measured
 // before: 82 us with keys in registers and code unrolled over them, 36 with three digits over all
@@ -156,7 +153,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
 
   uint32_t T = 0xffffffffu;  // the H-th largest key
   int need = 0;              // of those equal to it, the first `need` stay
-  bool few = false;          // gt and eq hold the row's masks already
+  bool held = false;         // gt and eq hold the row's masks already
   for (int i = tid; i < 2048; i += kSelThreads) sh.hist[i] = 0;
   lds_sync();
   {
@@ -176,37 +173,31 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
     hist_pick<kSelThreads>(sh, 2048, need, bin, above, count);
     uint32_t prefix = static_cast<uint32_t>(bin) << 21;
     need -= above;
-    few = nseg == 1 && count <= kSelNear;
-    int listed = 0;
-    if (few) {
-      masks(0, prefix, prefix | 0x1fffffu);
-      const int at = wave_part(__popc(eq), 0);
-      lds_sync();
-      int k = at + block_part(0, listed);
-      for (uint32_t m = eq; m; m &= m - 1) sh.near[k++] = key_of(__builtin_ctz(m));
-    }
+    held = nseg == 1;
+    if (held) masks(0, prefix, prefix | 0x1fffffu);
 #pragma unroll 1
     for (int pass = 1; pass < 3; ++pass) {
       const int shift = pass == 1 ? 10 : 0, nb = pass == 1 ? 2048 : 1024;
       const uint32_t hmask = pass == 1 ? 0xffe00000u : 0xfffffc00u;
       for (int i = tid; i < 2048; i += kSelThreads) sh.hist[i] = 0;
       lds_sync();
-      if (few) {
-        for (int i = tid; i < listed; i += kSelThreads) {
-          const uint32_t key = sh.near[i];
-          if (((key ^ prefix) & hmask) == 0u) atomicAdd(&sh.hist[(key >> shift) & (nb - 1)], 1);
-        }
+      int zeros = 0;
+      auto count_key = [&](uint32_t key) {
+        const bool zero = key == kZero;
+        zeros += zero ? 1 : 0;
+        if ((((key ^ prefix) & hmask) | (zero ? 1u : 0u)) == 0u) atomicAdd(&sh.hist[(key >> shift) & (nb - 1)], 1);
+      };
+      if (held) {
+        for (uint32_t m = eq; m; m &= m - 1) count_key(key_of(__builtin_ctz(m)));
       } else {
-        int zeros = 0;
         for (int seg = 0; seg < nseg; ++seg) {
-          if (nseg > 1) load(seg, [](uint32_t) {});
-          each(seg, [&](uint32_t key) {
-            const bool zero = key == kZero;
-            zeros += __popcll(__ballot(zero));
-            if ((((key ^ prefix) & hmask) | (zero ? 1u : 0u)) == 0u) atomicAdd(&sh.hist[(key >> shift) & (nb - 1)], 1);
-          });
+          load(seg, [](uint32_t) {});
+          each(seg, count_key);
         }
-        if (((kZero ^ prefix) & hmask) == 0 && lane == 0 && zeros) atomicAdd(&sh.hist[(kZero >> shift) & (nb - 1)], zeros);
+      }
+      if (((kZero ^ prefix) & hmask) == 0) {
+        zeros = wave_incl_scan(zeros, lane);
+        if (lane == kWave - 1 && zeros) atomicAdd(&sh.hist[(kZero >> shift) & (nb - 1)], zeros);
       }
       lds_sync();
       hist_pick<kSelThreads>(sh, nb, need, bin, above, count);
@@ -214,7 +205,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
       need -= above;
     }
     T = prefix;
-    if (few) {  // of the H-th's bin: above T, and T
+    if (held) {  // of the H-th's bin: above T, and T
       uint32_t same = 0;
       for (uint32_t m = eq; m; m &= m - 1) {
         const uint32_t key = key_of(__builtin_ctz(m));
@@ -233,7 +224,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
       load(seg, [](uint32_t) {});
       lds_sync();
     }
-    if (!few) masks(seg, T, T);
+    if (!held) masks(seg, T, T);
     const int p0 = seg * SEG + tid * 32, ne = __popc(eq), eq_at = wave_part(ne, 1);
     lds_sync();
     int all;
