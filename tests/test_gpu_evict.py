@@ -230,7 +230,7 @@ def test_evict_selection(kind, keep, recent):
 @pytest.mark.parametrize("L", [8192, 8193, 33000, 65536, 65537, 150001])
 @pytest.mark.parametrize("kind", ["random", "zeros", "special"])
 def test_evict_long_rows(L, kind):
-    """Lengths around what a selection holds in registers."""
+    """Lengths around what a selection holds at a time (32768 positions), and several of it."""
     g = _gen(L)
     w = _random_weights(g, kind, 2, 1, L)
     k, v = _randn(g, 2, 1, L, 64, dtype=torch.float16), _randn(g, 2, 1, L, 64, dtype=torch.float16)
