@@ -33,13 +33,6 @@
 
 namespace saga {
 
-// Wave-local LDS ordering: a wave's scales are private to it.
-__device__ __forceinline__ void q4_wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // N bytes (2, 4, 8 or 16) at an address aligned to them, as dwords (2 bytes in the low half).
 template <int N>
 struct Bytes {
@@ -265,7 +258,7 @@ __global__ void __launch_bounds__(256, 2) dense_q4_kernel(DenseQ4Params p) {
     for (int u = 0; u < NV; ++u) {
       r.sv[u].store(slds + 32 * SB * (1 + u) + (lane >> 1) * SB + (SB / 2) * (lane & 1));
     }
-    q4_wave_sync();
+    wave_sync();  // (a wave's scales are private to it)
     float x[8];  // positions c0 + 4 i + s
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -369,7 +362,7 @@ __global__ void __launch_bounds__(256, 2) dense_q4_kernel(DenseQ4Params p) {
         tile(4 * hv + 2, u32x4{q4_pair<2>(two[0], qc), q4_pair<2>(two[1], qc), q4_pair<2>(two[2], qc), q4_pair<2>(two[3], qc)});
         tile(4 * hv + 3, u32x4{q4_pair<3>(two[0], qc), q4_pair<3>(two[1], qc), q4_pair<3>(two[2], qc), q4_pair<3>(two[3], qc)});
       }
-    q4_wave_sync();  // the scales are rewritten by this wave's next step
+    wave_sync();  // the scales are rewritten by this wave's next step
   };
 
   for (int it = w; it < nstep; it += 8) {

@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
       }
     }
   };
-  // f(key) of the segment's positions, a wave's those that it has read
+  // f(key) of the segment's positions, a wave's those that it has read (between wave_syncs: other lanes of it wrote them)
   auto each = [&](int seg, auto f) {
     for (int j0 = 0; j0 < min(SEG, nc - seg * SEG); j0 += 4 * kSelThreads) {
       uint32_t key[4];
@@ -192,7 +192,9 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
       } else {
         for (int seg = 0; seg < nseg; ++seg) {
           load(seg, [](uint32_t) {});
+          wave_sync();
           each(seg, count_key);
+          wave_sync();  // (the next segment's keys overwrite them)
         }
       }
       if (((kZero ^ prefix) & hmask) == 0) {
