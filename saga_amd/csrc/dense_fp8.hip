@@ -10,9 +10,10 @@
 //     query's type;
 //   * softmax with a running reference and sum in fp32: the reference moves only when a score
 //     exceeds it by kFp8Slack nats, so most steps exchange and rescale nothing;
-//   * o[h, i] += sum_j (p_hj s_v) c_ji: p s_v of the head's own value head is split into two bf16 terms
-//     (16 bits: one would cost 2^-9 of each weight, as much as a bf16 output's own rounding),
-//     an MFMA each.  Lane (m, s) loads dims [m d / 16, + d / 16) of positions 8 s .. 8 s + 7 and
+//   * o[h, i] += sum_j (p_hj s_v) c_ji: p s_v of the head's own value head is split into three bf16 terms,
+//     which hold its 24 bits, an MFMA each (a third term under the loads: 22.8 -> 22.9 us at 8 x 32769,
+//     193.5 -> 194.8 with weights at 32 x 65541; two were off by 2.4e-6 of an f32 output, 16 of its
+//     bits).  Lane (m, s) loads dims [m d / 16, + d / 16) of positions 8 s .. 8 s + 7 and
 //     pairs neighbouring positions with byte permutes, so that values pass through no LDS;
 //     MFMA e has dim m d / 16 + e in row m.
 // Kernel 2 joins the splits.  With weights per position asked for, a step's scores go to memory, and
@@ -230,9 +231,9 @@ __global__ void __launch_bounds__(256, 2) dense_fp8_kernel(DenseFp8Params p) {
       l_run += x[i];
       x[i] *= r.sv;
     }
-    u32x4 pf[2];
+    u32x4 pf[3];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 3; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i) pf[k][i] = fp8_split(x[2 * i], x[2 * i + 1]);
 #pragma unroll
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(256, 2) dense_fp8_kernel(DenseFp8Params p) {
           }
           const int e = 4 * c + 2 * half;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
+          for (int k = 0; k < 3; ++k) {
             o[u][e] = mfma_16b<SAGA_DTYPE_BF16>(a, pf[k], o[u][e]);
             o[u][e + 1] = mfma_16b<SAGA_DTYPE_BF16>(b, pf[k], o[u][e + 1]);
           }
