@@ -502,7 +502,9 @@ int saga_unpack_gemv_q4(const saga_unpack_q4_item* items, int32_t n, saga_stream
  * [B, n_k, Lmax, d] and [B, n_v, Lmax, d] the rows [batch[n], :, pos[n]] (batch
  * == NULL: token n is batch row n).  A pos or batch index out of range writes no
  * cache row and NaN queries.  The (batch, pos) of a call's tokens must differ
- * from each other. */
+ * from each other.  In fp32: of magnitudes whose squares sum past fp32 (2^60
+ * and more) a norm leaves 0, and where they sum to 0 (2^-75 and less) with eps 0
+ * no number. */
 int saga_norm_rope_kv_append(const saga_tensor* qkv, int64_t n_q, const float* rope_table, const saga_tensor* q_norm,
                              const saga_tensor* k_norm, float eps, const int32_t* pos, const int32_t* batch,
                              saga_tensor* q_out, saga_tensor* k_cache, saga_tensor* v_cache, saga_stream_t stream);
@@ -527,7 +529,8 @@ typedef struct saga_kv_fp8 {
 } saga_kv_fp8;
 
 /* saga_norm_rope_kv_append into an 8-bit cache, keys and values rounded from
- * the exact operations on qkv's numbers (keys: from fp64).  Batch row i of the
+ * the exact operations on qkv's numbers (keys: from fp64, whatever their
+ * magnitudes; queries from fp32, as there).  Batch row i of the
  * first `rows` takes tokens offsets[i] .. offsets[i + 1] - 1 (device int32
  * [rows + 1], from 0 to N, ascending; NULL: N / rows tokens each) at positions
  * start[i], start[i] + 1, ... (device int32 [rows]).  A token at a block's first

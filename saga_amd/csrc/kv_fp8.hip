@@ -117,8 +117,9 @@ __device__ __forceinline__ void norm_rope(float (&x)[2][8], bool normed, const f
 
 // The same for keys on their way to e4m3, in double and rounded to odd floats, so that they round as
 // the formula's values do (fp32 moves one in 2^19 across a rounding's border, and whoever reads
-// the cache sees 2^-3 of it).  EXACT: products of two numbers of x's and w's type are floats.
-template <int D, bool EXACT>
+// the cache sees 2^-3 of it).  F16: products of two f16 numbers are floats (22 bits from 2^-48 to 2^32);
+// those of bf16 numbers leave a float's range.
+template <int D, bool F16>
 __device__ __forceinline__ void norm_rope_exact(float (&x)[2][8], bool normed, const float (&w)[2][8], float eps, const Rotations& rot) {
   double r = 1.0;
   if (normed) {
@@ -127,7 +128,7 @@ __device__ __forceinline__ void norm_rope_exact(float (&x)[2][8], bool normed, c
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if constexpr (EXACT) sq += static_cast<double>(x[i][e] * x[i][e]);
+        if constexpr (F16) sq += static_cast<double>(x[i][e] * x[i][e]);
         else sq = __builtin_fma(static_cast<double>(x[i][e]), static_cast<double>(x[i][e]), sq);
       }
     r = 1.0 / sqrt(head_sum<D / 16>(sq) / D + static_cast<double>(eps));
@@ -137,8 +138,13 @@ __device__ __forceinline__ void norm_rope_exact(float (&x)[2][8], bool normed, c
     double y[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if constexpr (EXACT) y[i] = normed ? x[i][e] * w[i][e] : x[i][e];
-      else y[i] = normed ? static_cast<double>(x[i][e]) * static_cast<double>(w[i][e]) : static_cast<double>(x[i][e]);
+      if constexpr (F16) {
+        y[i] = normed ? x[i][e] * w[i][e] : x[i][e];
+      } else {
+        float xe = x[i][e], we = w[i][e];
+        asm volatile("" : "+v"(xe), "+v"(we));  // (doubles made here: those of the sum, or of the norm ahead of the heads, cost 40 registers)
+        y[i] = normed ? static_cast<double>(xe) * static_cast<double>(we) : static_cast<double>(xe);
+      }
     }
     const double cs = rot.r[e / 2][2 * (e & 1)], sn = rot.r[e / 2][2 * (e & 1) + 1];
     x[0][e] = odd_float(__builtin_fma(y[0], cs, -(y[1] * sn)) * r);
@@ -232,7 +238,7 @@ __global__ void __launch_bounds__(256) norm_rope_kv_append_kernel(NormRopeParams
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[i][e] = is_q ? w[i][e] : wk[i][e];
       const bool normed = is_q ? p.q_norm != nullptr : p.k_norm != nullptr;
-      if constexpr (FP8) norm_rope_exact<D, VT != 0>(x, normed, w, p.eps, rot);
+      if constexpr (FP8) norm_rope_exact<D, VT == SAGA_DTYPE_F16>(x, normed, w, p.eps, rot);
       else norm_rope<D>(x, normed, w, p.eps, rot);
     }
     if (is_q) {
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__((AppendShape<D, S>::NT)) norm_rope_kv_append_f
       if (live && mine) store_query<VT, D>(p, n, hh, t, ok, x);
     } else if (!is_v) {
       norms.k.open(nw);
-      norm_rope_exact<D, VT != 0>(x, p.k_norm != nullptr, nw, p.eps, rot);
+      norm_rope_exact<D, VT == SAGA_DTYPE_F16>(x, p.k_norm != nullptr, nw, p.eps, rot);
     }
     if (min(hb + HS, h1) <= p.n_q) continue;  // the whole block holds queries
     const Fp8Head c = fp8_head(p.kv, is_v, row, is_q ? 0 : hh - p.n_q - (is_v ? p.n_k : 0));
