@@ -538,7 +538,10 @@ typedef struct saga_kv_fp8 {
  * tokens leave the scale while they are at most 448 s in magnitude; beyond,
  * it is set anew by the call's tokens and the positions before them are
  * rounded to it.  What a block holds behind a call's last token is lost.  A row
- * whose positions are not all in [0, Lmax) writes nothing and NaN queries. */
+ * cut to fewer positions later keeps a scale that was raised and what was
+ * rounded to it: to come back to a row's end inside a block, keep that block's
+ * codes and scales.  A row whose positions are not all in [0, Lmax) writes
+ * nothing and NaN queries. */
 int saga_norm_rope_kv_append_fp8(const saga_tensor* qkv, int64_t n_q, const float* rope_table,
                                  const saga_tensor* q_norm, const saga_tensor* k_norm, float eps,
                                  const int32_t* start, const int32_t* offsets, int64_t rows, saga_tensor* q_out,

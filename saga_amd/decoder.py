@@ -31,7 +31,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, replace
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -204,6 +204,7 @@ class SagaDecoder:
         self.graph_cal: Optional[torch.cuda.CUDAGraph] = None
         self.graph_fast: Optional[torch.cuda.CUDAGraph] = None
         self.prompt_len = 0
+        self._tail: Tuple[torch.Tensor, ...] = ()
 
     # (attribute, shape as a function of the decoder shape) of every weight
     _WEIGHT_SHAPES = {
@@ -444,7 +445,9 @@ class SagaDecoder:
             c[:, 1:, :, :T] = c[:, 0:1, :, :T]
         self._evicted = False
         self.prompt_len = T
+        self._tail = ()
         self.reset()
+        self._tail = tuple(t.clone() for t in self._tail_views())
         self._first_token = first
         self.tokens.fill_(0)
         self.tokens.copy_(first.expand(self.batch))
@@ -472,7 +475,9 @@ class SagaDecoder:
         self._evicted = False
         self.prompt_len = prompt_len
         self._first_token = torch.zeros(1, dtype=torch.int64, device=self.device)
+        self._tail = ()
         self.reset()
+        self._tail = tuple(t.clone() for t in self._tail_views())
 
     def _fill_synthetic_held(self, prompt_len: int, g: torch.Generator) -> None:
         s, d, B = self.shape, self.shape.head_dim, self.batch
@@ -488,10 +493,21 @@ class SagaDecoder:
                 else:
                     ops.rope_kv_append_q4(x, 1, unrotated, pos, self.kv.layer(l), batch=rows)
 
+    def _tail_views(self) -> Tuple[torch.Tensor, ...]:
+        """The prompt's rows and scales in a block of an 8-bit cache that a prompt ends inside: a step's token there may
+        raise the block's scale, which rounds them again."""
+        n, block = self.prompt_len, self.kv_fp8_block
+        if not block or n % block == 0:
+            return ()
+        b = n // block
+        return tuple(t[..., b * block:n, :] if t.dtype == torch.uint8 else t[..., b] for t in self.kv.tensors)
+
     def reset(self) -> None:
         """Rewind the decode state to just after the prompt."""
         if self._evicted:
             raise RuntimeError("reset: positions of the prompt were evicted from the bounded cache (prefill again)")
+        for view, held in zip(self._tail_views(), self._tail):
+            view.copy_(held)
         self._used = self.prompt_len
         if self.kv_budget:
             self.slot.fill_(self.prompt_len)
