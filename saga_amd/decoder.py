@@ -37,8 +37,8 @@ import torch
 
 from . import ops
 from .attention.attention import sdpa_attention_forward
-from .kv_cache import (KVCache, check_fp8_decoder, check_q4_decoder, kv_cache_bytes, projection_shapes,  # noqa: F401  (kv_cache_bytes re-exported)
-                       skinny_gemm_supported)
+from .kv_cache import (MAX_GROUP, KVCache, check_bounded_decoder, check_fp8_decoder, check_q4_decoder, kv_cache_bytes,  # noqa: F401  (kv_cache_bytes re-exported)
+                       projection_shapes, skinny_gemm_supported)
 
 
 @dataclass(frozen=True)
@@ -131,10 +131,9 @@ class SagaDecoder:
         check_fp8_decoder(shape, dtype, kv_fp8_block, kv_bits)
         if kv_fp8_block and mode != "dense":
             raise ValueError("kv_fp8_block needs mode 'dense'")
-        if kv_budget and (mode != "dense" or kv_bits != 16 or shape.head_dim not in (64, 128)):
-            raise ValueError("kv_budget needs mode 'dense', 16- or 8-bit caches and a head dim of 64 or 128")
-        if (kv_budget or kv_recent) and not (0 < kv_budget < max_len and 0 <= kv_recent <= kv_budget):
-            raise ValueError("kv_budget must lie between 1 and max_len - 1, kv_recent between 0 and kv_budget")
+        if kv_budget and mode != "dense":
+            raise ValueError("kv_budget needs mode 'dense'")
+        check_bounded_decoder(shape, max_len, kv_bits, kv_fp8_block, kv_budget, kv_recent)
         self.kv_bits, self.weight_bits, self.weight_group = kv_bits, weight_bits, weight_group
         self.kv_fp8_block, self.kv_budget, self.kv_recent = kv_fp8_block, kv_budget, kv_recent
         self.shape, self.batch, self.max_len, self.mode, self.top_n = shape, batch, max_len, mode, top_n
@@ -457,7 +456,9 @@ class SagaDecoder:
         T, n = q.shape[0], min(self.PROMPT_QUERIES, q.shape[0])
         seen = torch.arange(T - n + 1, T + 1, device=self.device, dtype=torch.int32)
         w = torch.empty(n, self.kv_weights.shape[2], T, device=self.device)
-        ops.attention_weights(q[T - n:].unsqueeze(2), k.expand(n, -1, -1, -1), w, kv_len=seen, add=False)
+        q, k = q[T - n:].unflatten(1, (self.shape.n_k, -1)), k.expand(n, -1, -1, -1)
+        for h in range(0, q.shape[2], MAX_GROUP):  # (more query heads of a key head only over 8-bit caches)
+            ops.attention_weights(q[:, :, h:h + MAX_GROUP].flatten(1, 2).unsqueeze(2), k, w, kv_len=seen, add=h > 0)
         self._prompt_weights[l] = 0.0
         self._prompt_weights[l, :, :, :T] = w.sum(0)
 

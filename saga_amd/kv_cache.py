@@ -27,6 +27,7 @@ from typing import Optional
 import torch
 
 HBM_BYTES_MI355X = 288 * 10**9
+MAX_GROUP = 16  # query heads per key head that ops.attention_weights takes, as all attention over 16-bit caches
 
 
 def _es(dtype) -> int:
@@ -53,6 +54,16 @@ def check_fp8_decoder(shape, dtype, kv_fp8_block: int, kv_bits: int = 16) -> Non
             raise ValueError("kv_fp8_block needs bf16 or f16")
     if shape.qk_norm and (shape.head_dim not in (64, 128) or kv_bits != 16):
         raise ValueError("norms of queries and keys need a head dim of 64 or 128 and 16- or 8-bit caches")
+
+
+def check_bounded_decoder(shape, max_len: int, kv_bits: int, kv_fp8_block: int, kv_budget: int, kv_recent: int) -> None:
+    """ValueError for a bounded cache that SagaDecoder does not take."""
+    if kv_budget and (kv_bits != 16 or shape.head_dim not in (64, 128)):
+        raise ValueError("kv_budget needs 16- or 8-bit caches and a head dim of 64 or 128")
+    if kv_budget and not kv_fp8_block and shape.n_q > MAX_GROUP * shape.n_k:
+        raise ValueError(f"kv_budget over 16-bit caches takes at most {MAX_GROUP} query heads per key head")
+    if (kv_budget or kv_recent) and not (0 < kv_budget < max_len and 0 <= kv_recent <= kv_budget):
+        raise ValueError("kv_budget must lie between 1 and max_len - 1, kv_recent between 0 and kv_budget")
 
 
 def _check_fp8_rows(d: int, block: int) -> None:
