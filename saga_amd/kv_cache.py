@@ -21,6 +21,7 @@ GPU next to the decode weights and workspaces: an MI355X has 288 GB of HBM3E.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -128,7 +129,7 @@ def decode_weight_bytes(shape, dtype=torch.bfloat16, decode_copies: bool = True,
     es = _es(dtype)
     s = shape
     per_layer = (s.qkv_width * s.hidden + s.qkv_width + s.hidden * s.n_q * s.head_dim + 2 * s.intermediate * s.hidden
-                 + s.hidden * s.intermediate + 2 * s.hidden)
+                 + s.hidden * s.intermediate + 2 * s.hidden + (2 * s.head_dim if s.qk_norm else 0))
     base = (s.vocab * s.hidden + s.layers * per_layer + s.hidden) * es
     if not decode_copies:
         return base
@@ -141,17 +142,20 @@ def decode_weight_bytes(shape, dtype=torch.bfloat16, decode_copies: bool = True,
 
 
 def decode_workspace_bytes(shape, batch: int, max_len: int, top_n: int, kv_bits: int = 16,
-                           weight_bits: int = 16, kv_fp8_block: int = 0) -> int:
+                           weight_bits: int = 16, kv_fp8_block: int = 0, kv_budget: int = 0, kv_recent: int = 0,
+                           dtype=torch.bfloat16) -> int:
     """Atop-N and dense decode workspaces of one layer call (shared by all
     layers; a 4- or 8-bit cache: its dense workspace), the projections' (of 16-
-    or 4-bit weights), plus the per-step activations and the threshold table."""
+    or 4-bit weights), plus the per-step activations and the threshold table;
+    of a bounded cache besides the weights that its positions (and a prompt's)
+    gathered, the workspaces that gather them, and the eviction's."""
     from . import _lib
     lib = _lib.load()
     s = shape
     if kv_bits == 4:
         ws = lib.saga_dense_q4_workspace_bytes(batch, s.n_q, max_len, s.head_dim)
     elif kv_fp8_block:
-        ws = lib.saga_dense_fp8_workspace_bytes(batch, s.n_q, max_len, s.head_dim, 0)
+        ws = lib.saga_dense_fp8_workspace_bytes(batch, s.n_q, max_len, s.head_dim, 1 if kv_budget else 0)
     else:
         ws = lib.saga_atopn_workspace_bytes(batch, s.n_q, s.n_k, max_len, s.head_dim, min(2 * top_n, max_len))
         ws += lib.saga_dense_workspace_bytes(batch, s.n_q, max_len, s.head_dim)
@@ -159,6 +163,12 @@ def decode_workspace_bytes(shape, batch: int, max_len: int, top_n: int, kv_bits:
         ws += max(lib.saga_gemv_q4_workspace_bytes(batch, n, k) for n, k in projection_shapes(s))
     else:
         ws += lib.saga_gemv_workspace_bytes(batch, s.hidden, s.intermediate)
+    if kv_budget:
+        G, row = math.gcd(s.n_k, s.n_v), s.head_dim * (1 if kv_fp8_block else _es(dtype))
+        ws += 2 * s.layers * batch * G * max_len * 4
+        ws += lib.saga_evict_workspace_bytes(batch, G, kv_budget, kv_recent, s.n_k + s.n_v, row, 1)
+        if not kv_fp8_block:
+            ws += lib.saga_attention_weights_workspace_bytes(batch, s.n_q, s.n_k, max_len)
     ws += s.layers * batch * s.n_q * 4
     ws += batch * (3 * s.hidden + s.qkv_width + 2 * s.intermediate + s.vocab) * 2
     return int(ws)
@@ -188,7 +198,7 @@ def plan_capacity(shape, batch: Optional[int] = None, max_len: Optional[int] = N
                   reserve_fraction: float = 0.05, top_n: int = 512, dtype=torch.bfloat16,
                   align: int = 256, kv_bits: int = 16, weight_bits: int = 16, group: int = 64,
                   kv_group: Optional[int] = None, weight_group: Optional[int] = None,
-                  kv_fp8_block: int = 0) -> CapacityPlan:
+                  kv_fp8_block: int = 0, kv_budget: int = 0, kv_recent: int = 0) -> CapacityPlan:
     """The largest max_len for a given batch, or the largest batch for a given
     max_len (give exactly one), that fits budget_bytes (default: the current
     device's total memory, else 288 GB) minus reserve_fraction, next to the
@@ -196,13 +206,15 @@ def plan_capacity(shape, batch: Optional[int] = None, max_len: Optional[int] = N
     rounded down to a multiple of `align` positions.  kv_bits, weight_bits:
     caches and decode copies in 4 bits, in groups of kv_group and weight_group
     (`group` where not given); kv_fp8_block: caches in 8 bits, in blocks of so
-    many positions; what SagaDecoder refuses is refused, and a batch searched
-    for ends at the 32 rows that 4-bit weights take."""
+    many positions; kv_budget, kv_recent: a bounded cache of max_len places;
+    what SagaDecoder refuses is refused, and a batch searched for ends at the
+    32 rows that 4-bit weights take."""
     if (batch is None) == (max_len is None):
         raise ValueError("give exactly one of batch and max_len")
     kv_group, weight_group = kv_group or group, weight_group or group
     check_q4_decoder(shape, batch or 1, dtype, kv_bits, kv_group, weight_bits, weight_group)
     check_fp8_decoder(shape, dtype, kv_fp8_block, kv_bits)
+    check_bounded_decoder(shape, 1 << 30 if max_len is None else max_len, kv_bits, kv_fp8_block, kv_budget, kv_recent)
     if budget_bytes is None:
         budget_bytes = (torch.cuda.get_device_properties(0).total_memory if torch.cuda.is_available()
                         else HBM_BYTES_MI355X)
@@ -213,7 +225,7 @@ def plan_capacity(shape, batch: Optional[int] = None, max_len: Optional[int] = N
         if weight_bits == 4 and b > 32:
             return None
         kv = kv_cache_bytes(shape, b, L, dtype, kv_bits, kv_group, kv_fp8_block)
-        ws = decode_workspace_bytes(shape, b, L, top_n, kv_bits, weight_bits, kv_fp8_block)
+        ws = decode_workspace_bytes(shape, b, L, top_n, kv_bits, weight_bits, kv_fp8_block, kv_budget, kv_recent, dtype)
         if kv + wbytes + ws > avail:
             return None
         return CapacityPlan(b, L, kv, wbytes, ws, budget_bytes)
@@ -230,6 +242,8 @@ def plan_capacity(shape, batch: Optional[int] = None, max_len: Optional[int] = N
             else:
                 hi = mid
         best = fits(batch, lo * align) if lo > 0 else None
+        if best is not None and kv_budget >= best.max_len:
+            raise MemoryError(f"no cache of more than kv_budget {kv_budget} positions fits (at most {best.max_len})")
     else:
         lo, hi = 0, 1
         while fits(hi, max_len) is not None and hi < (1 << 20):
