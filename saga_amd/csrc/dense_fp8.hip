@@ -11,18 +11,17 @@
 //   * softmax with a running reference and sum in fp32: the reference moves only when a score
 //     exceeds it by kFp8Slack nats, so most steps exchange and rescale nothing;
 //   * o[h, i] += sum_j (p_hj s_v) c_ji: p s_v of the head's own value head is split into three bf16 terms,
-//     which hold its 24 bits, an MFMA each (a third term under the loads: 22.8 -> 22.9 us at 8 x 32769,
-//     193.5 -> 194.8 with weights at 32 x 65541; two were off by 2.4e-6 of an f32 output, 16 of its
-//     bits).  Lane (m, s) loads dims [m d / 16, + d / 16) of positions 8 s .. 8 s + 7 and
+//     which hold its 24 bits, an MFMA each (the third, under the loads: 22.8 -> 23.0 us at 8 x 32769, 193.5 ->
+//     194.8 with weights at 32 x 65541; with two, f32 outputs there were off by 2.4e-6, now by 4.4e-7).  Lane (m, s) loads dims [m d / 16, + d / 16) of positions 8 s .. 8 s + 7 and
 //     pairs neighbouring positions with byte permutes, so that values pass through no LDS;
 //     MFMA e has dim m d / 16 + e in row m.
 // Kernel 2 joins the splits.  With weights per position asked for, a step's scores go to memory, and
 // kernel 2 has blocks that turn them into weights beside those that join.
-// Bound by the cache's bytes: 12 / 1 / 2 heads of 128, 32 x 65541 positions (806 MB) 146 us with its
-// join, 5.5 TB/s, 8 x 32769 (101 MB) 22.8 + 3.9 (one of 17 steps over four waves, two launches).  With
-// weights 192 + 24 at 32 x 65541: 100 MB of scores written between the reads (906 MB at 4.7 TB/s, where a
+// Bound by the cache's bytes: 12 / 1 / 2 heads of 128, 32 x 65541 positions (806 MB) 144 us with its
+// join, 5.6 TB/s, 8 x 32769 (101 MB) 23.2 + 4.0 (one of 17 steps over four waves, two launches).  With
+// weights 191 + 23 at 32 x 65541: 100 MB of scores written between the reads (906 MB at 4.7 TB/s, where a
 // copy gets 5.1) and read; whole lines a store, stores past the caches and waits that leave the
-// stores out were the same 192.  Two blocks a CU: three or four spill.
+// stores out were the same.  Two blocks a CU: three or four spill.
 #include <algorithm>
 
 #include "dense_join.cuh"

@@ -64,10 +64,10 @@ __device__ __forceinline__ uint32_t bits_below(int end, int p0) {
 // mask, a thread's: every prefix of the selection is one scan of the block.  The result is, per 32
 // places below H, the mask of their gaps and the first one's rank, and the positions that move there
 // in order; what to do with them is the moving blocks' work, of which there are many.
-// One CU's work: 8 x 32769 positions 18.8 us, of which the row's 128 KB take 5 (what one CU gets from
-// memory; 16 or 32 loads in flight for 8, or 16 bytes each, no less), 20 rows of 8195 15.5.  Measured
-// before: 82 us with keys in registers and code unrolled over them, 36 with three digits over all
-// keys, 22 with masks by ballots over 64 positions a wave.
+// One CU's work: 8 x 32769 positions 18.5 us, of which the row's 128 KB take 5 (what one CU gets from
+// memory; 16 or 32 loads in flight for 8, or 16 bytes each, no less), 20 rows of 8195 15.5; rows of several
+// segments, read four times, 57 (8 x 65541) and 107 (4 x 131072).  Measured before: 82 us with keys in
+// registers and code unrolled over them, 22 with masks by ballots over 64 positions a wave.
 template <int SEG>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p) {
   __shared__ SelShared<SEG> sh;
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
 // the end, and zeros for the weights behind.  PIECES: 16 bytes each of a row; a thread's are all in
 // flight while the scales are compared.
 // Bound by the rows, read once and written once: 8 x 16384 rows of 3 heads of 256 bytes (201 MB)
-// 43.5 us, 4.6 TB/s.
+// 43.9 us, 4.6 TB/s; in place, where the larger part stays, 27.8 + 5.6.
 constexpr int kMoveRows = 128;
 
 template <int PHASE, bool FP8, int PIECES>

@@ -6,9 +6,10 @@
 // the token's rotations; values are stored as they come.  T = d / 16 threads take a head, dims
 // 8 t .. and d / 2 + 8 t .., the rotary partners: the mean is a sum over T lanes, everything
 // else stays in a thread.  Bound by the projection read once and written once: 4001 tokens of 15 heads
-// of 128 (32.8 MB) 9.4 us, few tokens by a launch and two round trips (one token 2.5, 8 tokens into 8
-// bits 4.6); 8-bit appends of prompts besides by the keys' doubles and a barrier per head (9001 tokens
-// of 25 heads of 64, 52 MB, 19.1 us).
+// of 128 (32.8 MB) 9.3 us, few tokens by a launch and two round trips (one token 2.7, 8 tokens into 8
+// bits 4.6), 8-bit appends of prompts besides by the keys' doubles and a barrier per head (9001 tokens
+// of 25 heads of 64, 52 MB, 19.4 us).  A token that raises its block's scale rounds the rows before it one
+// after another: 8 tokens, the last of their blocks of 32, 64 or 128 positions, 17.6, 29.0 and 54.2 us.
 #include <algorithm>
 
 #include "fp8.cuh"
