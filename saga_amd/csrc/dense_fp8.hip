@@ -12,9 +12,10 @@
 //     exceeds it by kFp8Slack nats, so most steps exchange and rescale nothing;
 //   * o[h, i] += sum_j (p_hj s_v) c_ji: p s_v of the head's own value head is split into three bf16 terms,
 //     which hold its 24 bits, an MFMA each (the third, under the loads: 22.8 -> 23.0 us at 8 x 32769, 193.5 ->
-//     194.8 with weights at 32 x 65541; with two, f32 outputs there were off by 2.4e-6, now by 4.4e-7).  Lane (m, s) loads dims [m d / 16, + d / 16) of positions 8 s .. 8 s + 7 and
-//     pairs neighbouring positions with byte permutes, so that values pass through no LDS;
-//     MFMA e has dim m d / 16 + e in row m.
+//     194.8 with weights at 32 x 65541; with two, f32 outputs there were off by 2.4e-6, now by 4.4e-7).
+//     Lane (m, s) loads dims [m d / 16, + d / 16) of positions 8 s .. 8 s + 7 and pairs neighbouring
+//     positions with byte permutes, so that values pass through no LDS; MFMA e has dim m d / 16 + e
+//     in row m.
 // Kernel 2 joins the splits.  With weights per position asked for, a step's scores go to memory, and
 // kernel 2 has blocks that turn them into weights beside those that join.
 // Bound by the cache's bytes: 12 / 1 / 2 heads of 128, 32 x 65541 positions (806 MB) 144 us with its

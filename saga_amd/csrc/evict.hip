@@ -107,7 +107,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictParams p
       }
     }
   };
-  // f(key) of the segment's positions, a wave's those that it has read (between wave_syncs: other lanes of it wrote them)
+  // f(key) of the segment's positions, a wave's those that it has read (other lanes of it wrote them:
+  // between wave_syncs)
   auto each = [&](int seg, auto f) {
     for (int j0 = 0; j0 < min(SEG, nc - seg * SEG); j0 += 4 * kSelThreads) {
       uint32_t key[4];

@@ -143,7 +143,8 @@ __device__ __forceinline__ void norm_rope_exact(float (&x)[2][8], bool normed, c
         y[i] = normed ? x[i][e] * w[i][e] : x[i][e];
       } else {
         float xe = x[i][e], we = w[i][e];
-        asm volatile("" : "+v"(xe), "+v"(we));  // (doubles made here: those of the sum, or of the norm ahead of the heads, cost 40 registers)
+        // (doubles made here: those of the sum, or of the norm ahead of the heads' loop, cost 40 registers)
+        asm volatile("" : "+v"(xe), "+v"(we));
         y[i] = normed ? static_cast<double>(xe) * static_cast<double>(we) : static_cast<double>(xe);
       }
     }
